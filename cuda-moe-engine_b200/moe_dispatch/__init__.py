@@ -8,7 +8,8 @@ from importlib import import_module
 
 __version__ = "0.2.0+b200"
 __all__ = ["dispatch", "combine", "PackedTokens", "CudaWorkspace", "MoEBlock", "MoEConfig",
-           "MoEWeights", "make_weights", "capture_forward", "get_extension", "HostPipeline"]
+           "MoEWeights", "make_weights", "capture_forward", "get_extension", "HostPipeline",
+           "balance_loss", "route", "route_backward"]
 _EXPORTS = {
     "dispatch": (".ops", "dispatch"),
     "combine": (".ops", "combine"),
@@ -21,6 +22,9 @@ _EXPORTS = {
     "capture_forward": (".graphs", "capture_forward"),
     "get_extension": ("._extension", "get_extension"),
     "HostPipeline": (".host_pipeline", "HostPipeline"),
+    "balance_loss": (".training", "balance_loss"),
+    "route": (".training", "route"),
+    "route_backward": (".training", "route_backward"),
 }
 
 

@@ -22,12 +22,25 @@ LIBRARY = Path(__file__).resolve().parent / "lib" / "libmoe_b200.so"
 _DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 # name -> (restype, argtypes) of every entry point in include/moe_b200.h
-_P, _I32, _I64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+_P, _I32, _I64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 SIGNATURES = {
     "moe_abi_version": (ctypes.c_int, []),
     "moe_last_error": (ctypes.c_char_p, []),
     "moe_topk_route": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),
     "moe_route": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P]),
+    "moe_balance_loss_scratch_bytes": (ctypes.c_int64, [_I32]),
+    "moe_balance_loss": (
+        ctypes.c_int,
+        [_P, _I32, _P, _P, _P, _F32, _P, _P, _P, _I64, _I32, _I32, _P, _I64, _P],
+    ),
+    "moe_balance_loss_backward": (
+        ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _F32, _P, _I64, _I32, _I32, _P]
+    ),
+    "moe_route_backward_scratch_bytes": (ctypes.c_int64, [_I64, _I64, _I32, _I32, _I32]),
+    "moe_route_backward": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _I64, _P],
+    ),
     "moe_dispatch_scratch_bytes": (ctypes.c_int64, [_I64, _I32, _I32]),
     "moe_dispatch": (
         ctypes.c_int,
@@ -97,6 +110,10 @@ def _check_cuda(tensor, anchor, name):
     _require(tensor.is_cuda, f"{name}: all tensors must be CUDA tensors")
     _require(tensor.is_contiguous(), f"{name}: all tensors must be contiguous")
     _require(tensor.device == anchor.device, f"{name}: device mismatch")
+
+
+def _ptr(tensor):
+    return None if tensor is None else tensor.data_ptr()
 
 
 class Extension:
@@ -285,6 +302,103 @@ class Extension:
             ids32.data_ptr(), ids64.data_ptr(), weights.data_ptr(), tokens, hidden, experts,
             ids32.shape[1],
         )
+
+    # ------------------------------------------------------- router training
+    def _balance_checks(self, logits, bias, token_mask, grad):
+        _require(logits.is_cuda and logits.is_contiguous() and logits.dim() == 2
+                 and logits.dtype in _DTYPE_CODES, "expected FP32, FP16 or BF16 CUDA logits[T,E]")
+        tokens, experts = logits.shape
+        if bias is not None:
+            _check_cuda(bias, logits, "balance_loss")
+            _require(bias.shape == (experts,) and bias.dtype == torch.float32,
+                     "expected FP32 bias[E]")
+        if token_mask is not None:
+            _check_cuda(token_mask, logits, "balance_loss")
+            _require(token_mask.shape == (tokens,) and token_mask.dtype == torch.bool,
+                     "expected bool token_mask[T]")
+        if grad is not None:
+            _check_cuda(grad, logits, "balance_loss")
+            _require(grad.shape == logits.shape and grad.dtype == logits.dtype,
+                     "expected grad with the logits' shape and dtype")
+        return tokens, experts
+
+    def balance_loss_out(self, logits, ids, bias, token_mask, coefficient, loss, counts, counted):
+        """Load-balance loss, counts[E] and the counted tokens (include/moe_b200.h)."""
+        _require(ids.dim() == 2, "expected int32 ids[T,K]")
+        tokens, experts = self._balance_checks(logits, bias, token_mask, None)
+        for tensor in (ids, loss, counts, counted):
+            _check_cuda(tensor, logits, "balance_loss")
+        _require(ids.shape[0] == tokens and ids.dtype == torch.int32, "expected int32 ids[T,K]")
+        _require(loss.numel() == 1 and loss.dtype == torch.float32, "expected one FP32 loss")
+        _require(counts.shape == (experts,) and counts.dtype == torch.int32
+                 and counted.numel() == 1 and counted.dtype == torch.int32,
+                 "expected int32 counts[E] and counted[1]")
+        # the sums of each CTA: a buffer of this call's own, so calls on several
+        # streams or in several captured graphs never share one
+        size = max(int(self.lib.moe_balance_loss_scratch_bytes(experts)), 1)
+        scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
+        self._call(
+            logits.device, self.lib.moe_balance_loss,
+            logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), ids.data_ptr(),
+            _ptr(token_mask), coefficient, loss.data_ptr(), counts.data_ptr(), counted.data_ptr(),
+            tokens, experts, ids.shape[1], scratch.data_ptr(), size,
+        )
+
+    def balance_loss_backward_out(self, logits, bias, token_mask, counts, counted, grad_loss,
+                                  coefficient, topk, grad_logits):
+        """d loss / d logits times the scalar grad_loss (include/moe_b200.h)."""
+        tokens, experts = self._balance_checks(logits, bias, token_mask, grad_logits)
+        for tensor in (counts, counted, grad_loss):
+            _check_cuda(tensor, logits, "balance_loss")
+        _require(counts.shape == (experts,) and counts.dtype == torch.int32
+                 and counted.numel() == 1 and counted.dtype == torch.int32,
+                 "expected int32 counts[E] and counted[1]")
+        _require(grad_loss.numel() == 1 and grad_loss.dtype == torch.float32,
+                 "expected one FP32 grad_loss")
+        self._call(
+            logits.device, self.lib.moe_balance_loss_backward,
+            logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), _ptr(token_mask),
+            counts.data_ptr(), counted.data_ptr(), grad_loss.data_ptr(), coefficient,
+            grad_logits.data_ptr(), tokens, experts, topk,
+        )
+
+    def route_backward_out(self, x, router_weight, ids, weights, grad_weights, grad_logits, grad_x,
+                           grad_router_weight):
+        """Backward of route_out (include/moe_b200.h); grad_logits, grad_x and
+        grad_router_weight may be None."""
+        _require(x.is_cuda and x.is_contiguous() and x.dtype == torch.bfloat16 and x.dim() == 2,
+                 "expected contiguous BF16 CUDA x[T,H]")
+        for tensor in (router_weight, ids, weights, grad_weights):
+            _check_cuda(tensor, x, "route_backward")
+        tokens, hidden = x.shape
+        _require(router_weight.dim() == 2 and router_weight.shape[1] == hidden
+                 and router_weight.dtype == torch.float32, "expected FP32 router_weight[E,H]")
+        experts = router_weight.shape[0]
+        _require(ids.dim() == 2 and ids.shape[0] == tokens and ids.dtype == torch.int32,
+                 "expected int32 ids[T,K]")
+        _require(weights.shape == ids.shape and weights.dtype == torch.float32
+                 and grad_weights.shape == ids.shape and grad_weights.dtype == torch.float32,
+                 "expected FP32 weights and grad_weights [T,K]")
+        for tensor, like, name in ((grad_logits, None, "grad_logits"), (grad_x, x, "grad_x"),
+                                   (grad_router_weight, router_weight, "grad_router_weight")):
+            if tensor is None:
+                continue
+            _check_cuda(tensor, x, "route_backward")
+            shape, dtype = ((tokens, experts), torch.float32) if like is None else (like.shape, like.dtype)
+            _require(tensor.shape == shape and tensor.dtype == dtype,
+                     f"{name}: expected {dtype} {tuple(shape)}")
+        index = x.device.index if x.device.index is not None else torch.cuda.current_device()
+        with torch.cuda.device(index):  # the scratch size depends on the device
+            size = int(self.lib.moe_route_backward_scratch_bytes(
+                tokens, hidden, experts, grad_x is not None, grad_router_weight is not None))
+            _require(size >= 0, self.lib.moe_last_error().decode())
+            scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
+            self._call(
+                x.device, self.lib.moe_route_backward,
+                x.data_ptr(), router_weight.data_ptr(), ids.data_ptr(), weights.data_ptr(),
+                grad_weights.data_ptr(), _ptr(grad_logits), _ptr(grad_x), _ptr(grad_router_weight),
+                tokens, hidden, experts, ids.shape[1], scratch.data_ptr(), scratch.numel(),
+            )
 
     def _gemm_checks(self, a, weight, offsets, out):
         _require(a.is_cuda and a.is_contiguous() and a.dtype == torch.bfloat16 and a.dim() == 2,

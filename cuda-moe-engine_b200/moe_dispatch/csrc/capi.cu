@@ -105,6 +105,115 @@ int moe_route(const void* x_bf16, const float* router_weight, const float* bias,
                        "moe_route");
 }
 
+static int check_balance(const void* logits, int32_t dtype, const float* bias, int64_t tokens,
+                         int32_t experts, int32_t topk) {
+    if (!valid_dtype(dtype)) return fail(MOE_ERR_INVALID, "logits must be FP32, FP16 or BF16");
+    if (experts < 1 || experts > moe::kMaxRouteExperts)
+        return fail(MOE_ERR_INVALID, "the balance loss supports 1..%d experts", moe::kMaxRouteExperts);
+    if (topk < 1 || topk > moe::kMaxTopk)
+        return fail(MOE_ERR_INVALID, "topk must be in 1..%d", moe::kMaxTopk);
+    if (tokens < 0 || tokens > INT_MAX / topk)
+        return fail(MOE_ERR_INVALID, "tokens * topk exceeds int32 counts");
+    if (tokens > 0 && !logits) return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(logits, moe::dtype_bytes(dtype)) || !aligned(bias, 4))
+        return fail(MOE_ERR_INVALID, "logits and bias must be aligned to their element size");
+    return MOE_OK;
+}
+
+int64_t moe_balance_loss_scratch_bytes(int32_t experts) {
+    if (experts < 1 || experts > moe::kMaxRouteExperts) return -1;
+    return moe::balance_scratch_bytes(experts);
+}
+
+int moe_balance_loss(const void* logits, int32_t dtype, const float* bias, const int32_t* ids,
+                     const uint8_t* token_mask, float coefficient, float* loss, int32_t* counts,
+                     int32_t* counted, int64_t tokens, int32_t experts, int32_t topk, void* scratch,
+                     int64_t scratch_bytes, void* stream) {
+    const int checked = check_balance(logits, dtype, bias, tokens, experts, topk);
+    if (checked != MOE_OK) return checked;
+    if (!loss || !counts || !counted || (tokens > 0 && !ids))
+        return fail(MOE_ERR_INVALID, "null pointer");
+    if (!scratch || !aligned(scratch, 16) || scratch_bytes < moe::balance_scratch_bytes(experts))
+        return fail(MOE_ERR_INVALID, "balance loss scratch too small or unaligned (%lld bytes needed)",
+                    static_cast<long long>(moe::balance_scratch_bytes(experts)));
+    return cuda_status(moe::launch_balance_loss(logits, dtype, bias, ids, token_mask, coefficient, loss,
+                                                counts, counted, scratch, tokens, experts, topk,
+                                                static_cast<cudaStream_t>(stream)),
+                       "moe_balance_loss");
+}
+
+int moe_balance_loss_backward(const void* logits, int32_t dtype, const float* bias,
+                              const uint8_t* token_mask, const int32_t* counts,
+                              const int32_t* counted, const float* grad_loss, float coefficient,
+                              void* grad_logits, int64_t tokens, int32_t experts, int32_t topk,
+                              void* stream) {
+    const int checked = check_balance(logits, dtype, bias, tokens, experts, topk);
+    if (checked != MOE_OK) return checked;
+    if (!counts || !counted || !grad_loss || (tokens > 0 && !grad_logits))
+        return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(grad_logits, moe::dtype_bytes(dtype)))
+        return fail(MOE_ERR_INVALID, "grad_logits must be aligned to its element size");
+    return cuda_status(moe::launch_balance_loss_backward(logits, dtype, bias, token_mask, counts, counted,
+                                                         grad_loss, coefficient, grad_logits, tokens,
+                                                         experts, topk,
+                                                         static_cast<cudaStream_t>(stream)),
+                       "moe_balance_loss_backward");
+}
+
+static int check_route_backward(int64_t tokens, int64_t hidden, int32_t experts) {
+    if (hidden < 8 || hidden % 8 || hidden > INT_MAX / 8)
+        return fail(MOE_ERR_INVALID, "hidden must be a positive multiple of 8");
+    if (experts < 1 || experts > moe::kMaxRouteExperts)
+        return fail(MOE_ERR_INVALID, "routing supports 1..%d experts", moe::kMaxRouteExperts);
+    if (tokens < 0 || tokens > INT_MAX / (2 * moe::kMaxRouteExperts))
+        return fail(MOE_ERR_INVALID, "shape exceeds int32 indexing capacity");
+    return MOE_OK;
+}
+
+int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int32_t experts,
+                                         int32_t want_grad_x, int32_t want_grad_weight) {
+    if (check_route_backward(tokens, hidden, experts) != MOE_OK) return -1;
+    int64_t bytes = 0;
+    if (cuda_status(moe::route_backward_scratch_bytes(tokens, hidden, experts, want_grad_x != 0,
+                                                      want_grad_weight != 0, &bytes),
+                    "moe_route_backward_scratch_bytes") != MOE_OK)
+        return -1;
+    return bytes;
+}
+
+int moe_route_backward(const void* x_bf16, const float* router_weight, const int32_t* ids,
+                       const float* weights, const float* grad_weights, const float* grad_logits,
+                       void* grad_x_bf16, float* grad_router_weight, int64_t tokens, int64_t hidden,
+                       int32_t experts, int32_t topk, void* scratch, int64_t scratch_bytes,
+                       void* stream) {
+    const int checked = check_route_backward(tokens, hidden, experts);
+    if (checked != MOE_OK) return checked;
+    if (topk < 1 || topk > moe::kMaxTopk)
+        return fail(MOE_ERR_INVALID, "topk must be in 1..%d", moe::kMaxTopk);
+    if (!grad_x_bf16 && !grad_router_weight) return MOE_OK;
+    if (tokens > 0 && (!ids || !weights || !grad_weights || (grad_x_bf16 && !router_weight) ||
+                       (grad_router_weight && !x_bf16)))
+        return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(x_bf16, 16) || !aligned(router_weight, 4) || !aligned(grad_x_bf16, 16) ||
+        !aligned(grad_router_weight, 16) || !aligned(grad_logits, 4))
+        return fail(MOE_ERR_INVALID, "x and the gradients must be 16-byte aligned");
+    int64_t need = 0;
+    const int sized = cuda_status(moe::route_backward_scratch_bytes(tokens, hidden, experts, grad_x_bf16 != nullptr,
+                                                                    grad_router_weight != nullptr, &need),
+                                  "moe_route_backward");
+    if (sized != MOE_OK) return sized;
+    if (!scratch || !aligned(scratch, 256) || scratch_bytes < need)
+        return fail(MOE_ERR_INVALID, "router backward scratch too small or unaligned (%lld bytes needed)",
+                    static_cast<long long>(need));
+    const char* message = nullptr;
+    const cudaError_t err = moe::launch_route_backward(
+        x_bf16, router_weight, ids, weights, grad_weights, grad_logits, grad_x_bf16,
+        grad_router_weight, scratch, tokens, hidden, experts, topk, static_cast<cudaStream_t>(stream),
+        &message);
+    if (message) return fail(MOE_ERR_INVALID, "%s", message);
+    return cuda_status(err, "moe_route_backward");
+}
+
 int64_t moe_dispatch_scratch_bytes(int64_t tokens, int32_t topk, int32_t experts) {
     if (tokens < 0 || topk < 1 || experts < 1) return -1;
     return moe::dispatch_scratch_bytes(tokens * topk, experts);
@@ -477,7 +586,10 @@ int moe_device_status(int32_t* code, int32_t clear) {
     status = cuda_status(moe::read_ep_status(&ep, clear != 0), "moe_device_status");
     if (status != MOE_OK) return status;
     status = cuda_status(moe::read_route_status(&route, clear != 0), "moe_device_status");
-    *code = gemm ? gemm : (ep ? ep : route);
+    if (status != MOE_OK) return status;
+    int32_t backward = 0;
+    status = cuda_status(moe::read_route_backward_status(&backward, clear != 0), "moe_device_status");
+    *code = gemm ? gemm : (ep ? ep : (route ? route : backward));
     return status;
 }
 

@@ -33,6 +33,7 @@
 // copies and MMAs in flight, frees its TMEM and returns.
 #include "common.cuh"
 #include "launch.h"
+#include "tcgen05.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -171,58 +172,6 @@ __device__ void build_tile_table(const GemmParams& p, int lane, int* mt_prefix, 
     if (lane == 0) mt_prefix[pairs] = carry;
 }
 
-// ---------------------------------------------------------------- PTX helpers
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ uint64_t global_timer() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-                 "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// The same with cluster-scope acquire: for phases completed by the other CTA
-// of a pair, whose shared-memory writes must be visible after the wait.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
 __device__ __forceinline__ void record_status(int32_t code) { atomicCAS(&g_gemm_status, 0, code); }
 
 // Bounded wait for the phase of `bar` with the given parity.  Returns false
@@ -255,49 +204,8 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
            mbar_wait_slow<true>(bar, parity, abort_flag, limit_ns);
 }
 
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x,
-                                            int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-        : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-// K-major operand, 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes
-// apart (SBO); the leading offset is unused for this layout (encoded as 1).
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
-    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
-           (static_cast<uint64_t>(2) << 61);
-}
-
-// Instruction descriptor: D fp32, both operands K-major, M x N; A and B bf16
-// (format 1 for kind::f16) or e4m3 (format 0 for kind::f8f6f4).
-constexpr uint32_t make_idesc(int m, int n, bool fp8 = false) {
-    const uint32_t ab = fp8 ? 0u : ((1u << 7) | (1u << 10));
-    return (1u << 4) | ab | (static_cast<uint32_t>(n >> 3) << 17) |
-           (static_cast<uint32_t>(m >> 4) << 24);
-}
-
 // Elements of one 128-byte swizzled row: one k-block per pipeline stage.
 template <bool kFp8> constexpr int stage_k() { return kFp8 ? 128 : kBK; }
-
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
-                                          uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate));
-}
 
 // e4m3 x e4m3 -> fp32, K = 32 per instruction (32 bytes of each operand row).
 __device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
@@ -314,30 +222,6 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t desc_a, uint64_t 
                                      uint32_t idesc, uint32_t accumulate) {
     if constexpr (kFp8) umma_e4m3(tmem_d, desc_a, desc_b, idesc, accumulate);
     else umma_bf16(tmem_d, desc_a, desc_b, idesc, accumulate);
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-            smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_wait_ld() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ float round_bf16(float v) {
@@ -1549,14 +1433,14 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 }
 
 // Row-major matrix [rows, cols] of bf16 (or e4m3 bytes with fp8), boxes of
-// box_rows rows x 128 bytes, 128B swizzle.
+// box_rows rows x 128 bytes, 128B swizzle; rows `stride` elements apart (0: cols).
 bool make_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
-                     bool fp8 = false, uint32_t box_rows = kBoxRows) {
+                     bool fp8 = false, uint32_t box_rows = kBoxRows, uint64_t stride = 0) {
     auto encode = tensor_map_encoder();
     if (!encode) return false;
     const uint64_t elem = fp8 ? 1 : 2;
     cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {cols * elem};
+    cuuint64_t strides[1] = {(stride ? stride : cols) * elem};
     cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem), static_cast<cuuint32_t>(box_rows)};
     cuuint32_t elem_strides[2] = {1, 1};
     return encode(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
@@ -1660,11 +1544,16 @@ cudaError_t launch_pair(Kernel kernel, int smem_bytes, bool& configured, int& re
 
 }  // namespace
 
+bool encode_bf16_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                            uint64_t stride, uint32_t box_rows) {
+    return make_tensor_map(map, base, rows, cols, false, box_rows, stride);
+}
+
 cudaError_t launch_grouped_gemm(const void* a, const void* b, const int32_t* offsets, void* out,
                                 int64_t rows, int64_t n_out, int64_t k_dim, int experts,
                                 bool swiglu, cudaStream_t stream, const char** error,
                                 const float* a_scale, const float* b_scale,
-                                const GemmArrival* arrival) {
+                                const GemmArrival* arrival, int64_t a_stride) {
     const bool fp8 = a_scale != nullptr;
     *error = nullptr;
     if (rows == 0 || experts == 0) return cudaSuccess;
@@ -1679,7 +1568,8 @@ cudaError_t launch_grouped_gemm(const void* a, const void* b, const int32_t* off
     if (info.sms == 0) MOE_CUDA_TRY(cudaDeviceGetAttribute(&info.sms, cudaDevAttrMultiProcessorCount, device));
     const int64_t b_rows = swiglu ? 2 * n_out : n_out;
     CUtensorMap map_a, map_b;
-    if (!make_tensor_map(&map_a, a, static_cast<uint64_t>(rows), static_cast<uint64_t>(k_dim), fp8) ||
+    if (!make_tensor_map(&map_a, a, static_cast<uint64_t>(rows), static_cast<uint64_t>(k_dim), fp8,
+                         kBoxRows, static_cast<uint64_t>(a_stride)) ||
         !make_tensor_map(&map_b, b, static_cast<uint64_t>(b_rows * experts), static_cast<uint64_t>(k_dim), fp8)) {
         *error = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
         return cudaErrorInvalidValue;

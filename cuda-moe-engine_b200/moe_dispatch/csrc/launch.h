@@ -22,6 +22,30 @@ cudaError_t launch_route(const void* x, const float* w, const float* bias, float
 cudaError_t launch_topk(const float* logits, const float* bias, int32_t* ids32, int64_t* ids64,
                         float* weights, int64_t tokens, int experts, int topk, cudaStream_t stream);
 
+// Load-balance loss, per-expert counts, and d loss / d logits (balance.cu).
+// counted[0] receives the tokens that the mask (null: all) keeps.
+int64_t balance_scratch_bytes(int experts);
+cudaError_t launch_balance_loss(const void* logits, int dtype, const float* bias,
+                                const int32_t* ids, const uint8_t* mask, float coefficient,
+                                float* loss, int32_t* counts, int32_t* counted, void* scratch,
+                                int64_t tokens, int experts, int topk, cudaStream_t stream);
+cudaError_t launch_balance_loss_backward(const void* logits, int dtype, const float* bias,
+                                         const uint8_t* mask, const int32_t* counts,
+                                         const int32_t* counted, const float* grad_loss,
+                                         float coefficient, void* grad, int64_t tokens, int experts,
+                                         int topk, cudaStream_t stream);
+
+// Router backward (route_backward.cu): grad_x [T,H] bf16 and grad_weight [E,H]
+// fp32, either may be null; grad_logits may be null.
+cudaError_t route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw,
+                                         int64_t* bytes);
+cudaError_t launch_route_backward(const void* x, const float* weight, const int32_t* ids,
+                                  const float* weights, const float* grad_weights,
+                                  const float* grad_logits, void* grad_x, float* grad_weight,
+                                  void* scratch, int64_t tokens, int64_t hidden, int experts, int topk,
+                                  cudaStream_t stream, const char** error);
+cudaError_t read_route_backward_status(int32_t* code, bool clear);
+
 int64_t dispatch_scratch_bytes(int64_t assignments, int experts);
 cudaError_t launch_dispatch(const void* x, int dtype, const int32_t* ids, int32_t* counts,
                             int32_t* offsets, int32_t* slots, void* packed, int32_t* inverse,
@@ -55,11 +79,12 @@ struct GemmArrival {
 // the returned status is not cudaSuccess because of a host-side check.
 // With a_scale (and b_scale) non-null, a and b are e4m3 bytes and every
 // accumulator is dequantised as (acc * a_scale[row]) * b_scale[weight row].
+// a_stride: elements between the rows of a (0: k_dim).
 cudaError_t launch_grouped_gemm(const void* a, const void* b, const int32_t* offsets, void* out,
                                 int64_t rows, int64_t n_out, int64_t k_dim, int experts,
                                 bool swiglu, cudaStream_t stream, const char** error,
                                 const float* a_scale = nullptr, const float* b_scale = nullptr,
-                                const GemmArrival* arrival = nullptr);
+                                const GemmArrival* arrival = nullptr, int64_t a_stride = 0);
 // e4m3 quantisation of bf16 rows: scale[r] = amax_r / 448, q[r,c] = e4m3(x[r,c] * (448 / amax_r))
 // (round to nearest even, saturating); an all-zero row gets scale 1 and zeros.
 cudaError_t launch_quantize_rows_e4m3(const void* x, void* q, float* scale, int64_t rows,

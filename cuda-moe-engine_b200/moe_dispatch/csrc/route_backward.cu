@@ -1,0 +1,513 @@
+// Backward pass of the router: gradients of the routing weights (and, where
+// given, of the logits) carried to the tokens and to the router weight.  No
+// counterpart in the reference, whose block is forward-only.
+//
+//   ds[t,k] = w[t,k] (gw[t,k] - sum_j w[t,j] gw[t,j])      softmax over the selected scores
+//   d       = grad_logits + scatter of ds to the ids        [T, E], fp32
+//   dx      = d W  [T, H], rounded once to bf16             dW = d^T x  [E, H], fp32
+//
+// Both products are 2 T E H flop of fp32 data.  The tensor cores take bf16, so
+// every fp32 operand is split into bf16 parts whose sum is the value: hi =
+// bf16(v), mid = bf16(v - hi), lo = bf16(v - hi - mid), each within half a step
+// (2^-8) of the rest, so hi + mid + lo is v to 2^-24.  x is bf16 already.  dW
+// (an fp32 result) takes all three parts of d; dx (a bf16 result) takes
+// d_mid W_hi + d_hi W_hi + d_hi W_lo, which leaves out terms of 2^-16 |d W|.
+//
+//   split_gradient_kernel  a warp per token writes d's parts, [T, 4 E8] bf16 with
+//                          columns lo | mid | hi | hi, E8 = E rounded up to 8
+//   split_weight_kernel    W^T parts, [H, 3 E8] bf16 with columns hi | hi | lo
+//   dx                     the grouped GEMM with one group: columns mid | hi | hi
+//                          of the first against the second, K = 3 E8
+//   router_dw_kernel       dW: tcgen05 over tokens as K, both operands MN-major
+//   add_parts_kernel       adds the token ranges' partial sums in order
+//
+// Bound: for few experts by reading x once per product; for 256 experts by the
+// tensor cores (6 bf16 flop per fp32 multiply-add).
+#include "common.cuh"
+#include "launch.h"
+#include "tcgen05.cuh"
+
+namespace moe {
+
+bool encode_bf16_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                            uint64_t stride, uint32_t box_rows);
+
+namespace {
+
+__device__ int32_t g_route_backward_status;
+constexpr int32_t kStatusRouterBackwardWait = 7;
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr uint64_t kDrainLimitNs = 200000000ull;
+
+// ------------------------------------------------------------------- splits
+
+__device__ __forceinline__ uint32_t bf16_part(float& rest) {
+    const __nv_bfloat16 h = __float2bfloat16_rn(rest);
+    rest -= __bfloat162float(h);
+    return __bfloat16_as_ushort(h);
+}
+
+// A warp per token; lane holds experts 2 (lane + 32 i) and the next one.
+template <int PAIRS>
+__global__ void __launch_bounds__(256)
+split_gradient_kernel(const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
+                      const float* __restrict__ weights, const float* __restrict__ grad_weights,
+                      uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded,
+                      int topk) {
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
+    pdl_trigger();
+    pdl_wait();
+    const int half = padded / 2;  // 32-bit words of one part's columns
+    for (int64_t t = blockIdx.x * 8ll + (threadIdx.x >> 5); t < tokens; t += warps) {
+        float d[PAIRS][2];
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            const int e = 2 * (lane + 32 * i);
+            d[i][0] = grad_logits && e < experts ? grad_logits[t * experts + e] : 0.0f;
+            d[i][1] = grad_logits && e + 1 < experts ? grad_logits[t * experts + e + 1] : 0.0f;
+        }
+        int id = -1;
+        float w = 0.0f, g = 0.0f;
+        if (lane < topk) {
+            id = ids[t * topk + lane];
+            w = weights[t * topk + lane];
+            g = grad_weights[t * topk + lane];
+        }
+        float dot = w * g;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+        const float ds = w * (g - dot);
+        for (int k = 0; k < topk; ++k) {  // in order: a repeated id adds the same way every time
+            const int e = __shfl_sync(0xffffffffu, id, k);
+            const float v = __shfl_sync(0xffffffffu, ds, k);
+            if (e < 0 || e >= experts) continue;
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i)
+                if (lane + 32 * i == e >> 1) {
+                    if (e & 1) d[i][1] += v;
+                    else d[i][0] += v;
+                }
+        }
+        uint32_t* row = parts + t * 4 * half;
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            const int at = lane + 32 * i;
+            if (at >= half) continue;
+            const uint32_t hi = bf16_part(d[i][0]) | bf16_part(d[i][1]) << 16;
+            const uint32_t mid = bf16_part(d[i][0]) | bf16_part(d[i][1]) << 16;
+            const uint32_t lo = bf16_part(d[i][0]) | bf16_part(d[i][1]) << 16;
+            row[at] = lo;
+            row[half + at] = mid;
+            row[2 * half + at] = hi;
+            row[3 * half + at] = hi;
+        }
+    }
+}
+
+// W [E, H] fp32 -> [H, 3 E8] bf16: 32 x 32 tiles through shared memory.  Thread
+// 0 of the first CTA also writes the grouped GEMM's offsets {0, T}.
+__global__ void __launch_bounds__(256)
+split_weight_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ out,
+                    int32_t* __restrict__ offsets, int tokens, int experts, int padded,
+                    int64_t hidden) {
+    __shared__ float tile[32][33];
+    pdl_trigger();
+    pdl_wait();
+    const int64_t h0 = blockIdx.x * 32ll;
+    const int e0 = blockIdx.y * 32;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+        offsets[0] = 0;
+        offsets[1] = tokens;
+    }
+    for (int i = y; i < 32; i += 8)
+        tile[i][x] = e0 + i < experts && h0 + x < hidden ? weight[(e0 + i) * hidden + h0 + x] : 0.0f;
+    __syncthreads();
+    if (e0 + x >= padded) return;
+    for (int i = y; i < 32; i += 8) {
+        if (h0 + i >= hidden) break;
+        float v = tile[x][i];
+        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+        __nv_bfloat16* row = out + (h0 + i) * 3 * padded + e0 + x;
+        row[0] = hi;
+        row[padded] = hi;
+        row[2 * padded] = __float2bfloat16_rn(v - __bfloat162float(hi));
+    }
+}
+
+// ----------------------------------------------------------------------- dW
+
+constexpr int kTileH = 128;   // rows of dW^T per CTA (M)
+constexpr int kTileT = 32;    // tokens per pipeline stage (K)
+constexpr int kBlock = kTileT * 128;  // bytes of 64 columns x kTileT tokens
+constexpr int kMaxStages = 8;
+constexpr int kDwThreads = 192;  // producer, issuer, four epilogue warps
+constexpr int kDwSmem = 224 * 1024;
+
+struct DwParams {
+    float* out;           // dW [E, H], or the partial sums [ranges, E, H]
+    int64_t hidden;
+    int tokens, experts, padded;
+    int range;            // tokens per CTA (a multiple of kTileT)
+    int terms;            // MMAs per 16 tokens: 3 (one per part) or 1 (parts side by side in N)
+    int blocks;           // 64-column boxes per term
+    int n;                // MMA N
+    int tmem_cols;
+    int hi_col;           // first column of the hi part's accumulator (3 terms)
+    int stages;
+};
+
+__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                             uint64_t limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t start = global_timer();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 31) == 0) {
+            if (*abort_flag) return false;
+            if (global_timer() - start > limit) {
+                atomicCAS(&g_route_backward_status, 0, kStatusRouterBackwardWait);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
+// MN-major operand, 128-byte swizzle: 64 columns x tokens as rows of 128 bytes;
+// 8-token groups 1024 bytes apart (stride offset), 64-column blocks kBlock apart
+// (leading offset).
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kBlock >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+           (static_cast<uint64_t>(2) << 61);
+}
+
+// dW^T tile [128 h, E] of one range of tokens.  Warp 0 loads x [32 tokens, 128]
+// and d's parts [32, E8 each] by TMA, warp 1 issues the MMAs (M = 128, K = 16),
+// warps 2-5 store the tile.  Up to E8 = 80 the three parts stand side by side in
+// N (3 E8 <= 240): one MMA per 16 tokens, and the epilogue adds the three column
+// groups.  Above that each part is an MMA of its own: hi into one accumulator,
+// lo and mid into a second.  (The tensor cores cut the sum of 16 products and
+// the accumulator off below its last bit.  With all parts in one accumulator the
+// small parts' products are cut off there too: dW at 32768 tokens, 256 experts
+// was 6.7e-6 of its norm away from the float64 product, 11 times the plain fp32
+// product's distance.)  A CTA's range bounds the additions in one accumulator
+// (at most 4096 tokens); ranges are added in a launch of their own.
+__global__ void __launch_bounds__(kDwThreads, 1)
+router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_d,
+                 const DwParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h0 = blockIdx.x * kTileH;
+    const int t0 = blockIdx.y * p.range;
+    const int t1 = min(t0 + p.range, p.tokens);
+    const int steps = (t1 - t0 + kTileT - 1) / kTileT;  // >= 1
+    const int stage_bytes = (2 + p.terms * p.blocks) * kBlock;
+
+    pdl_trigger();
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&done, 1);
+        mbar_init(&drain, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&tmem_slot)),
+                     "r"(p.tmem_cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0, armed = 0, parity = 0;
+        for (int i = 0; i < steps; ++i) {
+            if (!wait_bounded(&empty[stage], phase ^ 1u, &abort_flag, kWaitLimitNs)) break;
+            uint8_t* at = tiles + stage * stage_bytes;
+            const int t = t0 + i * kTileT;
+            mbar_expect_tx(&full[stage], stage_bytes);
+            tma_load_2d(at, &map_x, &full[stage], h0, t);
+            tma_load_2d(at + kBlock, &map_x, &full[stage], h0 + 64, t);
+            at += 2 * kBlock;
+            for (int s = 0; s < p.terms; ++s)
+                for (int b = 0; b < p.blocks; ++b, at += kBlock)
+                    tma_load_2d(at, &map_d, &full[stage], s * p.padded + b * 64, t);
+            armed |= 1u << stage;
+            parity = (parity & ~(1u << stage)) | (phase << stage);
+            if (++stage == p.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (abort_flag) {  // every copy in flight lands before the CTA exits
+            volatile int never = 0;
+            for (int s = 0; s < p.stages; ++s)
+                if (armed & (1u << s)) wait_bounded(&full[s], (parity >> s) & 1u, &never, kDrainLimitNs);
+        }
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t idesc = make_idesc(kTileH, p.n) | (1u << 15) | (1u << 16);  // both MN-major
+        int stage = 0;
+        uint32_t phase = 0;
+        bool issued = false;
+        for (int i = 0; i < steps; ++i) {
+            if (!wait_bounded(&full[stage], phase, &abort_flag, kWaitLimitNs)) break;
+            tc_fence_after();
+            const uint32_t x_at = smem_u32(tiles + stage * stage_bytes);
+            const uint32_t d_at = x_at + 2 * kBlock;
+            for (int k = 0; k < kTileT / 16; ++k)
+                for (int s = 0; s < p.terms; ++s) {
+                    const bool first = i == 0 && k == 0 && s != 1;  // of its accumulator
+                    umma_bf16(tmem + (s == 2 ? p.hi_col : 0), mn_desc(x_at + k * 2048),
+                              mn_desc(d_at + s * p.blocks * kBlock + k * 2048), idesc, first ? 0u : 1u);
+                }
+            issued = true;
+            umma_commit(&empty[stage]);
+            if (++stage == p.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (!abort_flag) {
+            umma_commit(&done);
+            volatile int never = 0;  // whatever the epilogue does, no MMA outlives this wait
+            wait_bounded(&done, 0, &never, kWaitLimitNs);
+        } else if (issued) {  // MMAs in flight end before the tensor memory is freed
+            umma_commit(&drain);
+            volatile int never = 0;
+            wait_bounded(&drain, 0, &never, kDrainLimitNs);
+        }
+    } else if (warp >= 2) {
+        // TMEM lane = row of the tile (h), column = expert: a warp stores 32 neighbours of one
+        // expert's row.  Lanes past H (only in the last tile) store nothing.
+        if (wait_bounded(&done, 0, &abort_flag, 2 * kWaitLimitNs)) {
+            tc_fence_after();
+            const int quarter = warp & 3;
+            const int64_t h = h0 + quarter * 32 + lane;
+            const uint32_t row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+            float* out = p.out + static_cast<int64_t>(blockIdx.y) * p.experts * p.hidden + h;
+            for (int c = 0; c < p.experts; c += 32) {
+                uint32_t v[32];
+                float sum[32];
+                tmem_ld32(row + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[j] = __uint_as_float(v[j]);
+                // the small parts first: lo + mid + hi, or (lo and mid) + hi
+                const int step = p.terms == 1 ? p.padded : p.hi_col;
+                for (int s = 1; s < (p.terms == 1 ? 3 : 2); ++s) {
+                    tmem_ld32(row + s * step + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(v[j]);
+                }
+                if (h < p.hidden) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < p.experts) out[(c + j) * p.hidden] = sum[j];
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+    }
+}
+
+__global__ void __launch_bounds__(256)
+add_parts_kernel(const float4* __restrict__ parts, float4* __restrict__ out, int64_t vecs, int ranges) {
+    pdl_trigger();
+    pdl_wait();
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < vecs; i += gridDim.x * 256ll) {
+        float4 sum = parts[i];
+#pragma unroll 4
+        for (int r = 1; r < ranges; ++r) {
+            const float4 v = parts[r * vecs + i];
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+        out[i] = sum;
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+int pad8(int experts) { return (experts + 7) / 8 * 8; }
+
+// Tokens per CTA of the dW kernel.  At most 4096 (see router_dw_kernel), at
+// least 256 (below that the ranges' partial sums cost more than they spread);
+// within that the number of ranges that leaves the fewest SMs idle in the last
+// wave of CTAs.
+constexpr int64_t kMinRange = 256, kMaxRange = 4096;
+int token_ranges(int64_t tokens, int64_t hidden, int sms) {
+    const int64_t tiles = (hidden + kTileH - 1) / kTileH;
+    const int64_t least = (tokens + kMaxRange - 1) / kMaxRange;
+    int64_t most = (tokens + kMinRange - 1) / kMinRange;
+    if (most > least + 15) most = least + 15;
+    int64_t best = least;
+    double best_time = 1e30;
+    for (int64_t r = least; r <= most; ++r) {
+        const double waves = static_cast<double>((tiles * r + sms - 1) / sms);
+        const double time = waves * (static_cast<double>(tokens) / r + 64.0);  // + a CTA's start and end
+        if (time < 0.98 * best_time) {
+            best_time = time;
+            best = r;
+        }
+    }
+    return static_cast<int>(best);
+}
+
+int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+struct Layout {
+    int64_t parts, weight, offsets, sums, total;
+};
+Layout layout(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw, int sms) {
+    const int64_t e8 = pad8(experts);
+    Layout l;
+    l.parts = 0;
+    l.weight = round256(tokens * 4 * e8 * 2);
+    l.offsets = l.weight + (dx ? round256(hidden * 3 * e8 * 2) : 0);
+    l.sums = l.offsets + 256;
+    const int ranges = token_ranges(tokens, hidden, sms);
+    l.total = l.sums + (dw && ranges > 1 ? round256(ranges * experts * hidden * 4) : 0);
+    return l;
+}
+
+cudaError_t device_sms(int* sms) {
+    static int cached[64] = {};
+    int device = 0;
+    MOE_CUDA_TRY(cudaGetDevice(&device));
+    if (cached[device & 63] == 0)
+        MOE_CUDA_TRY(cudaDeviceGetAttribute(&cached[device & 63], cudaDevAttrMultiProcessorCount, device));
+    *sms = cached[device & 63];
+    return cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw,
+                                         int64_t* bytes) {
+    int sms = 0;
+    MOE_CUDA_TRY(device_sms(&sms));
+    *bytes = layout(tokens, hidden, experts, dx, dw, sms).total;
+    return cudaSuccess;
+}
+
+cudaError_t launch_route_backward(const void* x, const float* weight, const int32_t* ids,
+                                  const float* weights, const float* grad_weights,
+                                  const float* grad_logits, void* grad_x, float* grad_weight,
+                                  void* scratch, int64_t tokens, int64_t hidden, int experts, int topk,
+                                  cudaStream_t stream, const char** error) {
+    *error = nullptr;
+    if (tokens == 0)
+        return grad_weight ? cudaMemsetAsync(grad_weight, 0, experts * hidden * 4, stream) : cudaSuccess;
+    int sms = 0;
+    MOE_CUDA_TRY(device_sms(&sms));
+    const int e8 = pad8(experts);
+    const Layout l = layout(tokens, hidden, experts, grad_x != nullptr, grad_weight != nullptr, sms);
+    char* base = static_cast<char*>(scratch);
+    auto* parts = reinterpret_cast<__nv_bfloat16*>(base + l.parts);
+
+    const int64_t blocks = (tokens + 7) / 8;
+    const unsigned grid = static_cast<unsigned>(blocks < 8ll * sms ? blocks : 8ll * sms);
+    auto split = experts <= 64 ? split_gradient_kernel<1>
+                               : (experts <= 128 ? split_gradient_kernel<2> : split_gradient_kernel<4>);
+    MOE_CUDA_TRY(launch_dependent(split, dim3(grid), dim3(256), 0, stream, grad_logits, ids, weights,
+                                  grad_weights, reinterpret_cast<uint32_t*>(parts), tokens, experts, e8,
+                                  topk));
+    if (grad_x) {
+        auto* wt = reinterpret_cast<__nv_bfloat16*>(base + l.weight);
+        auto* offsets = reinterpret_cast<int32_t*>(base + l.offsets);
+        MOE_CUDA_TRY(launch_dependent(split_weight_kernel,
+                                      dim3(static_cast<unsigned>((hidden + 31) / 32), (e8 + 31) / 32),
+                                      dim3(256), 0, stream, weight, wt, offsets,
+                                      static_cast<int>(tokens), experts, e8, hidden));
+        MOE_CUDA_TRY(launch_grouped_gemm(parts + e8, wt, offsets, grad_x, tokens, hidden, 3 * e8, 1,
+                                         false, stream, error, nullptr, nullptr, nullptr, 4 * e8));
+    }
+    if (grad_weight) {
+        DwParams p;
+        p.hidden = hidden;
+        p.tokens = static_cast<int>(tokens);
+        p.experts = experts;
+        p.padded = e8;
+        const bool side_by_side = 3 * e8 <= 240;
+        const int columns = side_by_side ? 3 * e8 : e8;
+        p.terms = side_by_side ? 1 : 3;
+        p.blocks = (columns + 63) / 64;
+        p.n = (columns + 15) / 16 * 16;
+        // the epilogue reads 32 columns at a time from each column group
+        const int reach = (side_by_side ? 2 * e8 : 0) + (e8 + 31) / 32 * 32;
+        const int need = reach > p.n ? reach : p.n;
+        p.tmem_cols = 32;
+        while (p.tmem_cols < need) p.tmem_cols *= 2;
+        p.hi_col = p.tmem_cols;
+        if (!side_by_side) p.tmem_cols *= 2;
+        const int stage_bytes = (2 + p.terms * p.blocks) * kBlock;
+        p.stages = kDwSmem / stage_bytes < kMaxStages ? kDwSmem / stage_bytes : kMaxStages;
+        const int ranges = token_ranges(tokens, hidden, sms);
+        const int64_t per = (tokens + ranges - 1) / ranges;
+        p.range = static_cast<int>((per + kTileT - 1) / kTileT * kTileT);
+        const unsigned used = static_cast<unsigned>((tokens + p.range - 1) / p.range);
+        p.out = used > 1 ? reinterpret_cast<float*>(base + l.sums) : grad_weight;
+        CUtensorMap map_x, map_d;
+        if (!encode_bf16_tensor_map(&map_x, x, tokens, hidden, 0, kTileT) ||
+            !encode_bf16_tensor_map(&map_d, parts, tokens, 4 * e8, 0, kTileT)) {
+            *error = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
+            return cudaErrorInvalidValue;
+        }
+        static bool configured[64] = {};
+        int device = 0;
+        MOE_CUDA_TRY(cudaGetDevice(&device));
+        const int smem = kDwSmem + 1024;
+        if (!configured[device & 63]) {
+            MOE_CUDA_TRY(cudaFuncSetAttribute(router_dw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            configured[device & 63] = true;
+        }
+        const unsigned tiles = static_cast<unsigned>((hidden + kTileH - 1) / kTileH);
+        MOE_CUDA_TRY(launch_dependent(router_dw_kernel, dim3(tiles, used), dim3(kDwThreads),
+                                      p.stages * stage_bytes + 1024, stream, map_x, map_d, p));
+        if (used > 1) {
+            const int64_t vecs = experts * hidden / 4;
+            const int64_t need_ctas = (vecs + 255) / 256;
+            MOE_CUDA_TRY(launch_dependent(add_parts_kernel,
+                                          dim3(static_cast<unsigned>(need_ctas < 8ll * sms ? need_ctas : 8ll * sms)),
+                                          dim3(256), 0, stream, reinterpret_cast<const float4*>(p.out),
+                                          reinterpret_cast<float4*>(grad_weight), vecs,
+                                          static_cast<int>(used)));
+        }
+    }
+    return cudaSuccess;
+}
+
+cudaError_t read_route_backward_status(int32_t* code, bool clear) {
+    MOE_CUDA_TRY(cudaMemcpyFromSymbol(code, g_route_backward_status, sizeof(int32_t)));
+    if (clear) {
+        const int32_t zero = 0;
+        MOE_CUDA_TRY(cudaMemcpyToSymbol(g_route_backward_status, &zero, sizeof(int32_t)));
+    }
+    return cudaSuccess;
+}
+
+}  // namespace moe

@@ -64,6 +64,56 @@ int moe_route(const void* x_bf16, const float* router_weight, const float* bias,
               int32_t* ids32, int64_t* ids64, float* weights, int64_t tokens, int64_t hidden,
               int32_t experts, int32_t topk, void* stream);
 
+/* Load-balance loss of a router and its per-expert counts (no counterpart in
+ * the reference, which is forward-only).  With z = logits + bias (bias may be
+ * NULL), p = softmax(z) over the experts, V the tokens whose token_mask byte is
+ * not 0 (token_mask may be NULL: all), counts[e] the ids equal to e of those
+ * tokens (ids outside [0, experts) count for nothing, a repeated id counts each
+ * time) and f[e] = counts[e] / (V topk):
+ *   loss = coefficient * experts * sum_e f[e] * (1/V) sum_t p[t,e].
+ * logits [tokens, experts] of `dtype`; loss, counts[experts] and counted (the
+ * number V) are device memory.  V = 0 gives loss 0.  A row whose scores are
+ * all -inf has p = 0.  Sums in fp32 in a fixed order: same bits on every run.
+ * scratch: moe_balance_loss_scratch_bytes(experts), 16-byte aligned, not
+ * initialised; calls that may overlap in time need one each. */
+int64_t moe_balance_loss_scratch_bytes(int32_t experts);
+int moe_balance_loss(const void* logits, int32_t dtype, const float* bias, const int32_t* ids,
+                     const uint8_t* token_mask, float coefficient, float* loss, int32_t* counts,
+                     int32_t* counted, int64_t tokens, int32_t experts, int32_t topk, void* scratch,
+                     int64_t scratch_bytes, void* stream);
+
+/* Its gradient, from the counts and counted that it wrote and a device scalar
+ * grad_loss:  grad_logits[t,e] = grad_loss * coefficient * experts / V *
+ * p[t,e] * (f[e] - sum_j f[j] p[t,j]) for the tokens that count, 0 for the
+ * others; rounded once to `dtype`. */
+int moe_balance_loss_backward(const void* logits, int32_t dtype, const float* bias,
+                              const uint8_t* token_mask, const int32_t* counts,
+                              const int32_t* counted, const float* grad_loss, float coefficient,
+                              void* grad_logits, int64_t tokens, int32_t experts, int32_t topk,
+                              void* stream);
+
+/* Backward pass of moe_route (no counterpart in the reference).  From its ids
+ * and weights [tokens, topk], the gradient of the weights and, unless NULL, a
+ * gradient grad_logits [tokens, experts] of its logits:
+ *   ds[t,k] = weights[t,k] (grad_weights[t,k] - sum_j weights[t,j] grad_weights[t,j])
+ *   d       = grad_logits + ds added at the ids (ids outside [0, experts) are skipped,
+ *             a repeated id adds each time)
+ *   grad_x [tokens, hidden] bf16 = d . router_weight  (rounded once; NULL: not computed)
+ *   grad_router_weight [experts, hidden] fp32 = d^T . x  (written; NULL: not computed)
+ * on tcgen05 with d and the weight split into bf16 parts: the products are
+ * fp32-accurate for grad_router_weight (d to 2^-24) and to 2^-16 for grad_x.
+ * Gradients that are not finite give results that are not finite.  Fixed
+ * summation order.  hidden % 8 == 0; x and the gradients 16-byte aligned.
+ * scratch: 256-byte aligned, not initialised, its size for the current device;
+ * calls that may overlap in time need one each. */
+int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int32_t experts,
+                                         int32_t want_grad_x, int32_t want_grad_weight);
+int moe_route_backward(const void* x_bf16, const float* router_weight, const int32_t* ids,
+                       const float* weights, const float* grad_weights, const float* grad_logits,
+                       void* grad_x_bf16, float* grad_router_weight, int64_t tokens, int64_t hidden,
+                       int32_t experts, int32_t topk, void* scratch, int64_t scratch_bytes,
+                       void* stream);
+
 /* --------------------------------------------------------------- transport */
 
 /* Device scratch (bytes) that moe_dispatch needs for `tokens*topk`
@@ -301,7 +351,8 @@ int moe_ep_p2p_down_return(const void* activated, const void* down, void* const*
  * launches that shared one tile-claim slot at the same time (one captured
  * graph replayed on two streams at once, or more than 512 captured GEMM
  * launches in flight together); their results are void; 6 a gate/up GEMM of
- * moe_ep_p2p_gate_up that gave up waiting for a peer's rows. */
+ * moe_ep_p2p_gate_up that gave up waiting for a peer's rows; 7 a pipeline wait
+ * of moe_route_backward. */
 int moe_device_status(int32_t* code, int32_t clear);
 
 #ifdef __cplusplus
