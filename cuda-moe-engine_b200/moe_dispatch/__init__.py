@@ -9,7 +9,8 @@ from importlib import import_module
 __version__ = "0.2.0+b200"
 __all__ = ["dispatch", "combine", "PackedTokens", "CudaWorkspace", "MoEBlock", "MoEConfig",
            "MoEWeights", "make_weights", "capture_forward", "get_extension", "HostPipeline",
-           "balance_loss", "route", "route_backward"]
+           "balance_loss", "route", "route_backward", "MoEAdapters", "adapter_add",
+           "adapter_swiglu"]
 _EXPORTS = {
     "dispatch": (".ops", "dispatch"),
     "combine": (".ops", "combine"),
@@ -25,6 +26,9 @@ _EXPORTS = {
     "balance_loss": (".training", "balance_loss"),
     "route": (".training", "route"),
     "route_backward": (".training", "route_backward"),
+    "MoEAdapters": (".adapters", "MoEAdapters"),
+    "adapter_add": (".adapters", "adapter_add"),
+    "adapter_swiglu": (".adapters", "adapter_swiglu"),
 }
 
 

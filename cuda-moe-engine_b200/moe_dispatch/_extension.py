@@ -55,6 +55,16 @@ SIGNATURES = {
     "moe_grouped_gemm_swiglu": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]),
     "moe_grouped_gemm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]),
     "moe_grouped_gemm_tile": (ctypes.c_int32, [_I64, _I32]),
+    "moe_adapter_scratch_bytes": (ctypes.c_int64, [_I64, _I64, _I32, _I32]),
+    "moe_adapter_add": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _I64, _P],
+    ),
+    "moe_adapter_swiglu": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _I64, _P],
+    ),
+    "moe_adapter_rows": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I64, _P]),
     "moe_quantize_rows_e4m3": (ctypes.c_int, [_P, _I32, _P, _P, _I64, _I64, _P]),
     "moe_grouped_gemm_swiglu_e4m3": (
         ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]
@@ -433,6 +443,69 @@ class Extension:
             a.device, self.lib.moe_grouped_gemm,
             a.data_ptr(), weight.data_ptr(), offsets.data_ptr(), out.data_ptr(), a.shape[0],
             n_cols, k_dim, experts,
+        )
+
+    # ------------------------------------------------------------- adapters
+    def _adapter(self, function, halves, base, x, a, b, scale, row_adapters, offsets, out):
+        _require(x.is_cuda and x.is_contiguous() and x.dtype == torch.bfloat16 and x.dim() == 2,
+                 "expected contiguous BF16 CUDA x[R,K]")
+        for tensor in (base, a, b, row_adapters, out):
+            _check_cuda(tensor, x, "adapter")
+        rows, k_dim = x.shape
+        _require(a.dim() == 4 and a.shape[3] == k_dim and a.dtype == torch.bfloat16,
+                 "expected BF16 a[P,E,r,K]")
+        adapters, experts, rank = a.shape[:3]
+        _require(out.dim() == 2 and out.shape[0] == rows and out.dtype == torch.bfloat16,
+                 "expected BF16 out[R,N]")
+        n_cols = halves * out.shape[1]
+        _require(tuple(base.shape) == (rows, n_cols) and base.dtype == torch.bfloat16,
+                 "expected BF16 base[R,N]")
+        _require(tuple(b.shape) == (adapters, experts, n_cols, rank) and b.dtype == torch.bfloat16,
+                 "expected BF16 b[P,E,N,r]")
+        _require(row_adapters.shape == (rows,) and row_adapters.dtype == torch.int32,
+                 "expected int32 row_adapters[R]")
+        if scale is not None:
+            _check_cuda(scale, x, "adapter")
+            _require(scale.shape == (adapters,) and scale.dtype == torch.float32,
+                     "expected FP32 scale[P]")
+        if offsets is not None:
+            _check_cuda(offsets, x, "adapter")
+            _require(offsets.shape == (experts + 1,) and offsets.dtype == torch.int32,
+                     "expected int32 offsets[E+1]")
+        index = x.device.index if x.device.index is not None else torch.cuda.current_device()
+        with torch.cuda.device(index):  # the scratch size depends on the device
+            size = int(self.lib.moe_adapter_scratch_bytes(rows, k_dim, rank, adapters))
+            _require(size >= 0, self.lib.moe_last_error().decode())
+            # a buffer of this call's own, as in balance_loss_out
+            scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
+            self._call(
+                x.device, function,
+                base.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(scale),
+                row_adapters.data_ptr(), _ptr(offsets), out.data_ptr(), rows, k_dim, out.shape[1],
+                rank, adapters, experts, scratch.data_ptr(), scratch.numel(),
+            )
+
+    def adapter_add_out(self, base, x, a, b, scale, row_adapters, offsets, out):
+        """out = base + the rows' low-rank adapters (include/moe_b200.h); out may be base."""
+        self._adapter(self.lib.moe_adapter_add, 1, base, x, a, b, scale, row_adapters, offsets, out)
+
+    def adapter_swiglu_out(self, projection, x, a, b, scale, row_adapters, offsets, activated):
+        """SwiGLU of projection + the rows' low-rank adapters (include/moe_b200.h)."""
+        self._adapter(self.lib.moe_adapter_swiglu, 2, projection, x, a, b, scale, row_adapters,
+                      offsets, activated)
+
+    def adapter_rows_out(self, token_adapters, inverse, counts, offsets, row_adapters):
+        """The adapter of every packed row from the tokens' (include/moe_b200.h)."""
+        for tensor in (token_adapters, inverse, counts, offsets, row_adapters):
+            _check_cuda(tensor, inverse, "adapter_rows")
+            _require(tensor.dtype == torch.int32, "adapter rows and indices must be int32")
+        _require(inverse.dim() == 2 and token_adapters.shape == (inverse.shape[0],)
+                 and offsets.numel() == counts.numel() + 1, "expected token_adapters[T], inverse[T,K]")
+        self._call(
+            inverse.device, self.lib.moe_adapter_rows,
+            token_adapters.data_ptr(), inverse.data_ptr(), counts.data_ptr(), offsets.data_ptr(),
+            row_adapters.data_ptr(), inverse.shape[0], inverse.shape[1], counts.numel(),
+            row_adapters.numel(),
         )
 
     # --------------------------------------------------- FP8 (e4m3) experts

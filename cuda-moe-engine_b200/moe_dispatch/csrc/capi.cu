@@ -320,6 +320,91 @@ int moe_swiglu(const void* projection, int32_t dtype, const int32_t* valid_rows,
                        "moe_swiglu");
 }
 
+static int check_adapter_shape(int64_t rows, int64_t k, int32_t rank, int32_t adapters) {
+    if (rows < 0 || rows > INT_MAX / 4) return fail(MOE_ERR_INVALID, "rows must be in 0..INT_MAX / 4");
+    if (k < 8 || k % 8 || k > INT_MAX / 8)
+        return fail(MOE_ERR_INVALID, "adapter dimensions must be positive multiples of 8");
+    if (rank < 8 || rank % 8 || rank > moe::kMaxAdapterRank)
+        return fail(MOE_ERR_INVALID, "rank must be a multiple of 8 up to %d", moe::kMaxAdapterRank);
+    if (adapters < 1 || adapters > moe::kMaxAdapters)
+        return fail(MOE_ERR_INVALID, "adapters must be in 1..%d", moe::kMaxAdapters);
+    return MOE_OK;
+}
+
+int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters) {
+    if (check_adapter_shape(rows, k_dim, rank, adapters) != MOE_OK) return -1;
+    int64_t bytes = 0;
+    if (cuda_status(moe::adapter_scratch_bytes(rows, k_dim, rank, adapters, &bytes),
+                    "moe_adapter_scratch_bytes") != MOE_OK)
+        return -1;
+    return bytes;
+}
+
+static int adapter_common(const void* base, const void* x, const void* a, const void* b,
+                          const float* scale, const int32_t* row_adapters, const int32_t* offsets,
+                          void* out, int64_t rows, int64_t k_dim, int64_t out_cols, int32_t rank,
+                          int32_t adapters, int32_t experts, bool swiglu, void* scratch,
+                          int64_t scratch_bytes, void* stream) {
+    const int checked = check_adapter_shape(rows, k_dim, rank, adapters);
+    if (checked != MOE_OK) return checked;
+    if (out_cols < 8 || out_cols % 8 || out_cols > INT_MAX / 16)
+        return fail(MOE_ERR_INVALID, "adapter dimensions must be positive multiples of 8");
+    if (experts < 1 || experts > moe::kMaxDispatchExperts)
+        return fail(MOE_ERR_INVALID, "experts must be in 1..%d", moe::kMaxDispatchExperts);
+    if (!offsets && experts != 1)
+        return fail(MOE_ERR_INVALID, "offsets may be null for one expert only");
+    if ((rows + 63) / 64 * ((out_cols + 63) / 64) > INT_MAX)
+        return fail(MOE_ERR_INVALID, "shape exceeds the launch grid");
+    if (rows == 0) return MOE_OK;
+    if (!base || !x || !a || !b || !row_adapters || !out) return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(base, 16) || !aligned(x, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(out, 16))
+        return fail(MOE_ERR_INVALID, "adapter operands must be 16-byte aligned");
+    if (swiglu && base == out) return fail(MOE_ERR_INVALID, "out must not be the projection");
+    int64_t need = 0;
+    const int sized = cuda_status(moe::adapter_scratch_bytes(rows, k_dim, rank, adapters, &need), "moe_adapter");
+    if (sized != MOE_OK) return sized;
+    if (!scratch || !aligned(scratch, 256) || scratch_bytes < need)
+        return fail(MOE_ERR_INVALID, "adapter scratch too small or unaligned (%lld bytes needed)",
+                    static_cast<long long>(need));
+    return cuda_status(moe::launch_adapter(base, x, a, b, scale, row_adapters, offsets, out, rows, k_dim,
+                                           swiglu ? 2 * out_cols : out_cols, rank, adapters, experts,
+                                           swiglu, scratch, static_cast<cudaStream_t>(stream)),
+                       swiglu ? "moe_adapter_swiglu" : "moe_adapter_add");
+}
+
+int moe_adapter_add(const void* base, const void* x, const void* a, const void* b, const float* scale,
+                    const int32_t* row_adapters, const int32_t* offsets, void* out, int64_t rows,
+                    int64_t k_dim, int64_t n_cols, int32_t rank, int32_t adapters, int32_t experts,
+                    void* scratch, int64_t scratch_bytes, void* stream) {
+    return adapter_common(base, x, a, b, scale, row_adapters, offsets, out, rows, k_dim, n_cols, rank,
+                          adapters, experts, false, scratch, scratch_bytes, stream);
+}
+
+int moe_adapter_swiglu(const void* projection, const void* x, const void* a, const void* b,
+                       const float* scale, const int32_t* row_adapters, const int32_t* offsets,
+                       void* activated, int64_t rows, int64_t hidden, int64_t intermediate, int32_t rank,
+                       int32_t adapters, int32_t experts, void* scratch, int64_t scratch_bytes,
+                       void* stream) {
+    return adapter_common(projection, x, a, b, scale, row_adapters, offsets, activated, rows, hidden,
+                          intermediate, rank, adapters, experts, true, scratch, scratch_bytes, stream);
+}
+
+int moe_adapter_rows(const int32_t* token_adapters, const int32_t* inverse, const int32_t* counts,
+                     const int32_t* offsets, int32_t* row_adapters, int64_t tokens, int32_t topk,
+                     int32_t experts, int64_t rows, void* stream) {
+    if (tokens < 0 || topk < 1 || topk > moe::kMaxTopk || tokens * topk > INT_MAX || rows < 0)
+        return fail(MOE_ERR_INVALID, "shape exceeds int32 indexing capacity");
+    if (experts < 1 || experts > moe::kMaxDispatchExperts)
+        return fail(MOE_ERR_INVALID, "experts must be in 1..%d", moe::kMaxDispatchExperts);
+    if (rows == 0) return MOE_OK;
+    if (!counts || !offsets || !row_adapters || (tokens > 0 && (!token_adapters || !inverse)))
+        return fail(MOE_ERR_INVALID, "null pointer");
+    return cuda_status(moe::launch_adapter_rows(token_adapters, inverse, counts, offsets, row_adapters,
+                                                tokens, topk, experts, rows,
+                                                static_cast<cudaStream_t>(stream)),
+                       "moe_adapter_rows");
+}
+
 static int grouped_gemm_common(const void* a, const void* w, const int32_t* offsets, void* out,
                                int64_t rows, int64_t n_out, int64_t k_dim, int32_t experts,
                                bool swiglu, void* stream) {

@@ -46,6 +46,18 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
                                   cudaStream_t stream, const char** error);
 cudaError_t read_route_backward_status(int32_t* code, bool clear);
 
+// Low-rank adapters beside the grouped projections (adapter.cu).
+constexpr int kMaxAdapters = 512;
+constexpr int kMaxAdapterRank = 128;
+cudaError_t adapter_scratch_bytes(int64_t rows, int64_t k, int rank, int adapters, int64_t* bytes);
+cudaError_t launch_adapter(const void* base, const void* x, const void* a, const void* b,
+                           const float* scale, const int32_t* row_adapters, const int32_t* offsets,
+                           void* out, int64_t rows, int64_t k, int64_t n, int rank, int adapters,
+                           int experts, bool swiglu, void* scratch, cudaStream_t stream);
+cudaError_t launch_adapter_rows(const int32_t* token_adapters, const int32_t* inverse,
+                                const int32_t* counts, const int32_t* offsets, int32_t* row_adapters,
+                                int64_t tokens, int topk, int experts, int64_t rows, cudaStream_t stream);
+
 int64_t dispatch_scratch_bytes(int64_t assignments, int experts);
 cudaError_t launch_dispatch(const void* x, int dtype, const int32_t* ids, int32_t* counts,
                             int32_t* offsets, int32_t* slots, void* packed, int32_t* inverse,

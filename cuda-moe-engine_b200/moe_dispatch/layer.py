@@ -21,6 +21,7 @@ to 32).  Every stage runs a kernel from libmoe_b200.so:
 from dataclasses import dataclass
 import math
 import torch
+from .adapters import adapter_ids32, check_adapters
 from .workspace import CudaWorkspace
 from ._extension import get_extension
 
@@ -93,6 +94,9 @@ class LayerWorkspace:
     expert_output: torch.Tensor
     packed_q: torch.Tensor = None      # e4m3 copy of the packed rows (expert_dtype="fp8_e4m3")
     packed_scale: torch.Tensor = None  # their per-row dequantisation scales
+    # buffers of the adapters' forward pass, made at its first call
+    row_adapters: torch.Tensor = None
+    adapter_projection: torch.Tensor = None
 
 
 def check_out(out, x):
@@ -164,6 +168,7 @@ class MoEBlock(torch.nn.Module):
         self.register_buffer("routing_bias", torch.zeros(self.config.experts, device=device))
         self._workspaces = {}
         self._route_buffers = {}
+        self.adapters = None
         self.extension = get_extension()
         if expert_dtype == "fp8_e4m3":
             # gate/up weights in e4m3 with one scale per output channel (weight row);
@@ -182,6 +187,15 @@ class MoEBlock(torch.nn.Module):
         self.routing_bias.zero_()
         if pattern == "skewed":
             self.routing_bias[: self.config.topk] = 5.0
+
+    def set_adapters(self, adapters):
+        """Low-rank adapters (MoEAdapters, or None) that forward(adapter_ids=...) picks from.
+
+        A graph captured before keeps reading the tensors that were set then: keep
+        them alive, or capture again."""
+        if adapters is not None:
+            check_adapters(adapters, self.config, self.gate_up_weight.device)
+        self.adapters = adapters
 
     def route(self, x):
         """fp32 logits, top-k with ties to the lower index, softmax of the selected scores."""
@@ -226,48 +240,88 @@ class MoEBlock(torch.nn.Module):
             )
         return self._workspaces[key]
 
-    def experts_forward(self, state):
+    def _adapter_buffers(self, state):
+        """The adapters' row ids and unfused projection of this workspace."""
+        rows, device = state.transport.capacity_rows, state.transport.packed.device
+        if state.row_adapters is None:
+            state.row_adapters = torch.empty(rows, device=device, dtype=torch.int32)
+        if state.adapter_projection is None and self.adapters.gate_up_a is not None:
+            state.adapter_projection = (
+                state.projection if state.projection.shape[0] else torch.empty(
+                    (rows, 2 * self.config.intermediate), device=device,
+                    dtype=state.transport.dtype))
+
+    def experts_forward(self, state, adapter_ids=None):
+        """Expert outputs of the packed rows.  With adapter_ids [T] int32 the rows'
+        adapters change both projections: the gate/up projection is then written
+        out (unfused), and its adapters' kernel applies the SwiGLU."""
         transport = state.transport
         ext = self.extension
+        adapters = None
+        if adapter_ids is not None:
+            adapters = self.adapters
+            self._adapter_buffers(state)
+            ext.adapter_rows_out(adapter_ids, transport.inverse, transport.counts, transport.offsets,
+                                 state.row_adapters)
+        gate_up_adapters = adapters is not None and adapters.gate_up_a is not None
+        fused = self.implementation == "cuda_fused" and not gate_up_adapters
+        projection = state.adapter_projection if gate_up_adapters else state.projection
         if self.expert_dtype == "fp8_e4m3":
             # per-row e4m3 activations, e4m3 gate/up GEMM dequantised in its epilogue
             ext.quantize_rows_e4m3(transport.packed, state.packed_q, state.packed_scale)
-            if self.implementation == "cuda_fused":
+            if fused:
                 ext.grouped_gemm_swiglu_e4m3_out(state.packed_q, state.packed_scale, self.gate_up_q,
                                                  self.gate_up_scale, transport.offsets,
                                                  state.activated)
             else:
                 ext.grouped_gemm_e4m3_out(state.packed_q, state.packed_scale, self.gate_up_q,
-                                          self.gate_up_scale, transport.offsets, state.projection)
-                ext.swiglu_out(state.projection, transport.offsets[-1:], state.activated)
-        elif self.implementation == "cuda_fused":
+                                          self.gate_up_scale, transport.offsets, projection)
+        elif fused:
             ext.grouped_gemm_swiglu_out(
                 transport.packed, self.gate_up_weight, transport.offsets, state.activated
             )
         else:
             ext.grouped_gemm_out(
-                transport.packed, self.gate_up_weight, transport.offsets, state.projection
+                transport.packed, self.gate_up_weight, transport.offsets, projection
             )
-            ext.swiglu_out(state.projection, transport.offsets[-1:], state.activated)
+        if gate_up_adapters:
+            ext.adapter_swiglu_out(projection, transport.packed, adapters.gate_up_a,
+                                   adapters.gate_up_b, adapters.scale, state.row_adapters,
+                                   transport.offsets, state.activated)
+        elif not fused:
+            ext.swiglu_out(projection, transport.offsets[-1:], state.activated)
         ext.grouped_gemm_out(
             state.activated, self.down_weight, transport.offsets, state.expert_output
         )
+        if adapters is not None and adapters.down_a is not None:
+            ext.adapter_add_out(state.expert_output, state.activated, adapters.down_a,
+                                adapters.down_b, adapters.scale, state.row_adapters,
+                                transport.offsets, state.expert_output)
         return state.expert_output
 
     @torch.inference_mode()
-    def forward(self, x, out=None):
+    def forward(self, x, out=None, *, adapter_ids=None):
         """Block output for x[T,hidden].  Without `out` the result is the
         workspace's reusable output view; with `out` (a contiguous [T,hidden]
-        tensor of x's dtype and device) the combine writes there instead."""
+        tensor of x's dtype and device) the combine writes there instead.
+        adapter_ids [T] (int32 or int64) picks each token's adapter from those of
+        set_adapters; ids outside them (say -1) pick none, which gives such a
+        token the bits that it has without adapters."""
         if x.ndim != 2 or x.shape[1] != self.config.hidden or not x.is_contiguous():
             raise ValueError("expected contiguous x[T,hidden]")
         if x.dtype != self.gate_up_weight.dtype or x.device != self.gate_up_weight.device:
             raise ValueError("input dtype/device must match expert weights")
         check_out(out, x)
+        if adapter_ids is not None:
+            if self.adapters is None:
+                raise ValueError("adapter_ids need adapters: call set_adapters first")
+            if adapter_ids.device != x.device:
+                raise ValueError("adapter_ids must be on x's device")
+            adapter_ids = adapter_ids32(adapter_ids, x.shape[0], "token")
         if x.shape[0] == 0:
             return torch.empty_like(x) if out is None else out
         state = self.workspace(x)
         ids32, ids64, weights = self.route(x)
         state.transport.dispatch(x, ids32, ids64)
-        output = self.experts_forward(state)
+        output = self.experts_forward(state, adapter_ids)
         return state.transport.combine(output, weights, out)

@@ -30,6 +30,13 @@ def _check_ids(expert_ids, tokens, like):
         raise ValueError("all tensors must be on the same device")
 
 
+def _ids32(expert_ids):
+    """Contiguous int32 ids; int64 values past int32 stay out of range."""
+    if expert_ids.dtype == torch.int64:
+        expert_ids = expert_ids.clamp(-1, 2**31 - 1).to(torch.int32)
+    return expert_ids.contiguous()
+
+
 def _check_bias(bias, experts, like):
     if bias is None:
         return
@@ -110,7 +117,7 @@ def balance_loss(logits, expert_ids, *, bias=None, token_mask=None, coefficient=
             raise ValueError("all tensors must be on the same device")
         token_mask = token_mask.contiguous()
     _require_cuda(logits, "balance_loss")
-    return _BalanceLoss.apply(logits, expert_ids.to(torch.int32).contiguous(), bias, token_mask,
+    return _BalanceLoss.apply(logits, _ids32(expert_ids), bias, token_mask,
                               float(coefficient))
 
 
@@ -211,5 +218,5 @@ def route_backward(x, router_weight, expert_ids, weights, grad_weights, grad_log
             raise ValueError(f"{name} must be contiguous")
     _require_cuda(x, "route_backward")
     with torch.no_grad():
-        return _route_backward(x, router_weight, expert_ids.to(torch.int32).contiguous(), weights,
+        return _route_backward(x, router_weight, _ids32(expert_ids), weights,
                                grad_weights, grad_logits, True, True)

@@ -196,6 +196,46 @@ int moe_grouped_gemm_swiglu(const void* packed, const void* gate_up, const int32
 int moe_grouped_gemm(const void* a, const void* weight, const int32_t* offsets, void* out,
                      int64_t rows, int64_t n_cols, int64_t k_dim, int32_t experts, void* stream);
 
+/* ---------------------------------------------------------------- adapters
+ * Low-rank adapters of many requests beside the grouped projections (no
+ * counterpart in the reference).  bf16. */
+
+/* out[r] = bf16(base[r] + scale[p] * (x[r] . a[p,e]^T) . b[p,e]^T) for every
+ * row r of expert e's span [offsets[e], offsets[e+1]), p = row_adapters[r];
+ * rows whose p is outside [0, adapters) get base[r].  Rows at or past
+ * offsets[experts] are neither read nor written.  offsets NULL: one expert with
+ * every row.  base, out [rows, n_cols] (out may be base itself, and must not
+ * overlap any operand otherwise); x [rows, k_dim]; a [adapters, experts, rank,
+ * k_dim]; b [adapters, experts, n_cols, rank]; scale [adapters] fp32 or NULL (1).
+ * x . a^T is summed in fp32 and used to 2^-16 of its value or better; one
+ * rounding to bf16 at the end.  What is not finite in one adapter or row does
+ * not reach rows of others.  k_dim, n_cols multiples of 8; rank a multiple of 8
+ * up to 128; adapters <= 512.  scratch: 256-byte aligned, not initialised, sized
+ * for the current device; calls that may overlap in time need one each. */
+int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters);
+int moe_adapter_add(const void* base, const void* x, const void* a, const void* b, const float* scale,
+                    const int32_t* row_adapters, const int32_t* offsets, void* out, int64_t rows,
+                    int64_t k_dim, int64_t n_cols, int32_t rank, int32_t adapters, int32_t experts,
+                    void* scratch, int64_t scratch_bytes, void* stream);
+
+/* The gate/up form: with y = projection + the adapters' product as above over
+ * 2 * intermediate columns (not rounded in between),
+ * activated[r, c] = bf16(silu(y[r, c]) * y[r, intermediate + c]).  For a row
+ * without an adapter the bits of moe_swiglu.  b [adapters, experts,
+ * 2 * intermediate, rank]; activated [rows, intermediate] apart from projection. */
+int moe_adapter_swiglu(const void* projection, const void* x, const void* a, const void* b,
+                       const float* scale, const int32_t* row_adapters, const int32_t* offsets,
+                       void* activated, int64_t rows, int64_t hidden, int64_t intermediate, int32_t rank,
+                       int32_t adapters, int32_t experts, void* scratch, int64_t scratch_bytes,
+                       void* stream);
+
+/* The adapter of each packed row after moe_dispatch: row_adapters[inverse[t,k]] =
+ * token_adapters[t], and -1 for the padding rows of every span.  Rows at or past
+ * `rows` or offsets[experts] are not written. */
+int moe_adapter_rows(const int32_t* token_adapters, const int32_t* inverse, const int32_t* counts,
+                     const int32_t* offsets, int32_t* row_adapters, int64_t tokens, int32_t topk,
+                     int32_t experts, int64_t rows, void* stream);
+
 /* ------------------------------------------------------ FP8 (e4m3) experts
  * No counterpart in the reference, whose experts are bf16 only
  * (layer.py:97-98): an extension on tcgen05.mma.kind::f8f6f4. */
