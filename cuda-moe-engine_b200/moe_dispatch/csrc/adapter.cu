@@ -19,13 +19,16 @@
 // Many rows: rows that share a pair (p, e) share its weights through tiles.
 //   count_kernel, order_kernel  stable counting sort of the rows by adapter.  Rows
 //       come expert by expert, so the sorted rows are grouped by (p, e).
-//   shrink_tile_kernel  64 sorted rows x rank, K in 64-wide cp.async stages; a
-//       tile walks the runs of equal pairs inside it as one pipelined sequence
-//   expand_tile_kernel  64 sorted rows x 128 columns; s enters the tensor cores as
-//       two bf16 parts (s to 2^-16), base is added in fp32; each run of a tile finishes
-//       its own rows, so what is not finite in one adapter stays in its rows
+//   tiles_kernel        cuts each group into tiles of up to 64 rows.  (Tiles over 64
+//       consecutive sorted rows, whatever groups they touch, were measured first: a
+//       few tiles with 26 small groups held everything up, 1080 us against 420 at
+//       16384 tokens, 64 experts, top-6, 32 adapters of rank 32.)
+//   shrink_tile_kernel  a tile's rows x rank, K in 128-wide cp.async stages
+//   expand_tile_kernel  a tile's rows x column blocks of 128; s enters the tensor
+//       cores as two bf16 parts (s to 2^-16), base is added in fp32
 // Both use mma.sync: at rank <= 64 a 64-row tile does at most 64 flop per byte
-// moved, far below what the tensor cores need to be the bound.
+// moved, far below what the tensor cores need to be the bound.  A tile holds one
+// adapter's rows only, so what is not finite in one adapter or row stays there.
 //
 // Nothing depends on where a row lands in a tile: its products are its own, so
 // results do not change with the batch around it, except between the two forms
@@ -50,6 +53,8 @@ struct Adapter {
     int64_t rows, k, n, cols;     // cols: output columns (n, or n / 2 with SwiGLU)
     int rank, adapters, experts;
     int32_t *table, *order, *keys;
+    int32_t* tile_count;
+    int2* tiles;                  // {first sorted row, rows} of each tile
     float* s;                     // [splits][rows][padded rank]
     int splits;
     int64_t split_k;              // K elements per split
@@ -217,6 +222,7 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const Adapter p, in
     for (int i = threadIdx.x; i < buckets; i += kSortThreads) counts[i] = 0;
     pdl_wait();
     __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.tile_count = 0;
     const int64_t valid = valid_rows(p);
     const int64_t begin = blockIdx.x * chunk_rows;
     const int64_t end = begin + chunk_rows < p.rows ? begin + chunk_rows : p.rows;
@@ -312,7 +318,7 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const Adapter p, in
 // ------------------------------------------------------------ many rows: tiles
 
 constexpr int kTileRows = 64;
-constexpr int kTileThreads = 128;  // four warps, 16 rows each
+constexpr int kTileThreads = 128;  // of the shrink kernel: four warps, 16 rows each
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -344,160 +350,176 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The rows of a tile and the runs of equal pairs among them.  Rows without an
-// adapter stand behind all others, so a run ends where the next begins.
-struct TileRows {
-    int32_t key[kTileRows];
-    int32_t row[kTileRows];
-    int32_t run[kTileRows + 1];  // first row of each run, then the end of the last
-    int32_t runs;
-    uint32_t starts[2], has[2];
-};
-
-__device__ __forceinline__ void load_tile_rows(const Adapter& p, int64_t tile, TileRows& t) {
-    const int tid = threadIdx.x;
-    if (tid < kTileRows) {
-        const int64_t at = tile * kTileRows + tid;
-        const int key = at < p.rows ? p.keys[at] : kOutside;
-        t.key[tid] = key;
-        t.row[tid] = at < p.rows ? p.order[at] : 0;
-    }
-    __syncthreads();
-    bool start = false;
-    if (tid < kTileRows) {
-        const int key = t.key[tid];
-        start = key >= 0 && (tid == 0 || key != t.key[tid - 1]);
-        const uint32_t s = __ballot_sync(0xffffffffu, start), h = __ballot_sync(0xffffffffu, key >= 0);
-        if ((tid & 31) == 0) {
-            t.starts[tid >> 5] = s;
-            t.has[tid >> 5] = h;
+// Cuts the sorted rows' groups of equal keys into tiles.  A thread whose key
+// differs from the one before starts a group; where the next start lies in the
+// same warp the group's length is known, and the warp searches the end of its
+// last group together (32 probes at a time).  Tiles land in any order: each is
+// a piece of work of its own.  none: rows without an adapter need tiles too.
+__global__ void __launch_bounds__(256) tiles_kernel(const Adapter p, bool none) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t at = blockIdx.x * 256ll + threadIdx.x;
+    const int key = at < p.rows ? p.keys[at] : kOutside;
+    const bool start = at < p.rows && (at == 0 || p.keys[at - 1] != key);
+    const uint32_t starts = __ballot_sync(0xffffffffu, start);
+    if (starts == 0) return;
+    const int last = 31 - __clz(starts);
+    const uint32_t later = lane == 31 ? 0 : starts >> (lane + 1);
+    int64_t length = start && later ? __ffs(later) : 0;
+    const int last_key = __shfl_sync(0xffffffffu, key, last);
+    const int64_t last_at = at - lane + last;
+    int64_t lo = at - lane + 32, hi = p.rows;  // keys[lo - 1] is last_key; the end lies in [lo, hi]
+    if (lo > hi) lo = hi;
+    while (lo < hi) {
+        const int64_t step = (hi - lo + 31) / 32;
+        const int64_t probe = lo + step * (lane + 1) - 1;
+        const uint32_t past = __ballot_sync(0xffffffffu, probe >= hi || p.keys[probe] != last_key);
+        if (past == 0) {
+            lo = hi;
+        } else {
+            const int f = __ffs(past) - 1;
+            const int64_t bound = lo + step * (f + 1) - 1;
+            if (bound < hi) hi = bound;
+            lo += step * f;
         }
     }
-    __syncthreads();
-    const int runs = __popc(t.starts[0]) + __popc(t.starts[1]);
-    if (start) {
-        const int before = (tid >= 32 ? __popc(t.starts[0]) : 0) +
-                           __popc(t.starts[tid >> 5] & ((1u << (tid & 31)) - 1u));
-        t.run[before] = tid;
+    if (lane == last) length = lo - last_at;
+    const bool wanted = start && (key >= 0 || (none && key == kNone));
+    const int count = wanted ? static_cast<int>((length + kTileRows - 1) / kTileRows) : 0;
+    int inclusive = count;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inclusive, off);
+        if (lane >= off) inclusive += y;
     }
-    if (tid == 0) {
-        t.run[runs] = __popc(t.has[0]) + __popc(t.has[1]);
-        t.runs = runs;
+    const int total = __shfl_sync(0xffffffffu, inclusive, 31);
+    int first = 0;
+    if (lane == 0 && total > 0) first = atomicAdd(p.tile_count, total);
+    first = __shfl_sync(0xffffffffu, first, 0);
+    if (count > 0 && lane != last)  // at most 31 rows: one tile
+        p.tiles[first + inclusive - 1] = make_int2(static_cast<int>(at), static_cast<int>(length));
+    const int last_count = __shfl_sync(0xffffffffu, count, last);
+    for (int i = lane; i < last_count; i += 32) {
+        const int64_t row = last_at + static_cast<int64_t>(i) * kTileRows;
+        const int64_t rest = lo - row;
+        p.tiles[first + total - last_count + i] =
+            make_int2(static_cast<int>(row), static_cast<int>(rest < kTileRows ? rest : kTileRows));
     }
-    __syncthreads();
 }
 
-constexpr int kShrinkStages = 4;
-template <int RN> constexpr int shrink_stage_bytes() { return (kTileRows + RN) * 128; }
+constexpr int kShrinkStages = 3;
+constexpr int kShrinkK = 128;                   // K elements per stage: 256 bytes of each row
+constexpr int kShrinkRow = kShrinkK * 2;
+template <int RN> constexpr int shrink_stage_bytes() { return (kTileRows + RN) * kShrinkRow; }
+
+// 16-byte chunk c of row i of a stage: the low three bits are swizzled by the
+// row, so the eight rows of an ldmatrix lie in different banks.
+__device__ __forceinline__ uint32_t stage_at(int i, int c) { return i * kShrinkRow + ((c ^ (i & 7)) << 4); }
 
 // RN: rank rounded up to 8, 16, 32, 64 or 128; columns past the rank are zero.
+// CTAs walk the (tile, K split) pairs with the grid's stride.
 template <int RN>
 __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter p) {
     extern __shared__ __align__(128) uint8_t stages[];
-    __shared__ TileRows t;
+    constexpr int kChunks = kShrinkK / 8, kPass = kTileThreads / kChunks;  // rows copied at a time
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int c = tid % kChunks, i_first = tid / kChunks;  // this thread copies chunk c of every kPass-th row
     pdl_trigger();
     pdl_wait();
-    load_tile_rows(p, blockIdx.x, t);
-    const int runs = t.runs;
-    if (runs == 0) return;
-    const int64_t k0 = blockIdx.y * p.split_k;
-    const int64_t k1 = k0 + p.split_k < p.k ? k0 + p.split_k : p.k;
-    const int steps = static_cast<int>((k1 - k0 + 63) / 64);
-    const int total = runs * steps;
-
-    int load_run = 0, load_step = 0;
-    auto load = [&](int slot) {  // one 64-wide K step of one run
-        const uint32_t at = smem_addr(stages) + slot * shrink_stage_bytes<RN>();
-        const int i0 = t.run[load_run], i1 = t.run[load_run + 1];
-        const int64_t kc = k0 + load_step * 64;
+    const int items = *p.tile_count * p.splits;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int2 tile = p.tiles[item / p.splits];
+        const int split = item % p.splits;
+        const int key = p.keys[tile.x];
+        if (key < 0) continue;  // rows without an adapter
+        const int64_t k0 = split * p.split_k;
+        const int64_t k1 = k0 + p.split_k < p.k ? k0 + p.split_k : p.k;
+        const int steps = static_cast<int>((k1 - k0 + kShrinkK - 1) / kShrinkK);
+        const bf16* rows[kTileRows / kPass];
 #pragma unroll
-        for (int j = 0; j < kTileRows * 8 / kTileThreads; ++j) {
-            const int i = (tid + j * kTileThreads) >> 3, c = tid & 7;
-            if (i < i0 || i >= i1) continue;  // rows of other runs: products nobody stores
-            const bool in = kc + c * 8 < k1;
-            copy16(at + i * 128 + ((c ^ (i & 7)) << 4),
-                   p.x + static_cast<int64_t>(t.row[i]) * p.k + (in ? kc + c * 8 : 0), in);
+        for (int j = 0; j < kTileRows / kPass; ++j) {
+            const int i = i_first + j * kPass;
+            rows[j] = p.x + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.k + k0 + c * 8;
         }
-        const bf16* a = p.a + static_cast<int64_t>(t.key[i0]) * p.rank * p.k;
-        for (int i = tid >> 3; i < RN; i += kTileThreads / 8) {
-            const int c = tid & 7;
-            const bool in = i < p.rank && kc + c * 8 < k1;
-            copy16(at + kTileRows * 128 + i * 128 + ((c ^ (i & 7)) << 4),
-                   a + (in ? i * p.k + kc + c * 8 : 0), in);
+        const bf16* a = p.a + (static_cast<int64_t>(key) * p.rank + i_first) * p.k + k0 + c * 8;
+        auto load = [&](int slot, int step) {
+            const uint32_t at = smem_addr(stages) + slot * shrink_stage_bytes<RN>();
+            const int kc = step * kShrinkK;
+            const bool in = k0 + kc + c * 8 < k1;
+#pragma unroll
+            for (int j = 0; j < kTileRows / kPass; ++j) {
+                const int i = i_first + j * kPass;
+                if (i < tile.y)  // what stands in the other rows is multiplied, and stored nowhere
+                    copy16(at + stage_at(i, c), in ? rows[j] + kc : p.x, in);
+            }
+#pragma unroll
+            for (int j = 0; j < (RN + kPass - 1) / kPass; ++j) {
+                const int i = i_first + j * kPass;
+                const bool here = in && i < p.rank;
+                if (i < RN) copy16(at + kTileRows * kShrinkRow + stage_at(i, c),
+                                   here ? a + static_cast<int64_t>(j * kPass) * p.k + kc : p.a, here);
+            }
+        };
+        __syncthreads();  // the item before has read its stages
+#pragma unroll
+        for (int s = 0; s < kShrinkStages - 1; ++s) {
+            if (s < steps) load(s, s);
+            copy_commit();
         }
-        if (++load_step == steps) {
-            load_step = 0;
-            ++load_run;
-        }
-    };
+        float acc[RN / 8][4] = {};
+        int slot = 0, load_slot = kShrinkStages - 1;
+        for (int step = 0; step < steps; ++step) {
+            copy_wait<kShrinkStages - 2>();
+            __syncthreads();  // this stage has landed everywhere, and the one before has been read
+            if (step + kShrinkStages - 1 < steps) load(load_slot, step + kShrinkStages - 1);
+            copy_commit();
+            if (warp * 16 < tile.y) {
+                const uint32_t xs = smem_addr(stages) + slot * shrink_stage_bytes<RN>();
+                const uint32_t as = xs + kTileRows * kShrinkRow;
 #pragma unroll
-    for (int s = 0; s < kShrinkStages - 1; ++s) {
-        if (s < total) load(s);
-        copy_commit();
-    }
-    float acc[RN / 8][4] = {};
-    int run = 0, step = 0;
-    for (int it = 0; it < total; ++it) {
-        copy_wait<kShrinkStages - 2>();
-        __syncthreads();  // stage `it` has landed everywhere, and stage it - 1 has been read
-        if (it + kShrinkStages - 1 < total) load((it + kShrinkStages - 1) % kShrinkStages);
-        copy_commit();
-        const int i0 = t.run[run], i1 = t.run[run + 1];
-        if (warp * 16 < i1 && warp * 16 + 16 > i0) {
-            const uint32_t xs = smem_addr(stages) + (it % kShrinkStages) * shrink_stage_bytes<RN>();
-            const uint32_t as = xs + kTileRows * 128;
+                for (int kk = 0; kk < kShrinkK / 16; ++kk) {
+                    uint32_t xf[4];
+                    ldmatrix4(xs + stage_at(warp * 16 + (lane & 15), kk * 2 + (lane >> 4)), xf);
+                    if constexpr (RN == 8) {
+                        uint32_t af[2];
+                        ldmatrix2(as + stage_at(lane & 7, kk * 2 + ((lane >> 3) & 1)), af);
+                        mma16816(acc[0], xf, af[0], af[1]);
+                    } else {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-                uint32_t xf[4];
-                const int i = warp * 16 + (lane & 15);
-                ldmatrix4(xs + i * 128 + (((kk * 2 + (lane >> 4)) ^ (i & 7)) << 4), xf);
-                if constexpr (RN == 8) {
-                    uint32_t af[2];
-                    const int n = lane & 7;
-                    ldmatrix2(as + n * 128 + (((kk * 2 + ((lane >> 3) & 1)) ^ (n & 7)) << 4), af);
-                    mma16816(acc[0], xf, af[0], af[1]);
-                } else {
-#pragma unroll
-                    for (int n0 = 0; n0 < RN; n0 += 16) {
-                        uint32_t af[4];
-                        const int n = n0 + (lane & 7) + ((lane >> 4) << 3);
-                        ldmatrix4(as + n * 128 + (((kk * 2 + ((lane >> 3) & 1)) ^ (n & 7)) << 4), af);
-                        mma16816(acc[n0 / 8], xf, af[0], af[1]);
-                        mma16816(acc[n0 / 8 + 1], xf, af[2], af[3]);
+                        for (int n0 = 0; n0 < RN; n0 += 16) {
+                            uint32_t af[4];
+                            ldmatrix4(as + stage_at(n0 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), af);
+                            mma16816(acc[n0 / 8], xf, af[0], af[1]);
+                            mma16816(acc[n0 / 8 + 1], xf, af[2], af[3]);
+                        }
                     }
                 }
             }
-            if (step == steps - 1) {
-                const int64_t first = static_cast<int64_t>(blockIdx.y) * p.rows + blockIdx.x * static_cast<int64_t>(kTileRows);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int i = warp * 16 + (lane >> 2) + 8 * h;
-                    if (i < i0 || i >= i1) continue;
-                    float* s = p.s + (first + i) * RN + 2 * (lane & 3);
-#pragma unroll
-                    for (int n = 0; n < RN / 8; ++n)
-                        *reinterpret_cast<float2*>(s + n * 8) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
-                }
-#pragma unroll
-                for (int n = 0; n < RN / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-            }
+            if (++slot == kShrinkStages) slot = 0;
+            if (++load_slot == kShrinkStages) load_slot = 0;
         }
-        if (++step == steps) {
-            step = 0;
-            ++run;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = warp * 16 + (lane >> 2) + 8 * h;
+            if (i >= tile.y) continue;
+            float* s = p.s + (split * p.rows + tile.x + i) * RN + 2 * (lane & 3);
+#pragma unroll
+            for (int n = 0; n < RN / 8; ++n)
+                *reinterpret_cast<float2*>(s + n * 8) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
         }
     }
     copy_wait<0>();
 }
 
-constexpr int kTileCols = 128;                        // rows of B per tile: 128 columns, or 64 gate + 64 up
+constexpr int kExpandThreads = 256;                   // 4 x 16 rows, 2 halves of the columns
+constexpr int kExpandStages = 3;
+constexpr int kTileCols = 128;                        // rows of B per step: 128 columns, or 64 gate + 64 up
 constexpr int kBaseStride = kTileCols * 2 + 16;       // bytes; the pads keep ldmatrix and row stores conflict-free
 template <int RN> constexpr int rank_k() { return RN < 16 ? 16 : RN; }
 template <int RN> constexpr int b_stride() { return rank_k<RN>() * 2 + 16; }
-template <int RN> constexpr int s_stride() { return rank_k<RN>() + 8; }  // floats
 template <int RN> constexpr int expand_smem() {
-    return kTileRows * kBaseStride + 2 * kTileCols * b_stride<RN>() + kTileRows * s_stride<RN>() * 4;
+    return kExpandStages * (kTileRows * kBaseStride + kTileCols * b_stride<RN>());
 }
 
 // Two floats as bf16 hi parts, and the rests' as a second register.
@@ -507,139 +529,156 @@ __device__ __forceinline__ void split2(float2 v, uint32_t& hi, uint32_t& lo) {
     lo = pack_bf16x2(v.x - bf16_bits_to_f32(a), v.y - bf16_bits_to_f32(b));
 }
 
+// silu(g) u from the fast exponential and reciprocal, within 2^-21 of the value
+// for |g| up to 88 (the rounding to bf16 is 2^-8); beyond that 0 or g u, as it is.
+__device__ __forceinline__ float fast_silu_times(float g, float u) {
+    return __fdividef(g, 1.0f + __expf(-g)) * u;
+}
+
+// CTAs walk the (tile, group of `per` column blocks) pairs with the grid's
+// stride.  The blocks of a group form one cp.async pipeline whose stages hold the
+// tile's base rows and the pair's rows of B; s stays in registers as bf16 fragments.
 template <int RN, bool SWIGLU>
-__global__ void __launch_bounds__(kTileThreads) expand_tile_kernel(const Adapter p, int blocks) {
+__global__ void __launch_bounds__(kExpandThreads)
+expand_tile_kernel(const Adapter p, int blocks, int per, int groups) {
     constexpr int RK = rank_k<RN>();
+    constexpr int kOut = SWIGLU ? kTileCols / 2 : kTileCols;  // output columns of a block
+    constexpr int kStage = kTileRows * kBaseStride + kTileCols * b_stride<RN>();
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ TileRows t;
-    uint8_t* base_s = smem;
-    uint8_t* b_s = smem + kTileRows * kBaseStride;
-    float* s_s = reinterpret_cast<float*>(b_s + 2 * kTileCols * b_stride<RN>());
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t tile = blockIdx.x / blocks;
-    constexpr int kOut = SWIGLU ? kTileCols / 2 : kTileCols;  // output columns of the tile
-    const int64_t c0 = static_cast<int64_t>(blockIdx.x % blocks) * kOut;
+    const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, half = tid >> 7;
+    // this thread's share of the base rows: one 16-byte chunk of rows i_first + 16 j
+    const int c = (tid & 15) * 8, i_first = tid >> 4;
+    const int c_col = SWIGLU ? c & 63 : c;  // its column inside the block
+    const int r0 = warp * 16 + (lane >> 2);
     pdl_trigger();
     pdl_wait();
-    load_tile_rows(p, tile, t);
-    const int runs = t.runs;
-    if (t.key[0] == kOutside) return;  // and so are all behind it
-    if (runs == 0 && !SWIGLU && p.out == p.base) return;
-
-    // row c of the tile's B: column c0 + c, or with SwiGLU the gate and up columns
-    auto column = [&](int c) -> int64_t {
-        return SWIGLU ? c0 + (c & 63) + (c >= 64 ? p.cols : 0) : c0 + c;
-    };
-    auto inside = [&](int c) { return c0 + (SWIGLU ? c & 63 : c) < p.cols; };
-    // base: each warp its own 16 rows
+    const int items = *p.tile_count * groups;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int2 tile = p.tiles[item / groups];
+        const int first_block = (item % groups) * per;
+        const int count = min(per, blocks - first_block);
+        const int key = p.keys[tile.x];
+        const bf16* base[kTileRows / 16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int i = warp * 16 + j * 2 + (lane >> 4), c = (lane & 15) * 8;
-        if (t.key[i] != kOutside && inside(c))
-            copy16(smem_addr(base_s) + i * kBaseStride + c * 2,
-                   p.base + static_cast<int64_t>(t.row[i]) * p.n + column(c), true);
-    }
-    auto load_b = [&](int run, int slot) {
-        const bf16* b = p.b + static_cast<int64_t>(t.key[t.run[run]]) * p.n * p.rank;
-        const uint32_t at = smem_addr(b_s) + slot * kTileCols * b_stride<RN>();
-        constexpr int kChunks = RK / 8;
-        for (int i = tid; i < kTileCols * kChunks; i += kTileThreads) {
-            const int c = i / kChunks, q = i % kChunks;
-            const bool in = q * 8 < p.rank && inside(c);
-            copy16(at + c * b_stride<RN>() + q * 16, b + (in ? column(c) * p.rank + q * 8 : 0), in);
+        for (int j = 0; j < kTileRows / 16; ++j) {
+            const int i = i_first + 16 * j;
+            base[j] = p.base + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.n + c_col +
+                      (SWIGLU && c >= 64 ? p.cols : 0);
         }
-    };
-    if (runs > 0) load_b(0, 0);
-    copy_commit();
+        auto load = [&](int slot, int block) {
+            const int64_t c0 = static_cast<int64_t>(block) * kOut;
+            const uint32_t at = smem_addr(smem) + slot * kStage;
+            if (c0 + c_col < p.cols) {
+#pragma unroll
+                for (int j = 0; j < kTileRows / 16; ++j)
+                    if (i_first + 16 * j < tile.y)
+                        copy16(at + (i_first + 16 * j) * kBaseStride + c * 2, base[j] + c0, true);
+            }
+            if (key < 0) return;
+            const bf16* b = p.b + static_cast<int64_t>(key) * p.n * p.rank;
+            const uint32_t b_at = at + kTileRows * kBaseStride;
+            constexpr int kChunks = RK / 8;
+#pragma unroll
+            for (int j = 0; j < kTileCols * kChunks / kExpandThreads; ++j) {
+                const int i = tid + j * kExpandThreads, n = i / kChunks, q = i % kChunks;
+                const int64_t col = c0 + (SWIGLU ? n & 63 : n);
+                const bool in = q * 8 < p.rank && col < p.cols;
+                copy16(b_at + n * b_stride<RN>() + q * 16,
+                       in ? b + (col + (SWIGLU && n >= 64 ? p.cols : 0)) * p.rank + q * 8 : p.b, in);
+            }
+        };
+        __syncthreads();  // the item before is done with its stages
+#pragma unroll
+        for (int s = 0; s < kExpandStages - 1; ++s) {
+            if (s < count) load(s, first_block + s);
+            copy_commit();
+        }
 
-    // s: the splits' sum, scaled; zero past the rank and in rows without an adapter
-    if (runs > 0) {
-        const int64_t first = tile * kTileRows;
-        for (int i = tid; i < kTileRows * (RK / 4); i += kTileThreads) {
-            const int r = i / (RK / 4), q = (i % (RK / 4)) * 4;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int key = t.key[r];
-            if (key >= 0 && q < RN) {
-                for (int z = 0; z < p.splits; ++z) {
-                    const float4 w = *reinterpret_cast<const float4*>(
-                        p.s + (static_cast<int64_t>(z) * p.rows + first + r) * RN + q);
-                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        // s of this warp's 16 rows as fragments: the splits' sum, scaled; zero past the rank
+        uint32_t hi[RK / 16][4], lo[RK / 16][4];
+        if (key >= 0) {
+            const float scale = p.scale ? p.scale[key / p.experts] : 1.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int kk = 0; kk < RK / 8; ++kk) {
+                    float2 v = make_float2(0.0f, 0.0f);
+                    if (r0 + 8 * h < tile.y && kk * 8 < RN) {
+                        const float* s = p.s + (static_cast<int64_t>(tile.x) + r0 + 8 * h) * RN + kk * 8 + 2 * (lane & 3);
+                        for (int z = 0; z < p.splits; ++z) {
+                            const float2 w = *reinterpret_cast<const float2*>(s + z * p.rows * RN);
+                            v.x += w.x, v.y += w.y;
+                        }
+                        v.x *= scale, v.y *= scale;
+                    }
+                    split2(v, hi[kk / 2][(kk & 1) * 2 + h], lo[kk / 2][(kk & 1) * 2 + h]);
                 }
-                const float scale = p.scale ? p.scale[key / p.experts] : 1.0f;
-                v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
-            }
-            *reinterpret_cast<float4*>(s_s + r * s_stride<RN>() + q) = v;
         }
-    }
 
-    // y = base + delta in place, for rows r (one of two per lane; conflict-free)
-    float acc[kTileCols / 8][4] = {};
-    auto finish = [&](int h) {
-        uint8_t* row = base_s + (warp * 16 + (lane >> 2) + 8 * h) * kBaseStride + (lane & 3) * 4;
+        int slot = 0, load_slot = kExpandStages - 1;
+        for (int step = 0; step < count; ++step) {
+            copy_wait<kExpandStages - 2>();
+            __syncthreads();  // this stage has landed everywhere, and the one before is done with
+            if (step + kExpandStages - 1 < count) load(load_slot, first_block + step + kExpandStages - 1);
+            copy_commit();
+            uint8_t* base_s = smem + slot * kStage;
+            const int64_t c0 = static_cast<int64_t>(first_block + step) * kOut;
+            if (warp * 16 < tile.y) {
+                // n8 fragments of this warp: SwiGLU: gate columns 32 half + 8 f (f < 4) and the up
+                // columns 64 further; else columns 64 half + 8 f
+                float acc[8][4] = {};
+                if (key >= 0) {
+                    const uint32_t bs = smem_addr(base_s) + kTileRows * kBaseStride;
 #pragma unroll
-        for (int n = 0; n < kOut / 8; ++n) {
-            uint32_t* at = reinterpret_cast<uint32_t*>(row + n * 16);
-            const uint32_t g = *at;
-            float y0 = bf16_lo(g) + acc[n][2 * h], y1 = bf16_hi(g) + acc[n][2 * h + 1];
-            if constexpr (SWIGLU) {
-                const uint32_t u = *reinterpret_cast<const uint32_t*>(row + n * 16 + 128);
-                y0 = silu_times(y0, bf16_lo(u) + acc[n + 8][2 * h]);
-                y1 = silu_times(y1, bf16_hi(u) + acc[n + 8][2 * h + 1]);
+                    for (int kk = 0; kk < RK / 16; ++kk) {
+#pragma unroll
+                        for (int f = 0; f < 8; f += 2) {
+                            uint32_t bf[4];
+                            const int n0 = SWIGLU ? half * 32 + (f & 3) * 8 + (f >= 4 ? 64 : 0) : half * 64 + f * 8;
+                            const int n = n0 + (lane & 7) + ((lane >> 4) << 3);
+                            ldmatrix4(bs + n * b_stride<RN>() + (kk * 2 + ((lane >> 3) & 1)) * 16, bf);
+                            mma16816(acc[f], lo[kk], bf[0], bf[1]);
+                            mma16816(acc[f + 1], lo[kk], bf[2], bf[3]);
+                            mma16816(acc[f], hi[kk], bf[0], bf[1]);
+                            mma16816(acc[f + 1], hi[kk], bf[2], bf[3]);
+                        }
+                    }
+                }
+                // y = base + delta in place (conflict-free), in this warp's rows and columns
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint8_t* row = base_s + (r0 + 8 * h) * kBaseStride + (lane & 3) * 4;
+#pragma unroll
+                    for (int f = 0; f < (SWIGLU ? 4 : 8); ++f) {
+                        uint32_t* at = reinterpret_cast<uint32_t*>(row + half * (SWIGLU ? 64 : 128) + f * 16);
+                        const uint32_t g = *at;
+                        float y0 = bf16_lo(g) + acc[f][2 * h], y1 = bf16_hi(g) + acc[f][2 * h + 1];
+                        if constexpr (SWIGLU) {
+                            const uint32_t u = at[32];  // 128 bytes further
+                            const float u0 = bf16_lo(u) + acc[f + 4][2 * h], u1 = bf16_hi(u) + acc[f + 4][2 * h + 1];
+                            // without an adapter the bits of swiglu_kernel
+                            y0 = key >= 0 ? fast_silu_times(y0, u0) : silu_times(y0, u0);
+                            y1 = key >= 0 ? fast_silu_times(y1, u1) : silu_times(y1, u1);
+                        }
+                        *at = pack_bf16x2(y0, y1);
+                    }
+                }
+                __syncwarp();
+                constexpr int kPieces = kOut / 16, kPer = 32 / kPieces;  // pieces of a half row; rows per step
+#pragma unroll
+                for (int j = 0; j < 16 / kPer; ++j) {
+                    const int i = warp * 16 + j * kPer + lane / kPieces;
+                    const int oc = half * (kOut / 2) + (lane % kPieces) * 8;
+                    if (i < tile.y && c0 + oc < p.cols)
+                        *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(p.order[tile.x + i]) * p.cols + c0 + oc) =
+                            *reinterpret_cast<const uint4*>(base_s + i * kBaseStride + oc * 2);
+                }
             }
-            *at = pack_bf16x2(y0, y1);
+            if (++slot == kExpandStages) slot = 0;
+            if (++load_slot == kExpandStages) load_slot = 0;
         }
-    };
-    const int r0 = warp * 16 + (lane >> 2), r1 = r0 + 8;
-    for (int run = 0; run < runs; ++run) {
-        __syncthreads();  // the other slot has been read; s is in place
-        if (run + 1 < runs) load_b(run + 1, (run + 1) & 1);
-        copy_commit();
-        copy_wait<1>();
-        __syncthreads();
-        const int i0 = t.run[run], i1 = t.run[run + 1];
-        if (warp * 16 >= i1 || warp * 16 + 16 <= i0) continue;
-        const uint32_t bs = smem_addr(b_s) + (run & 1) * kTileCols * b_stride<RN>();
-#pragma unroll
-        for (int kk = 0; kk < RK / 16; ++kk) {
-            uint32_t hi[4], lo[4];
-            const float* s0 = s_s + r0 * s_stride<RN>() + kk * 16 + 2 * (lane & 3);
-            const float* s1 = s0 + 8 * s_stride<RN>();
-            split2(*reinterpret_cast<const float2*>(s0), hi[0], lo[0]);
-            split2(*reinterpret_cast<const float2*>(s1), hi[1], lo[1]);
-            split2(*reinterpret_cast<const float2*>(s0 + 8), hi[2], lo[2]);
-            split2(*reinterpret_cast<const float2*>(s1 + 8), hi[3], lo[3]);
-#pragma unroll
-            for (int n0 = 0; n0 < kTileCols; n0 += 16) {
-                uint32_t bf[4];
-                const int n = n0 + (lane & 7) + ((lane >> 4) << 3);
-                ldmatrix4(bs + n * b_stride<RN>() + (kk * 2 + ((lane >> 3) & 1)) * 16, bf);
-                mma16816(acc[n0 / 8], lo, bf[0], bf[1]);
-                mma16816(acc[n0 / 8], hi, bf[0], bf[1]);
-                mma16816(acc[n0 / 8 + 1], lo, bf[2], bf[3]);
-                mma16816(acc[n0 / 8 + 1], hi, bf[2], bf[3]);
-            }
-        }
-        if (r0 >= i0 && r0 < i1) finish(0);
-        if (r1 >= i0 && r1 < i1) finish(1);
-#pragma unroll
-        for (int n = 0; n < kTileCols / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
     }
     copy_wait<0>();
-    __syncwarp();  // base rows are the warp's own
-    if constexpr (SWIGLU) {  // rows without an adapter (elsewhere base stands as it is)
-        if (t.key[r0] == kNone) finish(0);
-        if (t.key[r1] == kNone) finish(1);
-    }
-    __syncwarp();
-    constexpr int kPieces = kOut / 8, kPer = 32 / kPieces;  // 16-byte pieces of a row; rows per step
-#pragma unroll
-    for (int j = 0; j < 16 / kPer; ++j) {
-        const int i = warp * 16 + j * kPer + lane / kPieces, c = (lane % kPieces) * 8;
-        if (t.key[i] == kOutside || c0 + c >= p.cols) continue;
-        if (!SWIGLU && t.key[i] == kNone && p.out == p.base) continue;
-        *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(t.row[i]) * p.cols + c0 + c) =
-            *reinterpret_cast<const uint4*>(base_s + i * kBaseStride + c * 2);
-    }
 }
 
 // ---------------------------------------------------- adapters of packed rows
@@ -680,7 +719,7 @@ constexpr int64_t kFewRows = 256;
 struct Shape {
     bool few;
     int splits;
-    int64_t split_k, chunk_rows, table, order, keys, s, total;
+    int64_t split_k, chunk_rows, table, order, keys, tiles, s, total;
     int chunks;
 };
 
@@ -695,13 +734,15 @@ Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int sms) {
         f.total = round256(rows * rank * 4 * f.splits);
         return f;
     }
-    // K is split until about four CTAs of the shrink kernel stand on every SM, in
-    // parts of at least 256 elements.
+    // K is split until about three CTAs of the shrink kernel stand on every SM, in
+    // parts of at least 512 elements, and into eight at most: the expand kernel adds
+    // the parts of s every time it loads them.
     const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
-    int64_t splits = 4ll * sms / tiles;
-    const int64_t most = (k + 255) / 256;
+    int64_t splits = 3ll * sms / tiles;
+    int64_t most = (k + 511) / 512;
+    if (most > 8) most = 8;
     splits = splits < 1 ? 1 : (splits > most ? most : splits);
-    f.split_k = ((k + splits - 1) / splits + 63) / 64 * 64;
+    f.split_k = ((k + splits - 1) / splits + kShrinkK - 1) / kShrinkK * kShrinkK;
     f.splits = static_cast<int>((k + f.split_k - 1) / f.split_k);
     f.chunk_rows = (rows + static_cast<int64_t>(kMaxChunks) * kSortThreads - 1) /
                    (static_cast<int64_t>(kMaxChunks) * kSortThreads) * kSortThreads;
@@ -709,7 +750,8 @@ Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int sms) {
     f.table = 0;
     f.order = round256(static_cast<int64_t>(adapters + 2) * f.chunks * 4);
     f.keys = f.order + round256(rows * 4);
-    f.s = f.keys + round256(rows * 4);
+    f.tiles = f.keys + round256(rows * 4);
+    f.s = f.tiles + round256(rows * 8 + 256);  // the count, then at most one tile per row
     f.total = f.s + round256(rows * padded_rank(rank) * 4 * f.splits);
     return f;
 }
@@ -755,8 +797,10 @@ cudaError_t few_rows(const Adapter& p, cudaStream_t stream) {
     return expand_rows<16, SWIGLU>(p, stream);
 }
 
+constexpr int kMaxWalk = 16;
+
 template <int RN, bool SWIGLU>
-cudaError_t tiles(const Adapter& p, const Shape& f, cudaStream_t stream) {
+cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream) {
     static bool order_ok[64] = {}, shrink_ok[64] = {}, expand_ok[64] = {};
     const int buckets = p.adapters + 2;
     const int order_smem = (32 * (buckets | 1) + 2 * buckets) * 4;
@@ -769,23 +813,43 @@ cudaError_t tiles(const Adapter& p, const Shape& f, cudaStream_t stream) {
                                   f.chunk_rows));
     MOE_CUDA_TRY(launch_dependent(order_kernel, dim3(f.chunks), dim3(kSortThreads), order_smem, stream, p,
                                   f.chunk_rows));
-    const unsigned n_tiles = static_cast<unsigned>((p.rows + kTileRows - 1) / kTileRows);
-    MOE_CUDA_TRY(launch_dependent(shrink_tile_kernel<RN>, dim3(n_tiles, f.splits), dim3(kTileThreads),
-                                  kShrinkSmem, stream, p));
+    const bool none = SWIGLU || p.out != p.base;
+    MOE_CUDA_TRY(launch_dependent(tiles_kernel, dim3(static_cast<unsigned>((p.rows + 255) / 256)), dim3(256), 0,
+                                  stream, p, none));
+    const int64_t n_tiles = (p.rows + kTileRows - 1) / kTileRows;  // at least; groups' ends add some
+    const auto resident = [&](int smem_bytes, int threads_most) {
+        const int fit = 227 * 1024 / (smem_bytes + 1024);
+        return static_cast<int64_t>(sms) * (fit < threads_most ? fit : threads_most);
+    };
+    const int64_t shrink_most = resident(kShrinkSmem, 4);
+    const int64_t shrink_items = p.rows * f.splits;
+    MOE_CUDA_TRY(launch_dependent(shrink_tile_kernel<RN>,
+                                  dim3(static_cast<unsigned>(shrink_items < shrink_most ? shrink_items : shrink_most)),
+                                  dim3(kTileThreads), kShrinkSmem, stream, p));
     const int out_cols = SWIGLU ? kTileCols / 2 : kTileCols;
     const int blocks = static_cast<int>((p.cols + out_cols - 1) / out_cols);
-    return launch_dependent(expand_tile_kernel<RN, SWIGLU>, dim3(n_tiles * static_cast<unsigned>(blocks)),
-                            dim3(kTileThreads), expand_smem<RN>(), stream, p, blocks);
+    // Column blocks per item: a longer walk spreads its start over more work, as long as every
+    // resident CTA gets about four items.
+    const int64_t expand_most = resident(expand_smem<RN>(), 3);
+    int64_t per = n_tiles * blocks / (4 * expand_most);
+    per = per < 1 ? 1 : (per > kMaxWalk ? kMaxWalk : per);
+    const int groups = static_cast<int>((blocks + per - 1) / per);
+    per = (blocks + groups - 1) / groups;
+    const int64_t expand_items = p.rows * groups;
+    return launch_dependent(expand_tile_kernel<RN, SWIGLU>,
+                            dim3(static_cast<unsigned>(expand_items < expand_most ? expand_items : expand_most)),
+                            dim3(kExpandThreads), expand_smem<RN>(), stream, p, blocks, static_cast<int>(per),
+                            groups);
 }
 
 template <bool SWIGLU>
-cudaError_t many_rows(const Adapter& p, const Shape& f, cudaStream_t stream) {
+cudaError_t many_rows(const Adapter& p, const Shape& f, int sms, cudaStream_t stream) {
     switch (padded_rank(p.rank)) {
-        case 8: return tiles<8, SWIGLU>(p, f, stream);
-        case 16: return tiles<16, SWIGLU>(p, f, stream);
-        case 32: return tiles<32, SWIGLU>(p, f, stream);
-        case 64: return tiles<64, SWIGLU>(p, f, stream);
-        default: return tiles<128, SWIGLU>(p, f, stream);
+        case 8: return tiles<8, SWIGLU>(p, f, sms, stream);
+        case 16: return tiles<16, SWIGLU>(p, f, sms, stream);
+        case 32: return tiles<32, SWIGLU>(p, f, sms, stream);
+        case 64: return tiles<64, SWIGLU>(p, f, sms, stream);
+        default: return tiles<128, SWIGLU>(p, f, sms, stream);
     }
 }
 
@@ -826,11 +890,13 @@ cudaError_t launch_adapter(const void* base, const void* x, const void* a, const
     p.table = reinterpret_cast<int32_t*>(at + f.table);
     p.order = reinterpret_cast<int32_t*>(at + f.order);
     p.keys = reinterpret_cast<int32_t*>(at + f.keys);
+    p.tile_count = reinterpret_cast<int32_t*>(at + f.tiles);
+    p.tiles = reinterpret_cast<int2*>(at + f.tiles + 256);
     p.s = reinterpret_cast<float*>(at + f.s);
     p.splits = f.splits;
     p.split_k = f.split_k;
     if (f.few) return swiglu ? few_rows<true>(p, stream) : few_rows<false>(p, stream);
-    return swiglu ? many_rows<true>(p, f, stream) : many_rows<false>(p, f, stream);
+    return swiglu ? many_rows<true>(p, f, sms, stream) : many_rows<false>(p, f, sms, stream);
 }
 
 cudaError_t launch_adapter_rows(const int32_t* token_adapters, const int32_t* inverse,
