@@ -53,7 +53,7 @@ struct Adapter {
     int64_t rows, k, n, cols;     // cols: output columns (n, or n / 2 with SwiGLU)
     int rank, adapters, experts;
     int32_t *table, *order, *keys;
-    int32_t* tile_count;
+    int32_t* tile_count;          // [0] tiles, [1] stretches claimed by the expand kernel
     int2* tiles;                  // {first sorted row, rows} of each tile
     float* s;                     // [splits][rows][padded rank]
     int splits;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const Adapter p, in
     for (int i = threadIdx.x; i < buckets; i += kSortThreads) counts[i] = 0;
     pdl_wait();
     __syncthreads();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.tile_count = 0;
+    if (blockIdx.x == 0 && threadIdx.x < 2) p.tile_count[threadIdx.x] = 0;
     const int64_t valid = valid_rows(p);
     const int64_t begin = blockIdx.x * chunk_rows;
     const int64_t end = begin + chunk_rows < p.rows ? begin + chunk_rows : p.rows;
@@ -348,6 +348,15 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same with c = 0 before it.
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Cuts the sorted rows' groups of equal keys into tiles.  A thread whose key
@@ -513,7 +522,7 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
 }
 
 constexpr int kExpandThreads = 256;                   // 4 x 16 rows, 2 halves of the columns
-constexpr int kExpandStages = 3;
+constexpr int kExpandStages = 2;
 constexpr int kTileCols = 128;                        // rows of B per step: 128 columns, or 64 gate + 64 up
 constexpr int kBaseStride = kTileCols * 2 + 16;       // bytes; the pads keep ldmatrix and row stores conflict-free
 template <int RN> constexpr int rank_k() { return RN < 16 ? 16 : RN; }
@@ -522,76 +531,160 @@ template <int RN> constexpr int expand_smem() {
     return kExpandStages * (kTileRows * kBaseStride + kTileCols * b_stride<RN>());
 }
 
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // Two floats as bf16 hi parts, and the rests' as a second register.
 __device__ __forceinline__ void split2(float2 v, uint32_t& hi, uint32_t& lo) {
-    const uint32_t a = f32_to_bf16_bits(v.x), b = f32_to_bf16_bits(v.y);
-    hi = a | b << 16;
-    lo = pack_bf16x2(v.x - bf16_bits_to_f32(a), v.y - bf16_bits_to_f32(b));
+    hi = pack2(v.x, v.y);
+    lo = pack2(v.x - bf16_lo(hi), v.y - bf16_hi(hi));
 }
 
-// silu(g) u from the fast exponential and reciprocal, within 2^-21 of the value
-// for |g| up to 88 (the rounding to bf16 is 2^-8); beyond that 0 or g u, as it is.
-__device__ __forceinline__ float fast_silu_times(float g, float u) {
-    return __fdividef(g, 1.0f + __expf(-g)) * u;
+// Two fp32 lanes in one register pair: one instruction for both.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t x, y, z;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(x), "l"(y));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(z));
+    return a;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t x, y, z;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(x), "l"(y));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(z));
+    return a;
 }
 
-// CTAs walk the (tile, group of `per` column blocks) pairs with the grid's
-// stride.  The blocks of a group form one cp.async pipeline whose stages hold the
-// tile's base rows and the pair's rows of B; s stays in registers as bf16 fragments.
+// silu(g) u from the hardware's exponential and reciprocal: g log2 e is rounded
+// once (|g| 2^-24), both are good to a few steps, so it is within (|g| + 8) 2^-23
+// of the value, against 2^-8 of the rounding to bf16.  Where 2^(-g log2 e) is
+// infinite the reciprocal is 0.  (With expf, a division and single lanes the
+// SwiGLU form of the expand kernel issued 36 instructions an element and was
+// bound by them: 309 us at 4096 tokens, 8 experts, top-2, against 195 with this.)
+__device__ __forceinline__ float2 fast_silu_times(float2 g, float2 u) {
+    const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = add2(e, make_float2(1.0f, 1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    return mul2(mul2(g, r), u);
+}
+
+// Stretch q of the (tile, column block) pairs: the first gridDim.x stretches cover
+// half of the pairs, the next as many half of the rest, and so on, down to
+// kLeastStretch pairs.  Returns its first pair and its end.
+constexpr int kLeastStretch = 8;
+struct Stretch { int64_t x, y; };
+__device__ __forceinline__ Stretch stretch_of(int64_t q, int64_t all) {
+    const int64_t round = gridDim.x;
+    int64_t first = 0;
+    for (;;) {
+        int64_t size = (all - first) / (2 * round);
+        if (size <= kLeastStretch) {
+            size = kLeastStretch;
+        } else if (q >= round) {
+            first += size * round;
+            q -= round;
+            continue;
+        }
+        first += q * size;
+        return {min(first, all), min(first + size, all)};
+    }
+}
+
+// CTAs claim stretches of the (tile, column block) pairs, long ones first, and walk
+// them tile by tile: tiles differ in their rows, so equal shares end far apart
+// (one share per CTA: 306 us instead of 186 at 4096 tokens, 8 experts of 14336,
+// top-2), and short stretches alone pay for many starts.  A CTA's blocks of one
+// tile form one cp.async pipeline whose stages hold the tile's base rows and the
+// pair's rows of B; s stays in registers as bf16 fragments.
 template <int RN, bool SWIGLU>
-__global__ void __launch_bounds__(kExpandThreads)
-expand_tile_kernel(const Adapter p, int blocks, int per, int groups) {
+__global__ void __launch_bounds__(kExpandThreads, RN <= 32 ? 3 : (RN <= 64 ? 2 : 1))
+expand_tile_kernel(const Adapter p, int blocks) {
     constexpr int RK = rank_k<RN>();
     constexpr int kOut = SWIGLU ? kTileCols / 2 : kTileCols;  // output columns of a block
+    constexpr int kHalves = SWIGLU ? 2 : 1;
     constexpr int kStage = kTileRows * kBaseStride + kTileCols * b_stride<RN>();
+    constexpr int kChunks = RK / 8, kBRows = kExpandThreads / kChunks, kBCopies = kTileCols / kBRows;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, half = tid >> 7;
     // this thread's share of the base rows: one 16-byte chunk of rows i_first + 16 j
     const int c = (tid & 15) * 8, i_first = tid >> 4;
     const int c_col = SWIGLU ? c & 63 : c;  // its column inside the block
+    const int b_q = tid % kChunks, b_n = tid / kChunks;
     const int r0 = warp * 16 + (lane >> 2);
+    constexpr int kPieces = kOut / 16, kPer = 32 / kPieces;  // out: 16-byte pieces of a half row; rows at a time
+    const int out_row = warp * 16 + lane / kPieces, out_col = half * (kOut / 2) + (lane % kPieces) * 8;
     pdl_trigger();
     pdl_wait();
-    const int items = *p.tile_count * groups;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int2 tile = p.tiles[item / groups];
-        const int first_block = (item % groups) * per;
-        const int count = min(per, blocks - first_block);
+    __shared__ int claimed[2];
+    const int64_t all = static_cast<int64_t>(*p.tile_count) * blocks;
+    Stretch stretch = stretch_of(blockIdx.x, all);
+    int turn = 0;
+    if (tid == 0) claimed[0] = atomicAdd(p.tile_count + 1, 1);
+    while (stretch.x < all) {
+        const int2 tile = p.tiles[stretch.x / blocks];
+        const int first_block = static_cast<int>(stretch.x % blocks);
+        const int count = static_cast<int>(min(static_cast<int64_t>(blocks - first_block), stretch.y - stretch.x));
         const int key = p.keys[tile.x];
         const bf16* base[kTileRows / 16];
 #pragma unroll
         for (int j = 0; j < kTileRows / 16; ++j) {
             const int i = i_first + 16 * j;
-            base[j] = p.base + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.n + c_col +
-                      (SWIGLU && c >= 64 ? p.cols : 0);
+            base[j] = p.base + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.n +
+                      static_cast<int64_t>(first_block) * kOut + c_col + (SWIGLU && c >= 64 ? p.cols : 0);
         }
-        auto load = [&](int slot, int block) {
-            const int64_t c0 = static_cast<int64_t>(block) * kOut;
+        // and its share of B: chunk b_q of rows b_n + kBRows j
+        const int64_t col0 = static_cast<int64_t>(first_block) * kOut;
+        const bf16* b[kBCopies];
+#pragma unroll
+        for (int j = 0; j < kBCopies; ++j) {
+            const int n = b_n + kBRows * j;
+            const int64_t column = col0 + (SWIGLU ? (n & 63) + (n >= 64 ? p.cols : 0) : n);
+            b[j] = p.b + (key < 0 ? 0 : (static_cast<int64_t>(key) * p.n + column) * p.rank + b_q * 8);
+        }
+        int64_t left = p.cols - col0;  // columns from the next block to load on
+        auto load = [&](int slot) {
             const uint32_t at = smem_addr(smem) + slot * kStage;
-            if (c0 + c_col < p.cols) {
+            if (c_col < left) {
 #pragma unroll
-                for (int j = 0; j < kTileRows / 16; ++j)
+                for (int j = 0; j < kTileRows / 16; ++j) {
                     if (i_first + 16 * j < tile.y)
-                        copy16(at + (i_first + 16 * j) * kBaseStride + c * 2, base[j] + c0, true);
+                        copy16(at + (i_first + 16 * j) * kBaseStride + c * 2, base[j], true);
+                    base[j] += kOut;
+                }
             }
-            if (key < 0) return;
-            const bf16* b = p.b + static_cast<int64_t>(key) * p.n * p.rank;
-            const uint32_t b_at = at + kTileRows * kBaseStride;
-            constexpr int kChunks = RK / 8;
+            if (key >= 0) {
+                const uint32_t b_at = at + kTileRows * kBaseStride + b_n * b_stride<RN>() + b_q * 16;
 #pragma unroll
-            for (int j = 0; j < kTileCols * kChunks / kExpandThreads; ++j) {
-                const int i = tid + j * kExpandThreads, n = i / kChunks, q = i % kChunks;
-                const int64_t col = c0 + (SWIGLU ? n & 63 : n);
-                const bool in = q * 8 < p.rank && col < p.cols;
-                copy16(b_at + n * b_stride<RN>() + q * 16,
-                       in ? b + (col + (SWIGLU && n >= 64 ? p.cols : 0)) * p.rank + q * 8 : p.b, in);
+                for (int j = 0; j < kBCopies; ++j) {
+                    const int n = b_n + kBRows * j;
+                    const bool in = b_q * 8 < p.rank && (SWIGLU ? n & 63 : n) < left;
+                    copy16(b_at + j * kBRows * b_stride<RN>(), in ? b[j] : p.b, in);
+                    b[j] += kOut * p.rank;
+                }
             }
+            left -= kOut;
         };
         __syncthreads();  // the item before is done with its stages
 #pragma unroll
         for (int s = 0; s < kExpandStages - 1; ++s) {
-            if (s < count) load(s, first_block + s);
+            if (s < count) load(s);
             copy_commit();
+        }
+
+        bf16* out[16 / kPer];
+#pragma unroll
+        for (int j = 0; j < 16 / kPer; ++j) {
+            const int i = out_row + j * kPer;
+            out[j] = p.out + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.cols + out_col;
         }
 
         // s of this warp's 16 rows as fragments: the splits' sum, scaled; zero past the rank
@@ -619,63 +712,80 @@ expand_tile_kernel(const Adapter p, int blocks, int per, int groups) {
         for (int step = 0; step < count; ++step) {
             copy_wait<kExpandStages - 2>();
             __syncthreads();  // this stage has landed everywhere, and the one before is done with
-            if (step + kExpandStages - 1 < count) load(load_slot, first_block + step + kExpandStages - 1);
+            if (step + kExpandStages - 1 < count) load(load_slot);
             copy_commit();
             uint8_t* base_s = smem + slot * kStage;
             const int64_t c0 = static_cast<int64_t>(first_block + step) * kOut;
             if (warp * 16 < tile.y) {
-                // n8 fragments of this warp: SwiGLU: gate columns 32 half + 8 f (f < 4) and the up
-                // columns 64 further; else columns 64 half + 8 f
-                float acc[8][4] = {};
                 if (key >= 0) {
-                    const uint32_t bs = smem_addr(base_s) + kTileRows * kBaseStride;
+                    // 16 columns at a time (with SwiGLU 16 gate and the matching 16 up columns), so
+                    // few accumulators live at once
+                    const uint32_t bs = smem_addr(base_s) + kTileRows * kBaseStride +
+                                        ((lane & 7) + ((lane >> 4) << 3)) * b_stride<RN>() + ((lane >> 3) & 1) * 16;
 #pragma unroll
-                    for (int kk = 0; kk < RK / 16; ++kk) {
+                    for (int f = 0; f < kOut / 2; f += 16) {
+                        const int n0 = half * (kOut / 2) + f;
+                        float acc[kHalves][2][4];
 #pragma unroll
-                        for (int f = 0; f < 8; f += 2) {
-                            uint32_t bf[4];
-                            const int n0 = SWIGLU ? half * 32 + (f & 3) * 8 + (f >= 4 ? 64 : 0) : half * 64 + f * 8;
-                            const int n = n0 + (lane & 7) + ((lane >> 4) << 3);
-                            ldmatrix4(bs + n * b_stride<RN>() + (kk * 2 + ((lane >> 3) & 1)) * 16, bf);
-                            mma16816(acc[f], lo[kk], bf[0], bf[1]);
-                            mma16816(acc[f + 1], lo[kk], bf[2], bf[3]);
-                            mma16816(acc[f], hi[kk], bf[0], bf[1]);
-                            mma16816(acc[f + 1], hi[kk], bf[2], bf[3]);
-                        }
+                        for (int g = 0; g < kHalves; ++g)
+#pragma unroll
+                            for (int kk = 0; kk < RK / 16; ++kk) {
+                                uint32_t bf[4];
+                                ldmatrix4(bs + (n0 + g * 64) * b_stride<RN>() + kk * 32, bf);
+                                if (kk == 0) {
+                                    mma16816_first(acc[g][0], lo[0], bf[0], bf[1]);
+                                    mma16816_first(acc[g][1], lo[0], bf[2], bf[3]);
+                                } else {
+                                    mma16816(acc[g][0], lo[kk], bf[0], bf[1]);
+                                    mma16816(acc[g][1], lo[kk], bf[2], bf[3]);
+                                }
+                                mma16816(acc[g][0], hi[kk], bf[0], bf[1]);
+                                mma16816(acc[g][1], hi[kk], bf[2], bf[3]);
+                            }
+                        // y = base + delta in place (conflict-free), in this warp's rows and columns
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                uint32_t* at = reinterpret_cast<uint32_t*>(
+                                    base_s + (r0 + 8 * h) * kBaseStride + (n0 + q * 8) * 2 + (lane & 3) * 4);
+                                const uint32_t v = *at;
+                                float2 y = add2(make_float2(bf16_lo(v), bf16_hi(v)),
+                                                make_float2(acc[0][q][2 * h], acc[0][q][2 * h + 1]));
+                                if constexpr (SWIGLU) {
+                                    const uint32_t u = at[32];  // 128 bytes further
+                                    y = fast_silu_times(y, add2(make_float2(bf16_lo(u), bf16_hi(u)),
+                                                                make_float2(acc[1][q][2 * h], acc[1][q][2 * h + 1])));
+                                }
+                                *at = pack2(y.x, y.y);
+                            }
                     }
-                }
-                // y = base + delta in place (conflict-free), in this warp's rows and columns
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint8_t* row = base_s + (r0 + 8 * h) * kBaseStride + (lane & 3) * 4;
-#pragma unroll
-                    for (int f = 0; f < (SWIGLU ? 4 : 8); ++f) {
-                        uint32_t* at = reinterpret_cast<uint32_t*>(row + half * (SWIGLU ? 64 : 128) + f * 16);
-                        const uint32_t g = *at;
-                        float y0 = bf16_lo(g) + acc[f][2 * h], y1 = bf16_hi(g) + acc[f][2 * h + 1];
-                        if constexpr (SWIGLU) {
-                            const uint32_t u = at[32];  // 128 bytes further
-                            const float u0 = bf16_lo(u) + acc[f + 4][2 * h], u1 = bf16_hi(u) + acc[f + 4][2 * h + 1];
-                            // without an adapter the bits of swiglu_kernel
-                            y0 = key >= 0 ? fast_silu_times(y0, u0) : silu_times(y0, u0);
-                            y1 = key >= 0 ? fast_silu_times(y1, u1) : silu_times(y1, u1);
-                        }
-                        *at = pack_bf16x2(y0, y1);
+                } else if constexpr (SWIGLU) {  // without an adapter: the bits of swiglu_kernel
+#pragma unroll 4
+                    for (int i = 0; i < 16; ++i) {
+                        uint8_t* row = base_s + (warp * 16 + i) * kBaseStride + half * 64;
+                        const float g = __bfloat162float(reinterpret_cast<const bf16*>(row)[lane]);
+                        const float u = __bfloat162float(reinterpret_cast<const bf16*>(row + 128)[lane]);
+                        reinterpret_cast<bf16*>(row)[lane] = __float2bfloat16_rn(silu_times(g, u));
                     }
                 }
                 __syncwarp();
-                constexpr int kPieces = kOut / 16, kPer = 32 / kPieces;  // pieces of a half row; rows per step
 #pragma unroll
                 for (int j = 0; j < 16 / kPer; ++j) {
-                    const int i = warp * 16 + j * kPer + lane / kPieces;
-                    const int oc = half * (kOut / 2) + (lane % kPieces) * 8;
-                    if (i < tile.y && c0 + oc < p.cols)
-                        *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(p.order[tile.x + i]) * p.cols + c0 + oc) =
-                            *reinterpret_cast<const uint4*>(base_s + i * kBaseStride + oc * 2);
+                    const int i = out_row + j * kPer;
+                    if (i < tile.y && c0 + out_col < p.cols)
+                        *reinterpret_cast<uint4*>(out[j] + c0) =
+                            *reinterpret_cast<const uint4*>(base_s + i * kBaseStride + out_col * 2);
                 }
             }
             if (++slot == kExpandStages) slot = 0;
             if (++load_slot == kExpandStages) load_slot = 0;
+        }
+        stretch.x += count;
+        if (stretch.x == stretch.y) {  // the claim was made a stretch ago; make the next one now
+            stretch = stretch_of(static_cast<int64_t>(gridDim.x) + claimed[turn], all);
+            turn ^= 1;
+            if (tid == 0) claimed[turn] = atomicAdd(p.tile_count + 1, 1);
         }
     }
     copy_wait<0>();
@@ -797,8 +907,6 @@ cudaError_t few_rows(const Adapter& p, cudaStream_t stream) {
     return expand_rows<16, SWIGLU>(p, stream);
 }
 
-constexpr int kMaxWalk = 16;
-
 template <int RN, bool SWIGLU>
 cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream) {
     static bool order_ok[64] = {}, shrink_ok[64] = {}, expand_ok[64] = {};
@@ -816,7 +924,6 @@ cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream
     const bool none = SWIGLU || p.out != p.base;
     MOE_CUDA_TRY(launch_dependent(tiles_kernel, dim3(static_cast<unsigned>((p.rows + 255) / 256)), dim3(256), 0,
                                   stream, p, none));
-    const int64_t n_tiles = (p.rows + kTileRows - 1) / kTileRows;  // at least; groups' ends add some
     const auto resident = [&](int smem_bytes, int threads_most) {
         const int fit = 227 * 1024 / (smem_bytes + 1024);
         return static_cast<int64_t>(sms) * (fit < threads_most ? fit : threads_most);
@@ -828,18 +935,9 @@ cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream
                                   dim3(kTileThreads), kShrinkSmem, stream, p));
     const int out_cols = SWIGLU ? kTileCols / 2 : kTileCols;
     const int blocks = static_cast<int>((p.cols + out_cols - 1) / out_cols);
-    // Column blocks per item: a longer walk spreads its start over more work, as long as every
-    // resident CTA gets about four items.
-    const int64_t expand_most = resident(expand_smem<RN>(), 3);
-    int64_t per = n_tiles * blocks / (4 * expand_most);
-    per = per < 1 ? 1 : (per > kMaxWalk ? kMaxWalk : per);
-    const int groups = static_cast<int>((blocks + per - 1) / per);
-    per = (blocks + groups - 1) / groups;
-    const int64_t expand_items = p.rows * groups;
-    return launch_dependent(expand_tile_kernel<RN, SWIGLU>,
-                            dim3(static_cast<unsigned>(expand_items < expand_most ? expand_items : expand_most)),
-                            dim3(kExpandThreads), expand_smem<RN>(), stream, p, blocks, static_cast<int>(per),
-                            groups);
+    const int64_t expand_most = resident(expand_smem<RN>(), RN <= 32 ? 3 : (RN <= 64 ? 2 : 1));
+    return launch_dependent(expand_tile_kernel<RN, SWIGLU>, dim3(static_cast<unsigned>(expand_most)),
+                            dim3(kExpandThreads), expand_smem<RN>(), stream, p, blocks);
 }
 
 template <bool SWIGLU>
