@@ -18,7 +18,8 @@
 //   split_weight_kernel    W^T parts, [H, 3 E8] bf16 with columns hi | hi | lo
 //   dx                     the grouped GEMM with one group: columns mid | hi | hi
 //                          of the first against the second, K = 3 E8
-//   router_dw_kernel       dW: tcgen05 over tokens as K, both operands MN-major
+//   router_dw_kernel, router_dw_pair_kernel  dW: tcgen05 over tokens as K, both
+//                          operands MN-major; up to 80 experts, and above
 //   add_parts_kernel       adds the token ranges' partial sums in order
 //
 // Bound: for few experts by reading x once per product; for 256 experts by the
@@ -149,12 +150,10 @@ struct DwParams {
     float* out;           // dW [E, H], or the partial sums [ranges, E, H]
     int64_t hidden;
     int tokens, experts, padded;
-    int range;            // tokens per CTA (a multiple of kTileT)
-    int terms;            // MMAs per 16 tokens: 3 (one per part) or 1 (parts side by side in N)
-    int blocks;           // 64-column boxes per term
+    int range;            // tokens per CTA or CTA pair (a multiple of kTileT)
     int n;                // MMA N
+    int blocks;           // 64-column boxes of d per stage (pair: per part and CTA)
     int tmem_cols;
-    int hi_col;           // first column of the hi part's accumulator (3 terms)
     int stages;
 };
 
@@ -184,17 +183,12 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
            (static_cast<uint64_t>(2) << 61);
 }
 
-// dW^T tile [128 h, E] of one range of tokens.  Warp 0 loads x [32 tokens, 128]
-// and d's parts [32, E8 each] by TMA, warp 1 issues the MMAs (M = 128, K = 16),
-// warps 2-5 store the tile.  Up to E8 = 80 the three parts stand side by side in
-// N (3 E8 <= 240): one MMA per 16 tokens, and the epilogue adds the three column
-// groups.  Above that each part is an MMA of its own: hi into one accumulator,
-// lo and mid into a second.  (The tensor cores cut the sum of 16 products and
-// the accumulator off below its last bit.  With all parts in one accumulator the
-// small parts' products are cut off there too: dW at 32768 tokens, 256 experts
-// was 6.7e-6 of its norm away from the float64 product, 11 times the plain fp32
-// product's distance.)  A CTA's range bounds the additions in one accumulator
-// (at most 4096 tokens); ranges are added in a launch of their own.
+// dW^T tile [128 h, E] of one range of tokens, up to 80 experts.  Warp 0 loads x
+// [32 tokens, 128] and d's parts by TMA, warp 1 issues the MMAs (M = 128, K = 16),
+// warps 2-5 store the tile.  The three parts stand side by side in N (3 E8 <= 240):
+// one MMA per 16 tokens, and the epilogue adds the three column groups.  A CTA's
+// range bounds the additions in one accumulator (at most 2048 tokens, see the pair
+// kernel on why); ranges are added in a launch of their own.
 __global__ void __launch_bounds__(kDwThreads, 1)
 router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_d,
                  const DwParams p) {
@@ -209,7 +203,7 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const int t0 = blockIdx.y * p.range;
     const int t1 = min(t0 + p.range, p.tokens);
     const int steps = (t1 - t0 + kTileT - 1) / kTileT;  // >= 1
-    const int stage_bytes = (2 + p.terms * p.blocks) * kBlock;
+    const int stage_bytes = (2 + p.blocks) * kBlock;
 
     pdl_trigger();
     if (warp == 0 && lane == 0) {
@@ -245,9 +239,8 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             tma_load_2d(at, &map_x, &full[stage], h0, t);
             tma_load_2d(at + kBlock, &map_x, &full[stage], h0 + 64, t);
             at += 2 * kBlock;
-            for (int s = 0; s < p.terms; ++s)
-                for (int b = 0; b < p.blocks; ++b, at += kBlock)
-                    tma_load_2d(at, &map_d, &full[stage], s * p.padded + b * 64, t);
+            for (int b = 0; b < p.blocks; ++b, at += kBlock)
+                tma_load_2d(at, &map_d, &full[stage], b * 64, t);
             armed |= 1u << stage;
             parity = (parity & ~(1u << stage)) | (phase << stage);
             if (++stage == p.stages) {
@@ -271,11 +264,7 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             const uint32_t x_at = smem_u32(tiles + stage * stage_bytes);
             const uint32_t d_at = x_at + 2 * kBlock;
             for (int k = 0; k < kTileT / 16; ++k)
-                for (int s = 0; s < p.terms; ++s) {
-                    const bool first = i == 0 && k == 0 && s != 1;  // of its accumulator
-                    umma_bf16(tmem + (s == 2 ? p.hi_col : 0), mn_desc(x_at + k * 2048),
-                              mn_desc(d_at + s * p.blocks * kBlock + k * 2048), idesc, first ? 0u : 1u);
-                }
+                umma_bf16(tmem, mn_desc(x_at + k * 2048), mn_desc(d_at + k * 2048), idesc, (i | k) != 0 ? 1u : 0u);
             issued = true;
             umma_commit(&empty[stage]);
             if (++stage == p.stages) {
@@ -308,10 +297,8 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) sum[j] = __uint_as_float(v[j]);
-                // the small parts first: lo + mid + hi, or (lo and mid) + hi
-                const int step = p.terms == 1 ? p.padded : p.hi_col;
-                for (int s = 1; s < (p.terms == 1 ? 3 : 2); ++s) {
-                    tmem_ld32(row + s * step + c, v);
+                for (int s = 1; s < 3; ++s) {  // the small parts first: lo + mid + hi
+                    tmem_ld32(row + s * p.padded + c, v);
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(v[j]);
@@ -329,6 +316,199 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+    }
+}
+
+// dW^T tile [256 h, E] of one range of tokens on a CTA pair (cta_group::2), more
+// than 80 experts: each CTA loads its 128 columns of x and its half of every part's
+// E columns, the even CTA issues M = 256, N up to 256, one MMA per part and 16
+// tokens.  (On one CTA with M = 128 each SM is fed 112 KB per 64 tokens, which the
+// L2 cache delivers no faster than 49 bytes a cycle: 451 us at 32768 tokens, 256
+// experts, hidden 7168.)
+//
+// The tensor cores cut the sum of 16 products and the accumulator off below its last
+// bit, always downward, so long sums drift: with 500 MMAs into one accumulator dW was
+// 6.7e-6 of its norm off at this size, where plain fp32 products are 5.8e-7 off.  Here
+// an accumulator takes kChunk tokens (48 MMAs); meanwhile the epilogue warps add the
+// one before into fp32 registers, 128 columns of one row per thread.
+constexpr int kPairThreads = 320;  // producer, issuer, eight epilogue warps
+constexpr int kChunk = 256;
+constexpr int kPairStages = 6;
+constexpr int kChunkSteps = kChunk / kTileT;
+
+__device__ __forceinline__ bool wait_bounded_cluster(uint64_t* bar, uint32_t parity,
+                                                     volatile int* abort_flag, uint64_t limit) {
+    const uint64_t start = global_timer();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait_cluster(bar, parity)) return true;
+        if ((i & 31) == 0) {
+            if (*abort_flag) return false;
+            if (global_timer() - start > limit) {
+                atomicCAS(&g_route_backward_status, 0, kStatusRouterBackwardWait);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+router_dw_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_d,
+                      const DwParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int h0 = blockIdx.x * kTileH;  // the pair's tile: 256 columns of x from the even CTA's on
+    const int t0 = blockIdx.y * p.range;
+    const int t1 = min(t0 + p.range, p.tokens);
+    const int steps = (t1 - t0 + kTileT - 1) / kTileT;  // >= 1
+    const int chunks = (steps + kChunkSteps - 1) / kChunkSteps;
+    const int stage_bytes = (2 + 3 * p.blocks) * kBlock;  // of one CTA
+
+    pdl_trigger();
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&acc_full[a], 1);
+            mbar_init(&acc_empty[a], 2 * (kPairThreads - 64));  // both CTAs' epilogue threads
+        }
+        mbar_init(&drain, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers are set up
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0, armed = 0, parity = 0;
+        for (int i = 0; i < steps; ++i) {
+            if (!wait_bounded(&empty[stage], phase ^ 1u, &abort_flag, kWaitLimitNs)) break;
+            uint8_t* at = tiles + stage * stage_bytes;
+            const int t = t0 + i * kTileT;
+            const uint32_t leader_full = map_to_cta(smem_u32(&full[stage]), 0);
+            if (leader) mbar_expect_tx(&full[stage], 2 * stage_bytes);
+            tma_load_2d_pair(at, &map_x, leader_full, h0, t);
+            tma_load_2d_pair(at + kBlock, &map_x, leader_full, h0 + 64, t);
+            at += 2 * kBlock;
+            for (int s = 0; s < 3; ++s)
+                for (int b = 0; b < p.blocks; ++b, at += kBlock)
+                    tma_load_2d_pair(at, &map_d, leader_full, s * p.padded + rank * (p.n / 2) + b * 64, t);
+            armed |= 1u << stage;
+            parity = (parity & ~(1u << stage)) | (phase << stage);
+            if (++stage == kPairStages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (abort_flag && leader) {  // every copy in flight lands before the pair exits
+            volatile int never = 0;
+            for (int s = 0; s < kPairStages; ++s)
+                if (armed & (1u << s)) wait_bounded(&full[s], (parity >> s) & 1u, &never, kDrainLimitNs);
+        }
+    } else if (warp == 1 && lane == 0 && leader) {
+        const uint32_t idesc = make_idesc(2 * kTileH, p.n) | (1u << 15) | (1u << 16);  // both MN-major
+        int stage = 0;
+        uint32_t phase = 0;
+        bool issued = false, ok = true;
+        for (int chunk = 0; chunk < chunks && ok; ++chunk) {
+            const int acc = chunk & 1;
+            if (!wait_bounded_cluster(&acc_empty[acc], ((chunk >> 1) & 1) ^ 1u, &abort_flag, kWaitLimitNs)) break;
+            tc_fence_after();
+            const int here = min(kChunkSteps, steps - chunk * kChunkSteps);
+            for (int i = 0; i < here; ++i) {
+                if (!wait_bounded(&full[stage], phase, &abort_flag, kWaitLimitNs)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t x_at = smem_u32(tiles + stage * stage_bytes);
+                const uint32_t d_at = x_at + 2 * kBlock;
+                for (int k = 0; k < kTileT / 16; ++k)
+                    for (int s = 0; s < 3; ++s)
+                        umma_bf16_pair(tmem + acc * 256, mn_desc(x_at + k * 2048),
+                                       mn_desc(d_at + s * p.blocks * kBlock + k * 2048), idesc,
+                                       (i | k | s) != 0 ? 1u : 0u);
+                issued = true;
+                umma_commit_pair(&empty[stage]);
+                if (++stage == kPairStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (ok) umma_commit_pair(&acc_full[acc]);
+        }
+        if (issued) {  // no MMA outlives this wait, whatever the epilogue does
+            umma_commit_pair(&drain);
+            volatile int never = 0;
+            wait_bounded(&drain, 0, &never, kWaitLimitNs);
+        }
+    } else if (warp >= 2) {
+        // TMEM lane = row of the tile (h), column = expert: each warp takes half of the columns
+        // of 32 rows, and stores 32 neighbours of one expert's row at a time
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * (p.n / 2);
+        const uint32_t leader_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
+        const uint32_t leader_empty1 = map_to_cta(smem_u32(&acc_empty[1]), 0);
+        float sum[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+        bool ok = true;
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            const int acc = chunk & 1;
+            if (!wait_bounded(&acc_full[acc], (chunk >> 1) & 1, &abort_flag, kWaitLimitNs)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+                if (c < p.n / 2) {
+                    uint32_t v[32];
+                    tmem_ld32(row + acc * 256 + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(v[j]);
+                }
+            }
+            tc_fence_before();
+            mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+        }
+        const int64_t h = h0 + quarter * 32 + lane;
+        if (ok && h < p.hidden) {
+            const int e0 = half * (p.n / 2);
+            float* out = p.out + (static_cast<int64_t>(blockIdx.y) * p.experts + e0) * p.hidden + h;
+            const int mine = min(p.n / 2, p.experts - e0);
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+                if (j < mine) out[j * p.hidden] = sum[j];
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while its peer may still touch its memory
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
@@ -354,22 +534,31 @@ add_parts_kernel(const float4* __restrict__ parts, float4* __restrict__ out, int
 
 int pad8(int experts) { return (experts + 7) / 8 * 8; }
 
-// Tokens per CTA of the dW kernel.  At most 4096 (see router_dw_kernel), at
-// least 256 (below that the ranges' partial sums cost more than they spread);
-// within that the number of ranges that leaves the fewest SMs idle in the last
-// wave of CTAs.
-constexpr int64_t kMinRange = 256, kMaxRange = 4096;
-int token_ranges(int64_t tokens, int64_t hidden, int sms) {
-    const int64_t tiles = (hidden + kTileH - 1) / kTileH;
-    const int64_t least = (tokens + kMaxRange - 1) / kMaxRange;
+// Up to this many (padded) experts d's parts fit side by side into one MMA.
+constexpr int kSideBySide = 80;
+
+// Ranges of tokens for dW: those that take the least time, as waves of CTAs (or
+// pairs) over the SMs, each as long as its tokens and a start of about 64, plus the
+// partial sums' way through memory.  A token costs an SM of the first kernel about
+// 6 ns (x read at the memory's rate), a pair of the second 12.6 ns at N = 256 (6
+// MMAs of 128 cycles per 32 tokens); the partial sums of a range cost
+// 8 E H bytes at 6500 bytes/ns.
+constexpr int64_t kMinRange = 256, kMaxRange = 2048;
+int token_ranges(int64_t tokens, int64_t hidden, int experts, int sms) {
+    const bool pair = pad8(experts) > kSideBySide;
+    const int64_t tiles = pair ? (hidden + 2 * kTileH - 1) / (2 * kTileH) : (hidden + kTileH - 1) / kTileH;
+    const int64_t slots = pair ? sms / 2 : sms;
+    const double token_ns = pair ? 12.6 * experts / 256 : 6.0;
+    const double part_tokens = 8.0 * experts * hidden / 6500.0 / token_ns;
+    const int64_t least = pair ? 1 : (tokens + kMaxRange - 1) / kMaxRange;
     int64_t most = (tokens + kMinRange - 1) / kMinRange;
-    if (most > least + 15) most = least + 15;
+    if (most > least + 31) most = least + 31;
     int64_t best = least;
     double best_time = 1e30;
     for (int64_t r = least; r <= most; ++r) {
-        const double waves = static_cast<double>((tiles * r + sms - 1) / sms);
-        const double time = waves * (static_cast<double>(tokens) / r + 64.0);  // + a CTA's start and end
-        if (time < 0.98 * best_time) {
+        const double waves = static_cast<double>((tiles * r + slots - 1) / slots);
+        const double time = waves * (static_cast<double>(tokens) / r + 64.0) + (r > 1 ? r * part_tokens : 0.0);
+        if (time < best_time) {
             best_time = time;
             best = r;
         }
@@ -389,7 +578,7 @@ Layout layout(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw, int
     l.weight = round256(tokens * 4 * e8 * 2);
     l.offsets = l.weight + (dx ? round256(hidden * 3 * e8 * 2) : 0);
     l.sums = l.offsets + 256;
-    const int ranges = token_ranges(tokens, hidden, sms);
+    const int ranges = token_ranges(tokens, hidden, experts, sms);
     l.total = l.sums + (dw && ranges > 1 ? round256(ranges * experts * hidden * 4) : 0);
     return l;
 }
@@ -452,21 +641,24 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
         p.tokens = static_cast<int>(tokens);
         p.experts = experts;
         p.padded = e8;
-        const bool side_by_side = 3 * e8 <= 240;
-        const int columns = side_by_side ? 3 * e8 : e8;
-        p.terms = side_by_side ? 1 : 3;
-        p.blocks = (columns + 63) / 64;
-        p.n = (columns + 15) / 16 * 16;
-        // the epilogue reads 32 columns at a time from each column group
-        const int reach = (side_by_side ? 2 * e8 : 0) + (e8 + 31) / 32 * 32;
-        const int need = reach > p.n ? reach : p.n;
-        p.tmem_cols = 32;
-        while (p.tmem_cols < need) p.tmem_cols *= 2;
-        p.hi_col = p.tmem_cols;
-        if (!side_by_side) p.tmem_cols *= 2;
-        const int stage_bytes = (2 + p.terms * p.blocks) * kBlock;
-        p.stages = kDwSmem / stage_bytes < kMaxStages ? kDwSmem / stage_bytes : kMaxStages;
-        const int ranges = token_ranges(tokens, hidden, sms);
+        const bool pair = e8 > kSideBySide;
+        if (pair) {
+            p.n = (experts + 63) / 64 * 64;
+            p.blocks = (p.n / 2 + 63) / 64;
+            p.tmem_cols = 512;
+            p.stages = kPairStages;
+        } else {
+            p.n = (3 * e8 + 15) / 16 * 16;
+            p.blocks = (3 * e8 + 63) / 64;
+            // the epilogue reads 32 columns at a time from each column group
+            const int reach = 2 * e8 + (e8 + 31) / 32 * 32;
+            p.tmem_cols = 32;
+            while (p.tmem_cols < (reach > p.n ? reach : p.n)) p.tmem_cols *= 2;
+            const int fit = kDwSmem / ((2 + p.blocks) * kBlock);
+            p.stages = fit < kMaxStages ? fit : kMaxStages;
+        }
+        const int stage_bytes = (2 + (pair ? 3 : 1) * p.blocks) * kBlock;
+        const int ranges = token_ranges(tokens, hidden, experts, sms);
         const int64_t per = (tokens + ranges - 1) / ranges;
         p.range = static_cast<int>((per + kTileT - 1) / kTileT * kTileT);
         const unsigned used = static_cast<unsigned>((tokens + p.range - 1) / p.range);
@@ -477,16 +669,17 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
             *error = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
             return cudaErrorInvalidValue;
         }
-        static bool configured[64] = {};
+        static bool configured[2][64] = {};
         int device = 0;
         MOE_CUDA_TRY(cudaGetDevice(&device));
-        const int smem = kDwSmem + 1024;
-        if (!configured[device & 63]) {
-            MOE_CUDA_TRY(cudaFuncSetAttribute(router_dw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-            configured[device & 63] = true;
+        auto kernel = pair ? router_dw_pair_kernel : router_dw_kernel;
+        if (!configured[pair][device & 63]) {
+            MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDwSmem + 1024));
+            configured[pair][device & 63] = true;
         }
-        const unsigned tiles = static_cast<unsigned>((hidden + kTileH - 1) / kTileH);
-        MOE_CUDA_TRY(launch_dependent(router_dw_kernel, dim3(tiles, used), dim3(kDwThreads),
+        const int tile = pair ? 2 * kTileH : kTileH;
+        const unsigned tiles = static_cast<unsigned>((hidden + tile - 1) / tile * (pair ? 2 : 1));
+        MOE_CUDA_TRY(launch_dependent(kernel, dim3(tiles, used), dim3(pair ? kPairThreads : kDwThreads),
                                       p.stages * stage_bytes + 1024, stream, map_x, map_d, p));
         if (used > 1) {
             const int64_t vecs = experts * hidden / 4;
