@@ -147,6 +147,14 @@ class Extension:
         else:
             self._run(function(*args, torch.cuda.current_stream(index).cuda_stream))
 
+    def _on_device(self, device, run):
+        """run() with `device` as the current one (scratch sizes depend on it)."""
+        if device.index is None or device.index == torch.cuda.current_device():
+            run()
+        else:
+            with torch.cuda.device(device):
+                run()
+
     def scratch_bytes(self, tokens, topk, experts):
         return int(self.lib.moe_dispatch_scratch_bytes(tokens, topk, experts))
 
@@ -343,10 +351,15 @@ class Extension:
         _require(counts.shape == (experts,) and counts.dtype == torch.int32
                  and counted.numel() == 1 and counted.dtype == torch.int32,
                  "expected int32 counts[E] and counted[1]")
+        self.launch_balance_loss(logits, ids, bias, token_mask, coefficient, loss, counts, counted)
+
+    def launch_balance_loss(self, logits, ids, bias, token_mask, coefficient, loss, counts, counted):
+        """balance_loss_out without its tensor checks (callers have made them)."""
+        tokens, experts = logits.shape
         # the sums of each CTA: a buffer of this call's own, so calls on several
         # streams or in several captured graphs never share one
-        size = max(int(self.lib.moe_balance_loss_scratch_bytes(experts)), 1)
-        scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
+        size = int(self.lib.moe_balance_loss_scratch_bytes(experts))
+        scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=logits.device)
         self._call(
             logits.device, self.lib.moe_balance_loss,
             logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), ids.data_ptr(),
@@ -365,6 +378,13 @@ class Extension:
                  "expected int32 counts[E] and counted[1]")
         _require(grad_loss.numel() == 1 and grad_loss.dtype == torch.float32,
                  "expected one FP32 grad_loss")
+        self.launch_balance_loss_backward(logits, bias, token_mask, counts, counted, grad_loss,
+                                          coefficient, topk, grad_logits)
+
+    def launch_balance_loss_backward(self, logits, bias, token_mask, counts, counted, grad_loss,
+                                     coefficient, topk, grad_logits):
+        """balance_loss_backward_out without its tensor checks."""
+        tokens, experts = logits.shape
         self._call(
             logits.device, self.lib.moe_balance_loss_backward,
             logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), _ptr(token_mask),
@@ -397,18 +417,28 @@ class Extension:
             shape, dtype = ((tokens, experts), torch.float32) if like is None else (like.shape, like.dtype)
             _require(tensor.shape == shape and tensor.dtype == dtype,
                      f"{name}: expected {dtype} {tuple(shape)}")
-        index = x.device.index if x.device.index is not None else torch.cuda.current_device()
-        with torch.cuda.device(index):  # the scratch size depends on the device
-            size = int(self.lib.moe_route_backward_scratch_bytes(
-                tokens, hidden, experts, grad_x is not None, grad_router_weight is not None))
+        self.launch_route_backward(x, router_weight, ids, weights, grad_weights, grad_logits, grad_x,
+                                   grad_router_weight)
+
+    def launch_route_backward(self, x, router_weight, ids, weights, grad_weights, grad_logits, grad_x,
+                              grad_router_weight):
+        """route_backward_out without its tensor checks."""
+        tokens, hidden = x.shape
+        experts, topk = router_weight.shape[0], ids.shape[1]
+
+        def run():
+            size = self.lib.moe_route_backward_scratch_bytes(
+                tokens, hidden, experts, grad_x is not None, grad_router_weight is not None)
             _require(size >= 0, self.lib.moe_last_error().decode())
             scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
             self._call(
                 x.device, self.lib.moe_route_backward,
                 x.data_ptr(), router_weight.data_ptr(), ids.data_ptr(), weights.data_ptr(),
                 grad_weights.data_ptr(), _ptr(grad_logits), _ptr(grad_x), _ptr(grad_router_weight),
-                tokens, hidden, experts, ids.shape[1], scratch.data_ptr(), scratch.numel(),
+                tokens, hidden, experts, topk, scratch.data_ptr(), size,
             )
+
+        self._on_device(x.device, run)
 
     def _gemm_checks(self, a, weight, offsets, out):
         _require(a.is_cuda and a.is_contiguous() and a.dtype == torch.bfloat16 and a.dim() == 2,
@@ -472,18 +502,27 @@ class Extension:
             _check_cuda(offsets, x, "adapter")
             _require(offsets.shape == (experts + 1,) and offsets.dtype == torch.int32,
                      "expected int32 offsets[E+1]")
-        index = x.device.index if x.device.index is not None else torch.cuda.current_device()
-        with torch.cuda.device(index):  # the scratch size depends on the device
-            size = int(self.lib.moe_adapter_scratch_bytes(rows, k_dim, rank, adapters))
+        self.launch_adapter(function, base, x, a, b, scale, row_adapters, offsets, out)
+
+    def launch_adapter(self, function, base, x, a, b, scale, row_adapters, offsets, out):
+        """adapter_add_out (function moe_adapter_add) or adapter_swiglu_out
+        (moe_adapter_swiglu) without their tensor checks."""
+        rows, k_dim = x.shape
+        adapters, experts, rank = a.shape[:3]
+
+        def run():
+            size = self.lib.moe_adapter_scratch_bytes(rows, k_dim, rank, adapters)
             _require(size >= 0, self.lib.moe_last_error().decode())
-            # a buffer of this call's own, as in balance_loss_out
+            # a buffer of this call's own, as in launch_balance_loss
             scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
             self._call(
                 x.device, function,
                 base.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(scale),
                 row_adapters.data_ptr(), _ptr(offsets), out.data_ptr(), rows, k_dim, out.shape[1],
-                rank, adapters, experts, scratch.data_ptr(), scratch.numel(),
+                rank, adapters, experts, scratch.data_ptr(), size,
             )
+
+        self._on_device(x.device, run)
 
     def adapter_add_out(self, base, x, a, b, scale, row_adapters, offsets, out):
         """out = base + the rows' low-rank adapters (include/moe_b200.h); out may be base."""

@@ -98,11 +98,6 @@ def adapter_ids32(ids, count, what):
     return ids.clamp(-1, 2**31 - 1).to(torch.int32)
 
 
-def _span(tensor):
-    start = tensor.data_ptr()
-    return start, start + tensor.numel() * tensor.element_size()
-
-
 def _apply(base, x, a, b, row_adapters, offsets, scale, out, swiglu):
     if base.ndim != 2 or x.ndim != 2 or base.shape[0] != x.shape[0]:
         raise ValueError("expected base[R,N] and x[R,K]")
@@ -125,29 +120,36 @@ def _apply(base, x, a, b, row_adapters, offsets, scale, out, swiglu):
     if out is not None and (tuple(out.shape) != shape or out.dtype != torch.bfloat16
                             or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous bf16 tensor [{shape[0]},{shape[1]}]")
-    tensors = [t for t in (base, x, a, b, row_adapters, offsets, scale, out) if t is not None]
-    if any(t.device != x.device for t in tensors):
-        raise ValueError("all tensors must be on the same device")
+    device = x.device
+    grad = torch.is_grad_enabled()
+    for t in (base, x, a, b, row_adapters, offsets, scale, out):
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError("all tensors must be on the same device")
+        if grad and t.requires_grad:
+            raise ValueError("CUDA operators are forward-only; detach inputs or use inference_mode")
     if not base.is_contiguous() or not x.is_contiguous():
         raise ValueError("base and x must be contiguous")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("CUDA operators are forward-only; detach inputs or use inference_mode")
+    if offsets is not None and not offsets.is_contiguous():
+        raise ValueError("offsets must be contiguous")
     row_adapters = adapter_ids32(row_adapters, rows, "row")
-    if out is not None and out.numel():
-        low, high = _span(out)
-        for t in tensors[:-1]:
-            if t is base and not swiglu and out.data_ptr() == base.data_ptr():
+    if out is not None:
+        low = out.data_ptr()
+        high = low + out.nbytes
+        for t in (base, x, a, b, row_adapters, offsets, scale):
+            if t is None or (t is base and not swiglu and t.data_ptr() == low):
                 continue
-            start, end = _span(t)
-            if start < high and low < end:
+            start = t.data_ptr()
+            if start < high and low < start + t.nbytes:
                 raise ValueError("out must not overlap an input (adapter_add may write base itself)")
     if not x.is_cuda:
         raise RuntimeError("adapters require CUDA")
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
     extension = get_extension()
-    call = extension.adapter_swiglu_out if swiglu else extension.adapter_add_out
-    call(base, x, a, b, scale, row_adapters, offsets, out)
+    function = extension.lib.moe_adapter_swiglu if swiglu else extension.lib.moe_adapter_add
+    extension.launch_adapter(function, base, x, a, b, scale, row_adapters, offsets, out)
     return out
 
 

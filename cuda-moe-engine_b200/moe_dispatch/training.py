@@ -61,8 +61,8 @@ class _BalanceLoss(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=logits.device)
         counts = torch.empty(experts, dtype=torch.int32, device=logits.device)
         counted = torch.empty(1, dtype=torch.int32, device=logits.device)
-        extension.balance_loss_out(logits, expert_ids, bias, token_mask, coefficient, loss, counts,
-                                   counted)
+        extension.launch_balance_loss(logits, expert_ids, bias, token_mask, coefficient, loss, counts,
+                                      counted)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, bias, token_mask, counts, counted)
@@ -76,7 +76,7 @@ class _BalanceLoss(torch.autograd.Function):
             return None, None, None, None, None
         logits, bias, token_mask, counts, counted = ctx.saved_tensors
         grad = torch.empty_like(logits)
-        get_extension().balance_loss_backward_out(
+        get_extension().launch_balance_loss_backward(
             logits, bias, token_mask, counts, counted, grad_loss.contiguous(), ctx.coefficient,
             ctx.topk, grad)
         return grad, None, None, None, None
@@ -154,8 +154,8 @@ class _Route(torch.autograd.Function):
 def _route_backward(x, router_weight, ids, weights, grad_weights, grad_logits, want_x, want_weight):
     grad_x = torch.empty_like(x) if want_x else None
     grad_weight = torch.empty_like(router_weight) if want_weight else None
-    get_extension().route_backward_out(x, router_weight, ids, weights, grad_weights, grad_logits,
-                                       grad_x, grad_weight)
+    get_extension().launch_route_backward(x, router_weight, ids, weights, grad_weights, grad_logits,
+                                          grad_x, grad_weight)
     return grad_x, grad_weight
 
 

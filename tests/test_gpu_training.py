@@ -400,3 +400,19 @@ def test_device_status_stays_clear():
     from moe_dispatch import get_extension
 
     assert get_extension().device_status() == 0
+
+
+@pytest.mark.parametrize("experts", [1, 2, 3, 4, 8, 40])
+def test_balance_loss_with_every_expert_chosen(experts):
+    """topk = E: every share is 1 / E, and the gradient vanishes but for roundings."""
+    from moe_dispatch import balance_loss
+
+    logits, ids, _ = make_logits(70, experts, min(experts, 32), torch.float32, 6)
+    ids = torch.arange(experts, dtype=torch.int32).repeat(70, 1)[:, :32].contiguous()
+    leaf = logits.cuda().requires_grad_()
+    loss, counts = balance_loss(leaf, ids.cuda())
+    (grad,) = torch.autograd.grad(loss, leaf)
+    want, want_counts, want_grad, terms = balance_reference(logits, ids)
+    assert counts.cpu().tolist() == want_counts.tolist()
+    assert abs(loss.item() - want) <= 268 * U * want
+    check_gradient(grad, want_grad, terms)
