@@ -639,13 +639,14 @@ class Extension:
         return code.value
 
 
-@lru_cache(maxsize=1)
-def _extension():
-    return Extension(load_library())
+_loaded = None
 
 
 def get_extension():
     """The loaded CUDA operators; RuntimeError without a GPU or without the library."""
-    if not torch.cuda.is_available():
-        raise RuntimeError("CUDA operators require an NVIDIA GPU.")
-    return _extension()
+    global _loaded
+    if _loaded is None:
+        if not torch.cuda.is_available():
+            raise RuntimeError("CUDA operators require an NVIDIA GPU.")
+        _loaded = Extension(load_library())
+    return _loaded

@@ -194,9 +194,9 @@ int moe_route_backward(const void* x_bf16, const float* router_weight, const int
     if (tokens > 0 && (!ids || !weights || !grad_weights || (grad_x_bf16 && !router_weight) ||
                        (grad_router_weight && !x_bf16)))
         return fail(MOE_ERR_INVALID, "null pointer");
-    if (!aligned(x_bf16, 16) || !aligned(router_weight, 4) || !aligned(grad_x_bf16, 16) ||
+    if (!aligned(x_bf16, 16) || !aligned(router_weight, 16) || !aligned(grad_x_bf16, 16) ||
         !aligned(grad_router_weight, 16) || !aligned(grad_logits, 4))
-        return fail(MOE_ERR_INVALID, "x and the gradients must be 16-byte aligned");
+        return fail(MOE_ERR_INVALID, "x, router_weight and their gradients must be 16-byte aligned");
     int64_t need = 0;
     const int sized = cuda_status(moe::route_backward_scratch_bytes(tokens, hidden, experts, grad_x_bf16 != nullptr,
                                                                     grad_router_weight != nullptr, &need),

@@ -22,8 +22,11 @@
 //                          operands MN-major; up to 80 experts, and above
 //   add_parts_kernel       adds the token ranges' partial sums in order
 //
-// Bound: for few experts by reading x once per product; for 256 experts by the
-// tensor cores (6 bf16 flop per fp32 multiply-add).
+// Up to kFewExperts experts one kernel does both products from the same parts and reads
+// x once (router_few_kernel).
+//
+// Bound: for few experts by x and dx through memory; for 256 experts by the tensor
+// cores (6 bf16 flop per fp32 multiply-add).
 #include "common.cuh"
 #include "launch.h"
 #include "tcgen05.cuh"
@@ -512,22 +515,298 @@ router_dw_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     }
 }
 
-__global__ void __launch_bounds__(256)
-add_parts_kernel(const float4* __restrict__ parts, float4* __restrict__ out, int64_t vecs, int ranges) {
+// ------------------------------------------------------------- few experts
+
+// Both products at once for up to EP (8 or 16) experts, bound by x and dx through
+// memory: x is read once, by mma.sync (tcgen05 tiles of 128 rows would be 7/8 empty).
+// A CTA has 512 columns of hidden and a range of tokens, a warp 64 of the columns.  The
+// warp copies its part of 16 tokens at a time into a ring in shared memory, makes dW
+// from it (M = the parts of d^T, K = tokens, N = columns), and dx (M = tokens, K = the
+// parts of d, N = columns, against W's parts in registers), which takes x's place in
+// the ring on its way out.  d's parts are made for 256 tokens at a time, a row of
+// hi | mid | lo per token; the one layout serves both products, transposed and not.
+// The sums hi and mid + lo of dW are kept apart until the end.
+// (fp32 multiply-adds on the CUDA cores, two lanes an instruction: 24 us at 4096
+// tokens, 8 experts, hidden 4096, against 7 for the bytes.)
+constexpr int kFewExperts = 16;
+constexpr int kFewThreads = 256;
+constexpr int kFewCols = 512;     // of a CTA
+constexpr int kFewWarpCols = kFewCols / (kFewThreads / 32);
+constexpr int kFewTile = 16;      // tokens
+constexpr int kFewStages = 4;
+constexpr int kFewTokens = 256;   // of d at a time
+constexpr int kFewRow = kFewWarpCols * 2 + 16;  // bytes of a token in a warp's ring; the pad spreads the banks
+constexpr int kFewStage = kFewTile * kFewRow;
+template <int EP> constexpr int few_d_row() { return 3 * EP * 2 + (EP == 8 ? 32 : 16); }  // 80 or 112: likewise
+template <int EP> constexpr int few_smem() {
+    return (kFewThreads / 32) * kFewStages * kFewStage + kFewTokens * few_d_row<EP>();
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_k16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {  // c = 0 before
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int EP>
+__global__ void __launch_bounds__(kFewThreads, 2)
+router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__ weight,
+                  const int32_t* __restrict__ ids, const float* __restrict__ weights,
+                  const float* __restrict__ grad_weights, const float* __restrict__ grad_logits,
+                  __nv_bfloat16* __restrict__ grad_x, float* __restrict__ sums, int tokens,
+                  int64_t hidden, int experts, int topk, int range) {
+    constexpr int kFrags = kFewWarpCols / 8;  // n8 fragments of a warp
+    extern __shared__ __align__(128) uint8_t few_smem_raw[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t ring = smem_u32(few_smem_raw) + warp * kFewStages * kFewStage;
+    uint8_t* d_rows = few_smem_raw + (kFewThreads / 32) * kFewStages * kFewStage;
+    const uint32_t d_at = smem_u32(d_rows);
+    const int64_t h0 = static_cast<int64_t>(blockIdx.x) * kFewCols + warp * kFewWarpCols;
+    const int t0 = blockIdx.y * range, t1 = min(t0 + range, tokens);
+    const bool active = h0 < hidden;  // this warp has columns
     pdl_trigger();
     pdl_wait();
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < vecs; i += gridDim.x * 256ll) {
-        float4 sum = parts[i];
-#pragma unroll 4
-        for (int r = 1; r < ranges; ++r) {
+
+    // lane: chunk lane % 8 of tokens lane / 8 + 4 j
+    const int chunk = lane & 7, row = lane >> 3;
+    const bool in_cols = h0 + chunk * 8 < hidden;
+    const uint32_t lane_at = row * kFewRow + chunk * 16;
+    const int64_t step = 4 * hidden;
+    const __nv_bfloat16* from_x = x + (static_cast<int64_t>(t0) + row) * hidden + h0 + chunk * 8;
+    __nv_bfloat16* to_dx = grad_x + (static_cast<int64_t>(t0) + row) * hidden + h0 + chunk * 8;
+    int load_t = t0 + row;  // this lane's first token of the next load
+    auto load = [&](int slot) {
+#pragma unroll
+        for (int j = 0; j < kFewTile / 4; ++j) {
+            const bool in = in_cols && load_t < t1;
+            copy16(ring + slot * kFewStage + lane_at + 4 * j * kFewRow, in ? from_x : x, in);
+            from_x += step;
+            load_t += 4;
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kFewStages - 1; ++s) {
+        if (active && sums) load(s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    // W's parts as B fragments: experts k = 2 (lane % 4) and the next (and 8 further), column lane / 4
+    uint32_t w_hi[kFrags][EP / 8], w_lo[kFrags][EP / 8];
+    if (grad_x) {
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+            for (int g = 0; g < EP / 8; ++g) {
+                const int e = g * 8 + 2 * (lane & 3);
+                const int64_t h = h0 + f * 8 + (lane >> 2);
+                float a = h < hidden && e < experts ? weight[e * hidden + h] : 0.0f;
+                float b = h < hidden && e + 1 < experts ? weight[(e + 1) * hidden + h] : 0.0f;
+                w_hi[f][g] = bf16_part(a) | bf16_part(b) << 16;
+                w_lo[f][g] = bf16_part(a) | bf16_part(b) << 16;
+            }
+    }
+
+    // dW: EP = 8: rows 0..7 of the fragment are hi, 8..15 mid and lo; EP = 16: one fragment each
+    float acc[kFrags][EP / 8][4] = {};
+    int slot = 0, load_slot = kFewStages - 1;
+    for (int batch = t0; batch < t1; batch += kFewTokens) {
+        if (batch > t0) __syncthreads();  // d of the batch before has been used
+        const int count = min(kFewTokens, t1 - batch);
+        for (int i = tid; i < (count + kFewTile - 1) / kFewTile * kFewTile; i += kFewThreads) {
+            float d[EP];
+#pragma unroll
+            for (int e = 0; e < EP; ++e) d[e] = 0.0f;
+            if (i < count) {
+                const int64_t t = batch + i;
+                float dot = 0.0f;
+                for (int k = 0; k < topk; ++k) dot = fmaf(weights[t * topk + k], grad_weights[t * topk + k], dot);
+                if (grad_logits) {
+#pragma unroll
+                    for (int e = 0; e < EP; ++e)
+                        if (e < experts) d[e] = grad_logits[t * experts + e];
+                }
+                for (int k = 0; k < topk; ++k) {  // in order: a repeated id adds the same way every time
+                    const int id = ids[t * topk + k];
+                    const float v = weights[t * topk + k] * (grad_weights[t * topk + k] - dot);
+                    if (id >= experts) continue;
+#pragma unroll
+                    for (int e = 0; e < EP; ++e)
+                        if (id == e) d[e] += v;
+                }
+            }
+            uint32_t* out = reinterpret_cast<uint32_t*>(d_rows + i * few_d_row<EP>());
+#pragma unroll
+            for (int part = 0; part < 3; ++part)
+#pragma unroll
+                for (int e = 0; e < EP; e += 2)
+                    out[(part * EP + e) / 2] = bf16_part(d[e]) | bf16_part(d[e + 1]) << 16;
+        }
+        __syncthreads();
+        if (!active) continue;
+        for (int first = batch; first < batch + count; first += kFewTile) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+            __syncwarp();
+            if (sums) load(load_slot);  // past the range: zeros
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            const uint32_t xs = ring + slot * kFewStage;
+            const uint32_t ds = d_at + (first - batch) * few_d_row<EP>();
+#pragma unroll
+            for (int k = 0; k < kFewTile / 16; ++k) {
+                // the 8 x 8 blocks (token half, part block) of these 16 tokens; matrix m of an
+                // ldmatrix is addressed by lanes 8 m .. 8 m + 7
+                const uint32_t at = ds + (k * 16 + (lane & 7)) * few_d_row<EP>();
+                const int m = lane >> 3;
+                if (sums) {
+                    // A = d^T: {rows 0-7, rows 8-15} x {tokens 0-7, tokens 8-15}, transposed on load
+                    uint32_t first_a[4], second_a[4], third_a[4];
+                    const uint32_t at_t = at + (m >> 1) * 8 * few_d_row<EP>() + (m & 1) * 16;
+                    ldmatrix4_trans(at_t, first_a);            // EP 8: hi, mid; EP 16: hi
+                    ldmatrix4_trans(at_t + 2 * EP, second_a);  // EP 8: mid, lo; EP 16: mid
+                    if constexpr (EP == 16) ldmatrix4_trans(at_t + 4 * EP, third_a);  // lo
+#pragma unroll
+                    for (int f = 0; f < kFrags; f += 2) {
+                        uint32_t bx[4];  // {tokens 0-7, 8-15} of columns 8 f, then of the next eight
+                        ldmatrix4_trans(xs + (k * 16 + (lane & 7) + (m & 1) * 8) * kFewRow + (f + (m >> 1)) * 16, bx);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            if constexpr (EP == 8) {
+                                mma_k16(acc[f + q][0], 0, second_a[1], 0, second_a[3], bx[2 * q], bx[2 * q + 1]);
+                                mma_k16(acc[f + q][0], first_a[0], first_a[1], first_a[2], first_a[3], bx[2 * q],
+                                        bx[2 * q + 1]);
+                            } else {
+                                mma_k16(acc[f + q][1], third_a[0], third_a[1], third_a[2], third_a[3], bx[2 * q],
+                                        bx[2 * q + 1]);
+                                mma_k16(acc[f + q][1], second_a[0], second_a[1], second_a[2], second_a[3],
+                                        bx[2 * q], bx[2 * q + 1]);
+                                mma_k16(acc[f + q][0], first_a[0], first_a[1], first_a[2], first_a[3], bx[2 * q],
+                                        bx[2 * q + 1]);
+                            }
+                        }
+                    }
+                }
+                if (grad_x) {
+                    // A = d: {tokens 0-7, tokens 8-15} x {k 0-7, k 8-15}
+                    uint32_t hi[4], mid[4];
+                    const uint32_t at_d = at + (m & 1) * 8 * few_d_row<EP>() + (m >> 1) * 16;
+                    ldmatrix4(at_d, hi);  // EP 8: hi, mid; EP 16: hi
+                    if constexpr (EP == 16) ldmatrix4(at_d + 2 * EP, mid);
+                    __syncwarp();  // x of these tokens has been read: dx may take its place
+#pragma unroll
+                    for (int f = 0; f < kFrags; ++f) {
+                        float c[4];
+                        if constexpr (EP == 8) {
+                            mma_k16_first(c, hi[0], hi[1], 0, 0, w_lo[f][0], 0);
+                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_hi[f][0], w_hi[f][0]);
+                        } else {
+                            mma_k16_first(c, hi[0], hi[1], hi[2], hi[3], w_lo[f][0], w_lo[f][1]);
+                            mma_k16(c, mid[0], mid[1], mid[2], mid[3], w_hi[f][0], w_hi[f][1]);
+                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_hi[f][0], w_hi[f][1]);
+                        }
+                        const uint32_t to = xs + (k * 16 + (lane >> 2)) * kFewRow + f * 16 + (lane & 3) * 4;
+                        const __nv_bfloat162 low = __floats2bfloat162_rn(c[0], c[1]);
+                        const __nv_bfloat162 high = __floats2bfloat162_rn(c[2], c[3]);
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<const uint32_t*>(&low)) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 8 * kFewRow), "r"(*reinterpret_cast<const uint32_t*>(&high)) : "memory");
+                    }
+                }
+            }
+            if (grad_x) {
+                __syncwarp();
+                const uint8_t* from = few_smem_raw + (warp * kFewStages + slot) * kFewStage + lane_at;
+#pragma unroll
+                for (int j = 0; j < kFewTile / 4; ++j) {
+                    if (in_cols && first + row + 4 * j < t1)
+                        *reinterpret_cast<uint4*>(to_dx) = *reinterpret_cast<const uint4*>(from + 4 * j * kFewRow);
+                    to_dx += step;
+                }
+                __syncwarp();  // the slot is free again
+            }
+            if (++slot == kFewStages) slot = 0;
+            if (++load_slot == kFewStages) load_slot = 0;
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!active || !sums) return;
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f) {
+        const int64_t h = h0 + f * 8 + 2 * (lane & 3);
+        if (h >= hidden) continue;
+        float* at = sums + static_cast<int64_t>(blockIdx.y) * experts * hidden + h;
+        const int e = lane >> 2;
+        if constexpr (EP == 8) {  // expert e: rows e and e + 8
+            if (e < experts)
+                *reinterpret_cast<float2*>(at + e * hidden) =
+                    make_float2(acc[f][0][0] + acc[f][0][2], acc[f][0][1] + acc[f][0][3]);
+        } else {
+            if (e < experts)
+                *reinterpret_cast<float2*>(at + e * hidden) =
+                    make_float2(acc[f][0][0] + acc[f][1][0], acc[f][0][1] + acc[f][1][1]);
+            if (e + 8 < experts)
+                *reinterpret_cast<float2*>(at + (e + 8) * hidden) =
+                    make_float2(acc[f][0][2] + acc[f][1][2], acc[f][0][3] + acc[f][1][3]);
+        }
+    }
+}
+
+// out = the parts' sum, in a fixed order: SLICES threads per vector add a stretch of
+// the parts each, the first adds the stretches' sums.
+template <int SLICES>
+__global__ void __launch_bounds__(256)
+add_parts_kernel(const float4* __restrict__ parts, float4* __restrict__ out, int64_t vecs, int ranges) {
+    constexpr int kColumns = 256 / SLICES;
+    __shared__ float4 sums[SLICES][kColumns];
+    pdl_trigger();
+    pdl_wait();
+    const int column = threadIdx.x % kColumns, slice = threadIdx.x / kColumns;
+    const int64_t i = blockIdx.x * static_cast<int64_t>(kColumns) + column;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i < vecs) {
+        const int from = ranges * slice / SLICES, to = ranges * (slice + 1) / SLICES;
+#pragma unroll 8
+        for (int r = from; r < to; ++r) {
             const float4 v = parts[r * vecs + i];
             sum.x += v.x;
             sum.y += v.y;
             sum.z += v.z;
             sum.w += v.w;
         }
-        out[i] = sum;
     }
+    if constexpr (SLICES > 1) {
+        sums[slice][column] = sum;
+        __syncthreads();
+        if (slice > 0) return;
+        for (int s = 1; s < SLICES; ++s) {
+            const float4 v = sums[s][column];
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+    }
+    if (i < vecs) out[i] = sum;
 }
 
 // ------------------------------------------------------------------ host side
@@ -568,12 +847,32 @@ int token_ranges(int64_t tokens, int64_t hidden, int experts, int sms) {
 
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// The few-experts kernel: ranges of tokens so that every SM has the two CTAs that it
+// holds, of whole tiles.
+struct FewShape {
+    int columns, range, ranges;
+};
+FewShape few_shape(int64_t tokens, int64_t hidden, int sms) {
+    FewShape f;
+    f.columns = static_cast<int>((hidden + kFewCols - 1) / kFewCols);
+    const int64_t ranges = 2 * sms / f.columns < 1 ? 1 : 2 * sms / f.columns;
+    f.range = static_cast<int>(((tokens + ranges - 1) / ranges + kFewTile - 1) / kFewTile * kFewTile);
+    f.ranges = static_cast<int>((tokens + f.range - 1) / f.range);
+    return f;
+}
+
 struct Layout {
     int64_t parts, weight, offsets, sums, total;
 };
 Layout layout(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw, int sms) {
     const int64_t e8 = pad8(experts);
-    Layout l;
+    Layout l = {};
+    if (tokens == 0) return l;  // nothing is launched but a fill
+    if (experts <= kFewExperts) {
+        const int64_t ranges = few_shape(tokens, hidden, sms).ranges;
+        l.total = dw && ranges > 1 ? round256(ranges * experts * hidden * 4) : 0;
+        return l;
+    }
     l.parts = 0;
     l.weight = round256(tokens * 4 * e8 * 2);
     l.offsets = l.weight + (dx ? round256(hidden * 3 * e8 * 2) : 0);
@@ -590,6 +889,40 @@ cudaError_t device_sms(int* sms) {
     if (cached[device & 63] == 0)
         MOE_CUDA_TRY(cudaDeviceGetAttribute(&cached[device & 63], cudaDevAttrMultiProcessorCount, device));
     *sms = cached[device & 63];
+    return cudaSuccess;
+}
+
+cudaError_t add_parts(const float* parts, float* out, int64_t count, int ranges, cudaStream_t stream) {
+    // Eight threads per vector where there are many parts (74 parts of 8 x 4096: 16 us with one).
+    const int64_t vecs = count / 4;
+    const int columns = ranges >= 16 ? 32 : 256;
+    auto kernel = ranges >= 16 ? add_parts_kernel<8> : add_parts_kernel<1>;
+    return launch_dependent(kernel, dim3(static_cast<unsigned>((vecs + columns - 1) / columns)), dim3(256), 0,
+                            stream, reinterpret_cast<const float4*>(parts), reinterpret_cast<float4*>(out),
+                            vecs, ranges);
+}
+
+cudaError_t few_experts(const __nv_bfloat16* x, const float* weight, const int32_t* ids,
+                        const float* weights, const float* grad_weights, const float* grad_logits,
+                        __nv_bfloat16* grad_x, float* grad_weight, float* scratch, int64_t tokens,
+                        int64_t hidden, int experts, int topk, int sms, cudaStream_t stream) {
+    const FewShape f = few_shape(tokens, hidden, sms);
+    float* sums = grad_weight && f.ranges > 1 ? scratch : grad_weight;
+    const bool eight = experts <= 8;
+    auto kernel = eight ? router_few_kernel<8> : router_few_kernel<16>;
+    const int smem = eight ? few_smem<8>() : few_smem<16>();
+    static bool configured[2][64] = {};
+    int device = 0;
+    MOE_CUDA_TRY(cudaGetDevice(&device));
+    if (!configured[eight][device & 63]) {
+        MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        configured[eight][device & 63] = true;
+    }
+    MOE_CUDA_TRY(launch_dependent(kernel, dim3(f.columns, f.ranges), dim3(kFewThreads), smem, stream, x, weight,
+                                  ids, weights, grad_weights, grad_logits, grad_x, sums, static_cast<int>(tokens),
+                                  hidden, experts, topk, f.range));
+    if (grad_weight && f.ranges > 1)
+        return add_parts(sums, grad_weight, experts * hidden, f.ranges, stream);
     return cudaSuccess;
 }
 
@@ -617,6 +950,11 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
     const Layout l = layout(tokens, hidden, experts, grad_x != nullptr, grad_weight != nullptr, sms);
     char* base = static_cast<char*>(scratch);
     auto* parts = reinterpret_cast<__nv_bfloat16*>(base + l.parts);
+
+    if (experts <= kFewExperts)
+        return few_experts(static_cast<const __nv_bfloat16*>(x), weight, ids, weights, grad_weights, grad_logits,
+                           static_cast<__nv_bfloat16*>(grad_x), grad_weight, reinterpret_cast<float*>(base + l.sums),
+                           tokens, hidden, experts, topk, sms, stream);
 
     const int64_t blocks = (tokens + 7) / 8;
     const unsigned grid = static_cast<unsigned>(blocks < 8ll * sms ? blocks : 8ll * sms);
@@ -681,15 +1019,8 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
         const unsigned tiles = static_cast<unsigned>((hidden + tile - 1) / tile * (pair ? 2 : 1));
         MOE_CUDA_TRY(launch_dependent(kernel, dim3(tiles, used), dim3(pair ? kPairThreads : kDwThreads),
                                       p.stages * stage_bytes + 1024, stream, map_x, map_d, p));
-        if (used > 1) {
-            const int64_t vecs = experts * hidden / 4;
-            const int64_t need_ctas = (vecs + 255) / 256;
-            MOE_CUDA_TRY(launch_dependent(add_parts_kernel,
-                                          dim3(static_cast<unsigned>(need_ctas < 8ll * sms ? need_ctas : 8ll * sms)),
-                                          dim3(256), 0, stream, reinterpret_cast<const float4*>(p.out),
-                                          reinterpret_cast<float4*>(grad_weight), vecs,
-                                          static_cast<int>(used)));
-        }
+        if (used > 1)
+            MOE_CUDA_TRY(add_parts(p.out, grad_weight, experts * hidden, static_cast<int>(used), stream));
     }
     return cudaSuccess;
 }

@@ -100,10 +100,12 @@ int moe_balance_loss_backward(const void* logits, int32_t dtype, const float* bi
  *             a repeated id adds each time)
  *   grad_x [tokens, hidden] bf16 = d . router_weight  (rounded once; NULL: not computed)
  *   grad_router_weight [experts, hidden] fp32 = d^T . x  (written; NULL: not computed)
- * on tcgen05 with d and the weight split into bf16 parts: the products are
- * fp32-accurate for grad_router_weight (d to 2^-24) and to 2^-16 for grad_x.
+ * on the tensor cores with d and the weight split into bf16 parts: d enters
+ * grad_router_weight to 2^-24, and the products of grad_x are good to 2^-16 of
+ * their size.
  * Gradients that are not finite give results that are not finite.  Fixed
- * summation order.  hidden % 8 == 0; x and the gradients 16-byte aligned.
+ * summation order.  hidden % 8 == 0; x, router_weight and their gradients 16-byte
+ * aligned.
  * scratch: 256-byte aligned, not initialised, its size for the current device;
  * calls that may overlap in time need one each. */
 int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int32_t experts,
