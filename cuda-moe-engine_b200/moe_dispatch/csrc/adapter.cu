@@ -78,11 +78,19 @@ __device__ __forceinline__ int expert_of(const Adapter& p, int64_t row) {
     return lo;
 }
 
-__device__ __forceinline__ int row_key(const Adapter& p, int64_t row, int64_t valid) {
-    if (row >= valid) return kOutside;
+// Key of one row for a whole warp: the spans that end at or before the row are
+// counted, all their ends loaded at once (a search would wait for each).
+__device__ __forceinline__ int row_key(const Adapter& p, int64_t row, int lane) {
     const int adapter = p.row_adapters[row];
-    if (adapter < 0 || adapter >= p.adapters) return kNone;
-    return adapter * p.experts + expert_of(p, row);
+    int expert = 0;
+    if (p.offsets) {
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + lane;
+            expert += __popc(__ballot_sync(0xffffffffu, e < p.experts && p.offsets[e + 1] <= row));
+        }
+        if (expert >= p.experts) return kOutside;
+    }
+    return adapter < 0 || adapter >= p.adapters ? kNone : adapter * p.experts + expert;
 }
 
 __device__ __forceinline__ float silu_times(float g, float u) { return (g / (1.0f + expf(-g))) * u; }
@@ -101,82 +109,118 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float sum)
     return fmaf(bf16_hi(a.w), bf16_hi(b.w), sum);
 }
 
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// 16 bytes, or zeros when !in (the source is not read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // ------------------------------------------------------------------ few rows
 
-constexpr int kRowsSplitK = 2048;  // K elements per warp: 8 loads of 16 bytes a lane
+constexpr int kRowsSplitK = 2048;  // K elements per CTA
 
+// CTA: one row, eight rows of its A (a warp each), 2048 elements of K.  Everything is
+// copied to shared memory at once, so that all of it is in flight together; loads
+// into registers were used one by one (16.8 us against 11 at 134 rows of 14336).
 __global__ void __launch_bounds__(256) shrink_rows_kernel(const Adapter p) {
-    const int lane = threadIdx.x & 31;
+    __shared__ uint4 xs[kRowsSplitK / 8];
+    __shared__ uint4 as[8][kRowsSplitK / 8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_trigger();
     pdl_wait();
     const int64_t row = blockIdx.x;
-    const int j = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int key = row_key(p, row, valid_rows(p));
-    if (key < 0 || j >= p.rank) return;
+    const int key = row_key(p, row, lane);
+    if (key < 0) return;
+    const int j = blockIdx.y * 8 + warp;  // < rank: rank is a multiple of 8
     const int64_t k0 = static_cast<int64_t>(blockIdx.z) * kRowsSplitK;
-    const int count = static_cast<int>(p.k - k0 < kRowsSplitK ? p.k - k0 : kRowsSplitK);
+    const int vecs = static_cast<int>(p.k - k0 < kRowsSplitK ? p.k - k0 : kRowsSplitK) / 8;
     const bf16* x = p.x + row * p.k + k0;
     const bf16* a = p.a + (static_cast<int64_t>(key) * p.rank + j) * p.k + k0;
-    uint4 xv[8], av[8];
+    if (static_cast<int>(threadIdx.x) < vecs) copy16(smem_addr(&xs[threadIdx.x]), x + threadIdx.x * 8, true);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = (lane + 32 * i) * 8;
-        const bool in = c < count;
-        av[i] = in ? __ldg(reinterpret_cast<const uint4*>(a + c)) : make_uint4(0, 0, 0, 0);
-        xv[i] = in ? __ldg(reinterpret_cast<const uint4*>(x + c)) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < kRowsSplitK / 8; i += 32)
+        if (i + lane < vecs) copy16(smem_addr(&as[warp][i + lane]), a + (i + lane) * 8, true);
+    copy_commit();
+    copy_wait<0>();
+    __syncthreads();
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = dot8(xv[i], av[i], sum);
+    for (int i = 0; i < kRowsSplitK / 8; i += 32)
+        if (i + lane < vecs) sum = dot8(xs[i + lane], as[warp][i + lane], sum);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (lane == 0) p.s[(static_cast<int64_t>(blockIdx.z) * p.rows + row) * p.rank + j] = sum;
 }
 
-// LANES (a power of two >= rank / 8) lanes per column, kUnroll columns per lane.
+// CTA: one row, 1024 / LANES columns (with SwiGLU as many gate and up columns), LANES (a
+// power of two >= rank / 8) lanes per column with 16 bytes of B each.  B, base and the
+// parts of s are copied to shared memory together, as above.
+constexpr int kSplitsAtOnce = 8;
+
 template <int LANES, bool SWIGLU>
 __global__ void __launch_bounds__(256) expand_rows_kernel(const Adapter p) {
-    constexpr int kUnroll = 4, kStep = 256 / LANES;
+    constexpr int kUnroll = 4, kStep = 256 / LANES, kHalves = SWIGLU ? 2 : 1, kCols = kUnroll * kStep;
+    __shared__ uint4 bs[kHalves][kUnroll][256];
+    __shared__ uint4 base_s[kHalves][kCols / 8];
+    __shared__ __align__(16) float s_s[kSplitsAtOnce][LANES * 8];
+    const int tid = threadIdx.x, chunk = tid % LANES, column = tid / LANES;
     pdl_trigger();
     pdl_wait();
     const int64_t row = blockIdx.y;
-    const int key = row_key(p, row, valid_rows(p));
+    const int key = row_key(p, row, tid & 31);
     if (key == kOutside) return;
     if (key == kNone && !SWIGLU && p.out == p.base) return;
-    const int chunk = threadIdx.x % LANES;
-    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * (kUnroll * kStep) + threadIdx.x / LANES;
-    const bf16* base = p.base + row * p.n;
-    float d[kUnroll][SWIGLU ? 2 : 1] = {};
-    if (key >= 0) {
-        const bool in_rank = chunk * 8 < p.rank;
-        const bf16* b = p.b + static_cast<int64_t>(key) * p.n * p.rank + chunk * 8;
-        uint4 bv[kUnroll][SWIGLU ? 2 : 1];
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kCols;
+    const int cols = static_cast<int>(p.cols - c0 < kCols ? p.cols - c0 : kCols);
+    const bool in_rank = key >= 0 && chunk * 8 < p.rank;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        const int64_t first = c0 + h * p.cols;
+        if (tid < cols / 8) copy16(smem_addr(&base_s[h][tid]), p.base + row * p.n + first + tid * 8, true);
+        const bf16* b = p.b + ((key >= 0 ? static_cast<int64_t>(key) : 0) * p.n + first + column) * p.rank + chunk * 8;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
-                const int64_t c = c0 + u * kStep;
-                bv[u][h] = in_rank && c < p.cols
-                               ? __ldg(reinterpret_cast<const uint4*>(b + (c + h * p.cols) * p.rank))
-                               : make_uint4(0, 0, 0, 0);
-            }
-        float s[8] = {};
-        if (in_rank) {
-            for (int z = 0; z < p.splits; ++z) {
-                const float4* part = reinterpret_cast<const float4*>(
-                    p.s + (static_cast<int64_t>(z) * p.rows + row) * p.rank + chunk * 8);
-                const float4 lo = part[0], hi = part[1];
-                s[0] += lo.x, s[1] += lo.y, s[2] += lo.z, s[3] += lo.w;
-                s[4] += hi.x, s[5] += hi.y, s[6] += hi.z, s[7] += hi.w;
-            }
+            if (in_rank && column + u * kStep < cols)
+                copy16(smem_addr(&bs[h][u][tid]), b + u * kStep * p.rank, true);
+    }
+    float s[8] = {};
+    for (int z0 = 0; z0 < (key >= 0 ? p.splits : 0); z0 += kSplitsAtOnce) {
+        const int count = min(kSplitsAtOnce, p.splits - z0);
+        if (z0 > 0) __syncthreads();
+        for (int i = tid; i < count * (p.rank / 4); i += 256) {
+            const int z = i / (p.rank / 4), q = i % (p.rank / 4) * 4;
+            copy16(smem_addr(&s_s[z][q]), p.s + ((z0 + z) * p.rows + row) * p.rank + q, true);
         }
-        const float scale = p.scale ? p.scale[key / p.experts] : 1.0f;
+        copy_commit();
+        copy_wait<0>();
+        __syncthreads();
+        if (in_rank)
+            for (int z = 0; z < count; ++z)
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+                for (int i = 0; i < 8; ++i) s[i] += s_s[z][chunk * 8 + i];
+    }
+    copy_commit();
+    copy_wait<0>();
+    __syncthreads();  // base has arrived everywhere
+    const float scale = key >= 0 && p.scale ? p.scale[key / p.experts] : 1.0f;
 #pragma unroll
-            for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
-                const uint4 v = bv[u][h];
-                float sum = s[0] * bf16_lo(v.x);
+    for (int u = 0; u < kUnroll; ++u) {
+        const int c = column + u * kStep;
+        float y[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            float sum = 0.0f;
+            if (in_rank && c < cols) {
+                const uint4 v = bs[h][u][tid];
+                sum = s[0] * bf16_lo(v.x);
                 sum = fmaf(s[1], bf16_hi(v.x), sum);
                 sum = fmaf(s[2], bf16_lo(v.y), sum);
                 sum = fmaf(s[3], bf16_hi(v.y), sum);
@@ -184,21 +228,13 @@ __global__ void __launch_bounds__(256) expand_rows_kernel(const Adapter p) {
                 sum = fmaf(s[5], bf16_hi(v.z), sum);
                 sum = fmaf(s[6], bf16_lo(v.w), sum);
                 sum = fmaf(s[7], bf16_hi(v.w), sum);
-#pragma unroll
-                for (int off = LANES / 2; off > 0; off >>= 1)
-                    sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                d[u][h] = sum * scale;
             }
-    }
-    if (chunk != 0) return;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const int64_t c = c0 + u * kStep;
-        if (c >= p.cols) continue;
-        const float g = __bfloat162float(base[c]) + d[u][0];
-        float y = g;
-        if constexpr (SWIGLU) y = silu_times(g, __bfloat162float(base[c + p.cols]) + d[u][1]);
-        p.out[row * p.cols + c] = __float2bfloat16_rn(y);
+            for (int off = LANES / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            y[h] = c < cols ? __bfloat162float(reinterpret_cast<const bf16*>(base_s[h])[c]) + sum * scale : 0.0f;
+        }
+        if constexpr (SWIGLU) y[0] = silu_times(y[0], y[1]);
+        if (chunk == 0 && c < cols) p.out[row * p.cols + c0 + c] = __float2bfloat16_rn(y[0]);
     }
 }
 
@@ -319,20 +355,6 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const Adapter p, in
 
 constexpr int kTileRows = 64;
 constexpr int kTileThreads = 128;  // of the shrink kernel: four warps, 16 rows each
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// 16 bytes, or zeros when !in (the source is not read then).
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
