@@ -55,7 +55,7 @@ SIGNATURES = {
     "moe_grouped_gemm_swiglu": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]),
     "moe_grouped_gemm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]),
     "moe_grouped_gemm_tile": (ctypes.c_int32, [_I64, _I32]),
-    "moe_adapter_scratch_bytes": (ctypes.c_int64, [_I64, _I64, _I32, _I32]),
+    "moe_adapter_scratch_bytes": (ctypes.c_int64, [_I64, _I64, _I32, _I32, _I32]),
     "moe_adapter_add": (
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _I64, _P],
@@ -511,7 +511,7 @@ class Extension:
         adapters, experts, rank = a.shape[:3]
 
         def run():
-            size = self.lib.moe_adapter_scratch_bytes(rows, k_dim, rank, adapters)
+            size = self.lib.moe_adapter_scratch_bytes(rows, k_dim, rank, adapters, experts)
             _require(size >= 0, self.lib.moe_last_error().decode())
             # a buffer of this call's own, as in launch_balance_loss
             scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)

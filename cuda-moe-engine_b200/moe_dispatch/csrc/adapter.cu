@@ -845,8 +845,18 @@ int padded_rank(int rank) {
     return r;
 }
 
-// Which form: see the comment at kFewRows.
+// Which form.  Measured in graphs (us, few-rows form / tiles), 8 experts, rank 16, down
+// projection 14336 -> 4096: one adapter, 128 rows 13 / 24, 256 rows 22 / 26, 512 rows
+// 41 / 31, 1024 rows 77 / 37; 64 adapters, a row's own each, 512 rows 46 / 129, 1024 rows
+// 83 / 159, 2048 rows 156 / 184.  (Rank 8 to 128 and 4096 -> 28672 cross over near the
+// same places.)  Where the rows are no more than twice the pairs that they may fall
+// on, tiles would hold few rows each.
 constexpr int64_t kFewRows = 256;
+constexpr int64_t kFewRowsScattered = 1024;
+bool few_rows_form(int64_t rows, int adapters, int experts) {
+    return rows <= kFewRows ||
+           (rows <= kFewRowsScattered && rows <= 2ll * adapters * experts);
+}
 
 struct Shape {
     bool few;
@@ -857,9 +867,9 @@ struct Shape {
 
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int sms) {
+Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int experts, int sms) {
     Shape f = {};
-    f.few = rows <= kFewRows;
+    f.few = few_rows_form(rows, adapters, experts);
     if (f.few) {
         f.split_k = kRowsSplitK;
         f.splits = static_cast<int>((k + kRowsSplitK - 1) / kRowsSplitK);
@@ -975,10 +985,11 @@ cudaError_t many_rows(const Adapter& p, const Shape& f, int sms, cudaStream_t st
 
 }  // namespace
 
-cudaError_t adapter_scratch_bytes(int64_t rows, int64_t k, int rank, int adapters, int64_t* bytes) {
+cudaError_t adapter_scratch_bytes(int64_t rows, int64_t k, int rank, int adapters, int experts,
+                                  int64_t* bytes) {
     int sms = 0;
     MOE_CUDA_TRY(device_sms(&sms));
-    *bytes = shape_of(rows, k, rank, adapters, sms).total;
+    *bytes = shape_of(rows, k, rank, adapters, experts, sms).total;
     return cudaSuccess;
 }
 
@@ -989,7 +1000,7 @@ cudaError_t launch_adapter(const void* base, const void* x, const void* a, const
     if (rows == 0) return cudaSuccess;
     int sms = 0;
     MOE_CUDA_TRY(device_sms(&sms));
-    const Shape f = shape_of(rows, k, rank, adapters, sms);
+    const Shape f = shape_of(rows, k, rank, adapters, experts, sms);
     Adapter p;
     p.base = static_cast<const bf16*>(base);
     p.x = static_cast<const bf16*>(x);

@@ -320,7 +320,7 @@ int moe_swiglu(const void* projection, int32_t dtype, const int32_t* valid_rows,
                        "moe_swiglu");
 }
 
-static int check_adapter_shape(int64_t rows, int64_t k, int32_t rank, int32_t adapters) {
+static int check_adapter_shape(int64_t rows, int64_t k, int32_t rank, int32_t adapters, int32_t experts) {
     if (rows < 0 || rows > INT_MAX / 4) return fail(MOE_ERR_INVALID, "rows must be in 0..INT_MAX / 4");
     if (k < 8 || k % 8 || k > INT_MAX / 8)
         return fail(MOE_ERR_INVALID, "adapter dimensions must be positive multiples of 8");
@@ -328,13 +328,16 @@ static int check_adapter_shape(int64_t rows, int64_t k, int32_t rank, int32_t ad
         return fail(MOE_ERR_INVALID, "rank must be a multiple of 8 up to %d", moe::kMaxAdapterRank);
     if (adapters < 1 || adapters > moe::kMaxAdapters)
         return fail(MOE_ERR_INVALID, "adapters must be in 1..%d", moe::kMaxAdapters);
+    if (experts < 1 || experts > moe::kMaxDispatchExperts)
+        return fail(MOE_ERR_INVALID, "experts must be in 1..%d", moe::kMaxDispatchExperts);
     return MOE_OK;
 }
 
-int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters) {
-    if (check_adapter_shape(rows, k_dim, rank, adapters) != MOE_OK) return -1;
+int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters,
+                                  int32_t experts) {
+    if (check_adapter_shape(rows, k_dim, rank, adapters, experts) != MOE_OK) return -1;
     int64_t bytes = 0;
-    if (cuda_status(moe::adapter_scratch_bytes(rows, k_dim, rank, adapters, &bytes),
+    if (cuda_status(moe::adapter_scratch_bytes(rows, k_dim, rank, adapters, experts, &bytes),
                     "moe_adapter_scratch_bytes") != MOE_OK)
         return -1;
     return bytes;
@@ -345,12 +348,10 @@ static int adapter_common(const void* base, const void* x, const void* a, const 
                           void* out, int64_t rows, int64_t k_dim, int64_t out_cols, int32_t rank,
                           int32_t adapters, int32_t experts, bool swiglu, void* scratch,
                           int64_t scratch_bytes, void* stream) {
-    const int checked = check_adapter_shape(rows, k_dim, rank, adapters);
+    const int checked = check_adapter_shape(rows, k_dim, rank, adapters, experts);
     if (checked != MOE_OK) return checked;
     if (out_cols < 8 || out_cols % 8 || out_cols > INT_MAX / 16)
         return fail(MOE_ERR_INVALID, "adapter dimensions must be positive multiples of 8");
-    if (experts < 1 || experts > moe::kMaxDispatchExperts)
-        return fail(MOE_ERR_INVALID, "experts must be in 1..%d", moe::kMaxDispatchExperts);
     if (!offsets && experts != 1)
         return fail(MOE_ERR_INVALID, "offsets may be null for one expert only");
     if ((rows + 63) / 64 * ((out_cols + 63) / 64) > INT_MAX)
@@ -361,7 +362,7 @@ static int adapter_common(const void* base, const void* x, const void* a, const 
         return fail(MOE_ERR_INVALID, "adapter operands must be 16-byte aligned");
     if (swiglu && base == out) return fail(MOE_ERR_INVALID, "out must not be the projection");
     int64_t need = 0;
-    const int sized = cuda_status(moe::adapter_scratch_bytes(rows, k_dim, rank, adapters, &need), "moe_adapter");
+    const int sized = cuda_status(moe::adapter_scratch_bytes(rows, k_dim, rank, adapters, experts, &need), "moe_adapter");
     if (sized != MOE_OK) return sized;
     if (!scratch || !aligned(scratch, 256) || scratch_bytes < need)
         return fail(MOE_ERR_INVALID, "adapter scratch too small or unaligned (%lld bytes needed)",

@@ -49,7 +49,8 @@ cudaError_t read_route_backward_status(int32_t* code, bool clear);
 // Low-rank adapters beside the grouped projections (adapter.cu).
 constexpr int kMaxAdapters = 512;
 constexpr int kMaxAdapterRank = 128;
-cudaError_t adapter_scratch_bytes(int64_t rows, int64_t k, int rank, int adapters, int64_t* bytes);
+cudaError_t adapter_scratch_bytes(int64_t rows, int64_t k, int rank, int adapters, int experts,
+                                  int64_t* bytes);
 cudaError_t launch_adapter(const void* base, const void* x, const void* a, const void* b,
                            const float* scale, const int32_t* row_adapters, const int32_t* offsets,
                            void* out, int64_t rows, int64_t k, int64_t n, int rank, int adapters,

@@ -214,7 +214,8 @@ int moe_grouped_gemm(const void* a, const void* weight, const int32_t* offsets, 
  * not reach rows of others.  k_dim, n_cols multiples of 8; rank a multiple of 8
  * up to 128; adapters <= 512.  scratch: 256-byte aligned, not initialised, sized
  * for the current device; calls that may overlap in time need one each. */
-int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters);
+int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters,
+                                  int32_t experts);
 int moe_adapter_add(const void* base, const void* x, const void* a, const void* b, const float* scale,
                     const int32_t* row_adapters, const int32_t* offsets, void* out, int64_t rows,
                     int64_t k_dim, int64_t n_cols, int32_t rank, int32_t adapters, int32_t experts,

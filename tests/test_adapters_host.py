@@ -128,5 +128,5 @@ def test_library_refuses_bad_row_maps_and_queries():
     assert lib.moe_adapter_rows(None, None, None, None, None, 4, 2, 0, 16, None) == 1
     assert lib.moe_adapter_rows(None, None, None, None, None, 4, 2, 8, 16, None) == 1
     assert "null" in lib.moe_last_error().decode()
-    assert lib.moe_adapter_scratch_bytes(4, 12, 8, 2) == -1
-    assert lib.moe_adapter_scratch_bytes(4, 16, 8, 600) == -1
+    assert lib.moe_adapter_scratch_bytes(4, 12, 8, 2, 1) == -1
+    assert lib.moe_adapter_scratch_bytes(4, 16, 8, 600, 1) == -1

@@ -111,7 +111,9 @@ CASES = [
     (1500, 200, 72, 300, 16),                    # runs of a few rows
     ([512] * 5, 136, 264, 3, 128),
     (5003, 64, 128, 24, 64),
-    ([9] * 64, 328, 88, 512, 8),                 # every row its own pair
+    ([9] * 64, 328, 88, 512, 8),                 # every row its own pair, few-rows form
+    ([20] * 60, 328, 88, 512, 8),                # and sorted: 1200 rows
+    ([100] * 9, 72, 136, 80, 16),                # 913 rows, scattered over 720 pairs
     ([3000, 0, 1096], 1096, 1160, 6, 96),
 ]
 
