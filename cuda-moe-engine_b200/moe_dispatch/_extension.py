@@ -122,6 +122,12 @@ def _check_cuda(tensor, anchor, name):
     _require(tensor.device == anchor.device, f"{name}: device mismatch")
 
 
+# The current stream's handle of a device; without torch's own short way to it, by
+# way of a Stream object (1.3 us a call).
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                  lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _ptr(tensor):
     return None if tensor is None else tensor.data_ptr()
 
@@ -132,6 +138,7 @@ class Extension:
     def __init__(self, lib):
         self.lib = lib
         self._scratch = {}
+        self._scratch_sizes = {}
 
     # ---------------------------------------------------------------- helpers
     def _run(self, status):
@@ -143,17 +150,28 @@ class Extension:
         index = device.index if device.index is not None else torch.cuda.current_device()
         if index != torch.cuda.current_device():
             with torch.cuda.device(index):
-                self._run(function(*args, torch.cuda.current_stream(index).cuda_stream))
+                self._run(function(*args, _stream(index)))
         else:
-            self._run(function(*args, torch.cuda.current_stream(index).cuda_stream))
+            self._run(function(*args, _stream(index)))
 
-    def _on_device(self, device, run):
-        """run() with `device` as the current one (scratch sizes depend on it)."""
-        if device.index is None or device.index == torch.cuda.current_device():
-            run()
-        else:
-            with torch.cuda.device(device):
-                run()
+    def _call_with_scratch(self, device, query, sizes, function, *args):
+        """_call with a scratch buffer behind the arguments, as large as the entry point
+        named `query` says for these sizes on `device`.  The buffer is this call's own, so calls on several streams
+        or in several captured graphs never share one."""
+        index = device.index
+        if index != torch.cuda.current_device():
+            with torch.cuda.device(index):
+                return self._call_with_scratch(device, query, sizes, function, *args)
+        key = (query, index, sizes)
+        size = self._scratch_sizes.get(key)
+        if size is None:
+            size = getattr(self.lib, query)(*sizes)
+            _require(size >= 0, self.lib.moe_last_error().decode())
+            if len(self._scratch_sizes) >= 4096:
+                self._scratch_sizes.clear()
+            self._scratch_sizes[key] = size
+        scratch = torch.empty(size or 1, dtype=torch.uint8, device=device)
+        self._run(function(*args, scratch.data_ptr(), size, _stream(index)))
 
     def scratch_bytes(self, tokens, topk, experts):
         return int(self.lib.moe_dispatch_scratch_bytes(tokens, topk, experts))
@@ -356,15 +374,12 @@ class Extension:
     def launch_balance_loss(self, logits, ids, bias, token_mask, coefficient, loss, counts, counted):
         """balance_loss_out without its tensor checks (callers have made them)."""
         tokens, experts = logits.shape
-        # the sums of each CTA: a buffer of this call's own, so calls on several
-        # streams or in several captured graphs never share one
-        size = int(self.lib.moe_balance_loss_scratch_bytes(experts))
-        scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=logits.device)
-        self._call(
-            logits.device, self.lib.moe_balance_loss,
+        self._call_with_scratch(
+            logits.device, "moe_balance_loss_scratch_bytes", (experts,),
+            self.lib.moe_balance_loss,
             logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), ids.data_ptr(),
             _ptr(token_mask), coefficient, loss.data_ptr(), counts.data_ptr(), counted.data_ptr(),
-            tokens, experts, ids.shape[1], scratch.data_ptr(), size,
+            tokens, experts, ids.shape[1],
         )
 
     def balance_loss_backward_out(self, logits, bias, token_mask, counts, counted, grad_loss,
@@ -424,21 +439,15 @@ class Extension:
                               grad_router_weight):
         """route_backward_out without its tensor checks."""
         tokens, hidden = x.shape
-        experts, topk = router_weight.shape[0], ids.shape[1]
-
-        def run():
-            size = self.lib.moe_route_backward_scratch_bytes(
-                tokens, hidden, experts, grad_x is not None, grad_router_weight is not None)
-            _require(size >= 0, self.lib.moe_last_error().decode())
-            scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
-            self._call(
-                x.device, self.lib.moe_route_backward,
-                x.data_ptr(), router_weight.data_ptr(), ids.data_ptr(), weights.data_ptr(),
-                grad_weights.data_ptr(), _ptr(grad_logits), _ptr(grad_x), _ptr(grad_router_weight),
-                tokens, hidden, experts, topk, scratch.data_ptr(), size,
-            )
-
-        self._on_device(x.device, run)
+        experts = router_weight.shape[0]
+        self._call_with_scratch(
+            x.device, "moe_route_backward_scratch_bytes",
+            (tokens, hidden, experts, grad_x is not None, grad_router_weight is not None),
+            self.lib.moe_route_backward,
+            x.data_ptr(), router_weight.data_ptr(), ids.data_ptr(), weights.data_ptr(),
+            grad_weights.data_ptr(), _ptr(grad_logits), _ptr(grad_x), _ptr(grad_router_weight),
+            tokens, hidden, experts, ids.shape[1],
+        )
 
     def _gemm_checks(self, a, weight, offsets, out):
         _require(a.is_cuda and a.is_contiguous() and a.dtype == torch.bfloat16 and a.dim() == 2,
@@ -509,20 +518,13 @@ class Extension:
         (moe_adapter_swiglu) without their tensor checks."""
         rows, k_dim = x.shape
         adapters, experts, rank = a.shape[:3]
-
-        def run():
-            size = self.lib.moe_adapter_scratch_bytes(rows, k_dim, rank, adapters, experts)
-            _require(size >= 0, self.lib.moe_last_error().decode())
-            # a buffer of this call's own, as in launch_balance_loss
-            scratch = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
-            self._call(
-                x.device, function,
-                base.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(scale),
-                row_adapters.data_ptr(), _ptr(offsets), out.data_ptr(), rows, k_dim, out.shape[1],
-                rank, adapters, experts, scratch.data_ptr(), size,
-            )
-
-        self._on_device(x.device, run)
+        self._call_with_scratch(
+            x.device, "moe_adapter_scratch_bytes", (rows, k_dim, rank, adapters, experts),
+            function,
+            base.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(scale),
+            row_adapters.data_ptr(), _ptr(offsets), out.data_ptr(), rows, k_dim, out.shape[1], rank,
+            adapters, experts,
+        )
 
     def adapter_add_out(self, base, x, a, b, scale, row_adapters, offsets, out):
         """out = base + the rows' low-rank adapters (include/moe_b200.h); out may be base."""

@@ -120,29 +120,28 @@ def _apply(base, x, a, b, row_adapters, offsets, scale, out, swiglu):
     if out is not None and (tuple(out.shape) != shape or out.dtype != torch.bfloat16
                             or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous bf16 tensor [{shape[0]},{shape[1]}]")
-    device = x.device
-    grad = torch.is_grad_enabled()
-    for t in (base, x, a, b, row_adapters, offsets, scale, out):
+    device, grad = x.device, torch.is_grad_enabled()
+    if out is not None:
+        low = out.data_ptr()
+        high = low + out.nbytes
+        if out.device != device:
+            raise ValueError("all tensors must be on the same device")
+    for t in (base, x, a, b, row_adapters, offsets, scale):
         if t is None:
             continue
         if t.device != device:
             raise ValueError("all tensors must be on the same device")
         if grad and t.requires_grad:
             raise ValueError("CUDA operators are forward-only; detach inputs or use inference_mode")
+        if out is not None:
+            start = t.data_ptr()
+            if start < high and low < start + t.nbytes and (swiglu or t is not base or start != low):
+                raise ValueError("out must not overlap an input (adapter_add may write base itself)")
     if not base.is_contiguous() or not x.is_contiguous():
         raise ValueError("base and x must be contiguous")
     if offsets is not None and not offsets.is_contiguous():
         raise ValueError("offsets must be contiguous")
     row_adapters = adapter_ids32(row_adapters, rows, "row")
-    if out is not None:
-        low = out.data_ptr()
-        high = low + out.nbytes
-        for t in (base, x, a, b, row_adapters, offsets, scale):
-            if t is None or (t is base and not swiglu and t.data_ptr() == low):
-                continue
-            start = t.data_ptr()
-            if start < high and low < start + t.nbytes:
-                raise ValueError("out must not overlap an input (adapter_add may write base itself)")
     if not x.is_cuda:
         raise RuntimeError("adapters require CUDA")
     if out is None:
