@@ -157,8 +157,8 @@ def adapter_add(base, x, a, b, row_adapters, *, offsets=None, scale=None, out=No
 
     base [R,N] and x [R,K] bf16; a [P,E,r,K] and b [P,E,N,r] bf16; row_adapters
     [R] int32 or int64: the row's adapter p, outside 0..P-1 (say -1) for none;
-    offsets [E+1] int32: expert e has rows offsets[e]..offsets[e+1]-1 (None: one
-    expert with every row); scale [P] fp32 (None: 1).  Sums in fp32, rounded once.
+    offsets [E+1] int32, from 0 up: expert e has rows offsets[e]..offsets[e+1]-1
+    (None: one expert with every row); scale [P] fp32 (None: 1).  Sums in fp32, rounded once.
     Writes ``out`` (base itself, or a bf16 [R,N] tensor that overlaps no input; a
     new one if None) and returns it.  Rows behind the last expert's are neither
     read nor written.  No host synchronisation; each call uses scratch of its own

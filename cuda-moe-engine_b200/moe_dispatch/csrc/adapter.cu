@@ -55,8 +55,8 @@ struct Adapter {
     int32_t *table, *order, *keys;
     int32_t* tile_count;          // [0] tiles, [1] stretches claimed by the expand kernel
     int2* tiles;                  // {first sorted row, rows} of each tile
-    float* s;                     // [splits][rows][padded rank]
-    int splits;
+    float* s;                     // few rows: [splits][rows][rank]; tiles: pieces (s_piece)
+    int splits;                   // of K
     int64_t split_k;              // K elements per split
 };
 
@@ -242,6 +242,20 @@ __global__ void __launch_bounds__(256) expand_rows_kernel(const Adapter p) {
 
 constexpr int kSortThreads = 1024;
 constexpr int kMaxChunks = 128;
+constexpr int kClusterChunks = 8;                 // the sort as one cluster: up to 8 chunks
+constexpr int64_t kClusterChunkRows = kSortThreads;  // of one round of rows
+constexpr int kTileRows = 64;
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word of this CTA's shared memory, in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t load_peer(const void* local, int rank) {
+    uint32_t address = smem_addr(local), value;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(address) : "r"(address), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(value) : "r"(address) : "memory");
+    return value;
+}
 
 // Buckets: the adapters, then rows without one, then rows outside every span.
 __device__ __forceinline__ int bucket_of(const Adapter& p, int64_t row, int64_t valid) {
@@ -269,31 +283,120 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const Adapter p, in
         p.table[static_cast<int64_t>(i) * gridDim.x + blockIdx.x] = counts[i];
 }
 
-// order[position] = row, keys[position] = its pair; stable inside a bucket.
-__global__ void __launch_bounds__(kSortThreads) order_kernel(const Adapter p, int64_t chunk_rows) {
+// Cuts the sorted rows' groups of equal keys into tiles.  A thread whose key
+// differs from the one before starts a group; where the next start lies in the
+// same warp the group's length is known, and the warp searches the end of its
+// last group together (32 probes at a time).  Tiles land in any order: each is
+// a piece of work of its own.  none: rows without an adapter need tiles too.
+// Called by whole warps, lane 0 at a multiple of 32; `at` may be past the rows.
+__device__ void cut_tiles(const Adapter& p, bool none, int64_t at) {
+    const int lane = threadIdx.x & 31;
+    const int key = at < p.rows ? p.keys[at] : kOutside;
+    const bool start = at < p.rows && (at == 0 || p.keys[at - 1] != key);
+    const uint32_t starts = __ballot_sync(0xffffffffu, start);
+    if (starts == 0) return;
+    const int last = 31 - __clz(starts);
+    const uint32_t later = lane == 31 ? 0 : starts >> (lane + 1);
+    int64_t length = start && later ? __ffs(later) : 0;
+    const int last_key = __shfl_sync(0xffffffffu, key, last);
+    const int64_t last_at = at - lane + last;
+    int64_t lo = at - lane + 32, hi = p.rows;  // keys[lo - 1] is last_key; the end lies in [lo, hi]
+    if (lo > hi) lo = hi;
+    while (lo < hi) {
+        const int64_t step = (hi - lo + 31) / 32;
+        const int64_t probe = lo + step * (lane + 1) - 1;
+        const uint32_t past = __ballot_sync(0xffffffffu, probe >= hi || p.keys[probe] != last_key);
+        if (past == 0) {
+            lo = hi;
+        } else {
+            const int f = __ffs(past) - 1;
+            const int64_t bound = lo + step * (f + 1) - 1;
+            if (bound < hi) hi = bound;
+            lo += step * f;
+        }
+    }
+    if (lane == last) length = lo - last_at;
+    const bool wanted = start && (key >= 0 || (none && key == kNone));
+    const int count = wanted ? static_cast<int>((length + kTileRows - 1) / kTileRows) : 0;
+    int inclusive = count;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inclusive, off);
+        if (lane >= off) inclusive += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, inclusive, 31);
+    int first = 0;
+    if (lane == 0 && total > 0) first = atomicAdd(p.tile_count, total);
+    first = __shfl_sync(0xffffffffu, first, 0);
+    if (count > 0 && lane != last)  // at most 31 rows: one tile
+        p.tiles[first + inclusive - 1] = make_int2(static_cast<int>(at), static_cast<int>(length));
+    const int last_count = __shfl_sync(0xffffffffu, count, last);
+    for (int i = lane; i < last_count; i += 32) {
+        const int64_t row = last_at + static_cast<int64_t>(i) * kTileRows;
+        const int64_t rest = lo - row;
+        p.tiles[first + total - last_count + i] =
+            make_int2(static_cast<int>(row), static_cast<int>(rest < kTileRows ? rest : kTileRows));
+    }
+}
+
+__global__ void __launch_bounds__(256) tiles_kernel(const Adapter p, bool none) {
+    pdl_trigger();
+    pdl_wait();
+    cut_tiles(p, none, blockIdx.x * 256ll + threadIdx.x);
+}
+
+// order[position] = row, keys[position] = its pair; stable inside a bucket.  One CTA
+// per chunk.  kCluster: the CTAs are one cluster, count their chunks themselves, learn
+// each other's counts from shared memory, and cut the tiles when all rows are placed,
+// in one launch instead of three.
+template <bool kCluster>
+__global__ void __launch_bounds__(kSortThreads) order_kernel(const Adapter p, int64_t chunk_rows, bool none) {
     extern __shared__ int32_t sort_smem[];
     const int buckets = p.adapters + 2;
     const int stride = buckets | 1;
     int32_t* hist = sort_smem;                  // [32 warps][buckets]
     int32_t* next = sort_smem + 32 * stride;    // [buckets] next position of this chunk's rows
-    int32_t* total = next + buckets;       // [buckets]
+    int32_t* total = next + buckets;            // [buckets]
+    int32_t* local = total + buckets;           // [buckets] this chunk's counts (cluster form)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int chunks = gridDim.x, me = blockIdx.x;
     pdl_trigger();
     for (int i = tid; i < 32 * stride; i += kSortThreads) hist[i] = 0;
+    if constexpr (kCluster)
+        for (int i = tid; i < buckets; i += kSortThreads) local[i] = 0;
     pdl_wait();
-    const int chunks = gridDim.x, me = blockIdx.x;
-    for (int b = warp; b < buckets; b += 32) {
-        int all = 0, before = 0;
-        for (int c = lane; c < chunks; c += 32) {
-            const int v = p.table[static_cast<int64_t>(b) * chunks + c];
-            all += v;
-            if (c < me) before += v;
-        }
-        all = __reduce_add_sync(0xffffffffu, all);
-        before = __reduce_add_sync(0xffffffffu, before);
-        if (lane == 0) {
+    if constexpr (kCluster) {
+        __syncthreads();
+        if (me == 0 && tid < 2) p.tile_count[tid] = 0;
+        const int64_t valid = valid_rows(p);
+        const int64_t end = (me + 1) * chunk_rows < p.rows ? (me + 1) * chunk_rows : p.rows;
+        for (int64_t row = me * chunk_rows + tid; row < end; row += kSortThreads)
+            atomicAdd(&local[bucket_of(p, row, valid)], 1);
+        cluster_barrier();
+        for (int b = tid; b < buckets; b += kSortThreads) {
+            int all = 0, before = 0;
+            for (int c = 0; c < chunks; ++c) {
+                const int v = static_cast<int>(load_peer(&local[b], c));
+                all += v;
+                if (c < me) before += v;
+            }
             total[b] = all;
             next[b] = before;
+        }
+    } else {
+        for (int b = warp; b < buckets; b += 32) {
+            int all = 0, before = 0;
+            for (int c = lane; c < chunks; c += 32) {
+                const int v = p.table[static_cast<int64_t>(b) * chunks + c];
+                all += v;
+                if (c < me) before += v;
+            }
+            all = __reduce_add_sync(0xffffffffu, all);
+            before = __reduce_add_sync(0xffffffffu, before);
+            if (lane == 0) {
+                total[b] = all;
+                next[b] = before;
+            }
         }
     }
     __syncthreads();
@@ -349,11 +452,16 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const Adapter p, in
         for (int x = warp; x < buckets; x += 32) hist[lane * stride + x] = 0;
         __syncthreads();
     }
+    if constexpr (kCluster) {
+        cluster_barrier();  // every row is in its place, and every peer's counts have been read
+        for (int64_t at = static_cast<int64_t>(me) * kSortThreads + tid; at - tid < p.rows;
+             at += static_cast<int64_t>(chunks) * kSortThreads)
+            cut_tiles(p, none, at);
+    }
 }
 
 // ------------------------------------------------------------ many rows: tiles
 
-constexpr int kTileRows = 64;
 constexpr int kTileThreads = 128;  // of the shrink kernel: four warps, 16 rows each
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -381,63 +489,6 @@ __device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// Cuts the sorted rows' groups of equal keys into tiles.  A thread whose key
-// differs from the one before starts a group; where the next start lies in the
-// same warp the group's length is known, and the warp searches the end of its
-// last group together (32 probes at a time).  Tiles land in any order: each is
-// a piece of work of its own.  none: rows without an adapter need tiles too.
-__global__ void __launch_bounds__(256) tiles_kernel(const Adapter p, bool none) {
-    pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t at = blockIdx.x * 256ll + threadIdx.x;
-    const int key = at < p.rows ? p.keys[at] : kOutside;
-    const bool start = at < p.rows && (at == 0 || p.keys[at - 1] != key);
-    const uint32_t starts = __ballot_sync(0xffffffffu, start);
-    if (starts == 0) return;
-    const int last = 31 - __clz(starts);
-    const uint32_t later = lane == 31 ? 0 : starts >> (lane + 1);
-    int64_t length = start && later ? __ffs(later) : 0;
-    const int last_key = __shfl_sync(0xffffffffu, key, last);
-    const int64_t last_at = at - lane + last;
-    int64_t lo = at - lane + 32, hi = p.rows;  // keys[lo - 1] is last_key; the end lies in [lo, hi]
-    if (lo > hi) lo = hi;
-    while (lo < hi) {
-        const int64_t step = (hi - lo + 31) / 32;
-        const int64_t probe = lo + step * (lane + 1) - 1;
-        const uint32_t past = __ballot_sync(0xffffffffu, probe >= hi || p.keys[probe] != last_key);
-        if (past == 0) {
-            lo = hi;
-        } else {
-            const int f = __ffs(past) - 1;
-            const int64_t bound = lo + step * (f + 1) - 1;
-            if (bound < hi) hi = bound;
-            lo += step * f;
-        }
-    }
-    if (lane == last) length = lo - last_at;
-    const bool wanted = start && (key >= 0 || (none && key == kNone));
-    const int count = wanted ? static_cast<int>((length + kTileRows - 1) / kTileRows) : 0;
-    int inclusive = count;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inclusive, off);
-        if (lane >= off) inclusive += y;
-    }
-    const int total = __shfl_sync(0xffffffffu, inclusive, 31);
-    int first = 0;
-    if (lane == 0 && total > 0) first = atomicAdd(p.tile_count, total);
-    first = __shfl_sync(0xffffffffu, first, 0);
-    if (count > 0 && lane != last)  // at most 31 rows: one tile
-        p.tiles[first + inclusive - 1] = make_int2(static_cast<int>(at), static_cast<int>(length));
-    const int last_count = __shfl_sync(0xffffffffu, count, last);
-    for (int i = lane; i < last_count; i += 32) {
-        const int64_t row = last_at + static_cast<int64_t>(i) * kTileRows;
-        const int64_t rest = lo - row;
-        p.tiles[first + total - last_count + i] =
-            make_int2(static_cast<int>(row), static_cast<int>(rest < kTileRows ? rest : kTileRows));
-    }
-}
 
 constexpr int kShrinkStages = 3;
 constexpr int kShrinkK = 128;                   // K elements per stage: 256 bytes of each row
@@ -448,25 +499,49 @@ template <int RN> constexpr int shrink_stage_bytes() { return (kTileRows + RN) *
 // row, so the eight rows of an ldmatrix lie in different banks.
 __device__ __forceinline__ uint32_t stage_at(int i, int c) { return i * kShrinkRow + ((c ^ (i & 7)) << 4); }
 
+template <int RN> constexpr int rank_k() { return RN < 16 ? 16 : RN; }
+
+// s of a sorted row as the tensor cores take it: for every 16 of its elements four
+// pieces of 16 bytes, piece q = bf16 {hi(2q, 2q + 1), hi(2q + 8, 2q + 9), lo of the same}.
+// A lane's part of an accumulator fragment is a piece, and so is its part of an operand.
+template <int RN> __device__ __forceinline__ uint4* s_piece(const Adapter& p, int64_t row, int kk, int q) {
+    return reinterpret_cast<uint4*>(p.s) + (row * (rank_k<RN>() / 16) + kk) * 4 + q;
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Two floats as bf16 hi parts, and the rests' as a second register.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack2(a, b);
+    lo = pack2(a - bf16_lo(hi), b - bf16_hi(hi));
+}
+
 // RN: rank rounded up to 8, 16, 32, 64 or 128; columns past the rank are zero.
-// CTAs walk the (tile, K split) pairs with the grid's stride.
+// Clusters walk the tiles with the grid's stride; K is split over a cluster's CTAs,
+// whose sums meet in shared memory: CTA z finishes the rows of the warps w with
+// w % CTAs = z, adding the CTAs' fragments in order, scaling and splitting.
 template <int RN>
 __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter p) {
     extern __shared__ __align__(128) uint8_t stages[];
     constexpr int kChunks = kShrinkK / 8, kPass = kTileThreads / kChunks;  // rows copied at a time
+    constexpr int kRegs = RN / 2;                                          // accumulators of a lane
+    __shared__ float partial[kTileThreads / 32][kRegs][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c = tid % kChunks, i_first = tid / kChunks;  // this thread copies chunk c of every kPass-th row
     pdl_trigger();
     pdl_wait();
-    const int items = *p.tile_count * p.splits;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int2 tile = p.tiles[item / p.splits];
-        const int split = item % p.splits;
+    const int splits = p.splits, split = blockIdx.x % splits;  // a cluster's CTAs are neighbours
+    const int tile_count = *p.tile_count;
+    const int64_t k0 = split * p.split_k;
+    const int64_t k1 = k0 + p.split_k < p.k ? k0 + p.split_k : p.k;
+    const int steps = static_cast<int>((k1 - k0 + kShrinkK - 1) / kShrinkK);
+    for (int item = blockIdx.x / splits; item < tile_count; item += gridDim.x / splits) {
+        const int2 tile = p.tiles[item];
         const int key = p.keys[tile.x];
-        if (key < 0) continue;  // rows without an adapter
-        const int64_t k0 = split * p.split_k;
-        const int64_t k1 = k0 + p.split_k < p.k ? k0 + p.split_k : p.k;
-        const int steps = static_cast<int>((k1 - k0 + kShrinkK - 1) / kShrinkK);
+        if (key < 0) continue;  // rows without an adapter: the same for the whole cluster
         const bf16* rows[kTileRows / kPass];
 #pragma unroll
         for (int j = 0; j < kTileRows / kPass; ++j) {
@@ -530,14 +605,39 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
             if (++slot == kShrinkStages) slot = 0;
             if (++load_slot == kShrinkStages) load_slot = 0;
         }
+        bool mine = warp * 16 < tile.y;
+        if (splits > 1) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = warp * 16 + (lane >> 2) + 8 * h;
-            if (i >= tile.y) continue;
-            float* s = p.s + (split * p.rows + tile.x + i) * RN + 2 * (lane & 3);
+            for (int j = 0; j < kRegs; ++j) partial[warp][j][lane] = acc[j / 4][j % 4];
+            cluster_barrier();
+            mine = mine && warp % splits == split;
+            if (mine) {
+                for (int z = 0; z < splits; ++z) {
+                    float v[kRegs];  // all on their way before the first is added
 #pragma unroll
-            for (int n = 0; n < RN / 8; ++n)
-                *reinterpret_cast<float2*>(s + n * 8) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+                    for (int j = 0; j < kRegs; ++j) v[j] = __uint_as_float(load_peer(&partial[warp][j][lane], z));
+#pragma unroll
+                    for (int j = 0; j < kRegs; ++j)
+                        acc[j / 4][j % 4] = z == 0 ? v[j] : acc[j / 4][j % 4] + v[j];
+                }
+            }
+            cluster_barrier();  // everyone's sums have been read
+        }
+        if (mine) {
+            const float scale = p.scale ? p.scale[key / p.experts] : 1.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = warp * 16 + (lane >> 2) + 8 * h;
+                if (i >= tile.y) continue;
+#pragma unroll
+                for (int kk = 0; kk < rank_k<RN>() / 16; ++kk) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    split2(acc[2 * kk][2 * h] * scale, acc[2 * kk][2 * h + 1] * scale, v.x, v.z);
+                    if constexpr (RN > 8)
+                        split2(acc[2 * kk + 1][2 * h] * scale, acc[2 * kk + 1][2 * h + 1] * scale, v.y, v.w);
+                    *s_piece<RN>(p, tile.x + i, kk, lane & 3) = v;
+                }
+            }
         }
     }
     copy_wait<0>();
@@ -547,21 +647,9 @@ constexpr int kExpandThreads = 256;                   // 4 x 16 rows, 2 halves o
 constexpr int kExpandStages = 2;
 constexpr int kTileCols = 128;                        // rows of B per step: 128 columns, or 64 gate + 64 up
 constexpr int kBaseStride = kTileCols * 2 + 16;       // bytes; the pads keep ldmatrix and row stores conflict-free
-template <int RN> constexpr int rank_k() { return RN < 16 ? 16 : RN; }
 template <int RN> constexpr int b_stride() { return rank_k<RN>() * 2 + 16; }
 template <int RN> constexpr int expand_smem() {
     return kExpandStages * (kTileRows * kBaseStride + kTileCols * b_stride<RN>());
-}
-
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// Two floats as bf16 hi parts, and the rests' as a second register.
-__device__ __forceinline__ void split2(float2 v, uint32_t& hi, uint32_t& lo) {
-    hi = pack2(v.x, v.y);
-    lo = pack2(v.x - bf16_lo(hi), v.y - bf16_hi(hi));
 }
 
 // Two fp32 lanes in one register pair: one instruction for both.
@@ -601,8 +689,9 @@ __device__ __forceinline__ float2 fast_silu_times(float2 g, float2 u) {
 
 // Stretch q of the (tile, column block) pairs: the first gridDim.x stretches cover
 // half of the pairs, the next as many half of the rest, and so on, down to
-// kLeastStretch pairs.  Returns its first pair and its end.
-constexpr int kLeastStretch = 8;
+// kLeastStretch pairs (8 at least left a third of the CTAs without work in a small
+// call).  Returns its first pair and its end.
+constexpr int kLeastStretch = 2;
 struct Stretch { int64_t x, y; };
 __device__ __forceinline__ Stretch stretch_of(int64_t q, int64_t all) {
     const int64_t round = gridDim.x;
@@ -709,24 +798,17 @@ expand_tile_kernel(const Adapter p, int blocks) {
             out[j] = p.out + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.cols + out_col;
         }
 
-        // s of this warp's 16 rows as fragments: the splits' sum, scaled; zero past the rank
-        uint32_t hi[RK / 16][4], lo[RK / 16][4];
+        // s of this warp's 16 rows as fragments
+        uint32_t hi[RK / 16][4] = {}, lo[RK / 16][4] = {};
         if (key >= 0) {
-            const float scale = p.scale ? p.scale[key / p.experts] : 1.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
+                if (r0 + 8 * h < tile.y) {
 #pragma unroll
-                for (int kk = 0; kk < RK / 8; ++kk) {
-                    float2 v = make_float2(0.0f, 0.0f);
-                    if (r0 + 8 * h < tile.y && kk * 8 < RN) {
-                        const float* s = p.s + (static_cast<int64_t>(tile.x) + r0 + 8 * h) * RN + kk * 8 + 2 * (lane & 3);
-                        for (int z = 0; z < p.splits; ++z) {
-                            const float2 w = *reinterpret_cast<const float2*>(s + z * p.rows * RN);
-                            v.x += w.x, v.y += w.y;
-                        }
-                        v.x *= scale, v.y *= scale;
+                    for (int kk = 0; kk < RK / 16; ++kk) {
+                        const uint4 v = *s_piece<RN>(p, static_cast<int64_t>(tile.x) + r0 + 8 * h, kk, lane & 3);
+                        hi[kk][h] = v.x, hi[kk][2 + h] = v.y, lo[kk][h] = v.z, lo[kk][2 + h] = v.w;
                     }
-                    split2(v, hi[kk / 2][(kk & 1) * 2 + h], lo[kk / 2][(kk & 1) * 2 + h]);
                 }
         }
 
@@ -859,7 +941,7 @@ bool few_rows_form(int64_t rows, int adapters, int experts) {
 }
 
 struct Shape {
-    bool few;
+    bool few, cluster_sort;
     int splits;
     int64_t split_k, chunk_rows, table, order, keys, tiles, s, total;
     int chunks;
@@ -867,6 +949,9 @@ struct Shape {
 
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// Twice the SMs: 98 tiles of K = 2048, rank 64: 14.9 us with two CTAs a tile, 18.6 with one,
+// 19.7 with four (which no longer fit at once).
+constexpr int64_t kSpread = 2;
 Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int experts, int sms) {
     Shape f = {};
     f.few = few_rows_form(rows, adapters, experts);
@@ -876,25 +961,25 @@ Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int experts, int
         f.total = round256(rows * rank * 4 * f.splits);
         return f;
     }
-    // K is split until about three CTAs of the shrink kernel stand on every SM, in
-    // parts of at least 512 elements, and into eight at most: the expand kernel adds
-    // the parts of s every time it loads them.
+    // K is split over clusters of 1, 2 or 4 CTAs: as long as the clusters still find a place
+    // on the SMs at once, and each CTA keeps at least 512 elements.
     const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
-    int64_t splits = 3ll * sms / tiles;
-    int64_t most = (k + 511) / 512;
-    if (most > 8) most = 8;
-    splits = splits < 1 ? 1 : (splits > most ? most : splits);
+    int64_t splits = 1;
+    while (splits < 4 && tiles * splits * 2 <= kSpread * sms && k >= splits * 2 * 512) splits *= 2;
     f.split_k = ((k + splits - 1) / splits + kShrinkK - 1) / kShrinkK * kShrinkK;
-    f.splits = static_cast<int>((k + f.split_k - 1) / f.split_k);
-    f.chunk_rows = (rows + static_cast<int64_t>(kMaxChunks) * kSortThreads - 1) /
-                   (static_cast<int64_t>(kMaxChunks) * kSortThreads) * kSortThreads;
+    f.splits = static_cast<int>(splits);  // the last ones may be empty
+    // One cluster sorts up to 8192 rows: 5003 rows in 8.6 us against 10.0 in three launches
+    // (8256 rows, two rounds a CTA: 11.0 against 10.3).
+    f.cluster_sort = rows <= kClusterChunks * kClusterChunkRows;
+    const int64_t spread = (f.cluster_sort ? kClusterChunks : kMaxChunks) * static_cast<int64_t>(kSortThreads);
+    f.chunk_rows = (rows + spread - 1) / spread * kSortThreads;
     f.chunks = static_cast<int>((rows + f.chunk_rows - 1) / f.chunk_rows);
     f.table = 0;
     f.order = round256(static_cast<int64_t>(adapters + 2) * f.chunks * 4);
     f.keys = f.order + round256(rows * 4);
     f.tiles = f.keys + round256(rows * 4);
     f.s = f.tiles + round256(rows * 8 + 256);  // the count, then at most one tile per row
-    f.total = f.s + round256(rows * padded_rank(rank) * 4 * f.splits);
+    f.total = f.s + round256(rows * (padded_rank(rank) < 16 ? 16 : padded_rank(rank)) * 4);
     return f;
 }
 
@@ -919,6 +1004,27 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&configured)[64]) {
     return cudaSuccess;
 }
 
+// A dependent launch of `ctas` CTAs in clusters of `cluster`.
+template <typename... Params, typename... Args>
+cudaError_t launch_clusters(void (*kernel)(Params...), int ctas, int cluster, int threads, int smem,
+                            cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attribute[2];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    attribute[1].id = cudaLaunchAttributeClusterDimension;
+    attribute[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attribute[1].val.clusterDim.y = 1;
+    attribute[1].val.clusterDim.z = 1;
+    config.gridDim = dim3(static_cast<unsigned>(ctas));
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
+    config.stream = stream;
+    config.attrs = attribute;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+}
+
 template <int LANES, bool SWIGLU>
 cudaError_t expand_rows(const Adapter& p, cudaStream_t stream) {
     constexpr int kCols = 4 * 256 / LANES;
@@ -941,30 +1047,34 @@ cudaError_t few_rows(const Adapter& p, cudaStream_t stream) {
 
 template <int RN, bool SWIGLU>
 cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream) {
-    static bool order_ok[64] = {}, shrink_ok[64] = {}, expand_ok[64] = {};
+    static bool order_ok[2][64] = {}, shrink_ok[64] = {}, expand_ok[64] = {};
     const int buckets = p.adapters + 2;
-    const int order_smem = (32 * (buckets | 1) + 2 * buckets) * 4;
-    constexpr int kOrderMost = (32 * ((kMaxAdapters + 2) | 1) + 2 * (kMaxAdapters + 2)) * 4;
+    const int order_smem = (32 * (buckets | 1) + 3 * buckets) * 4;
+    constexpr int kOrderMost = (32 * ((kMaxAdapters + 2) | 1) + 3 * (kMaxAdapters + 2)) * 4;
     constexpr int kShrinkSmem = kShrinkStages * shrink_stage_bytes<RN>();
-    MOE_CUDA_TRY(allow_smem(order_kernel, kOrderMost, order_ok));
+    MOE_CUDA_TRY(allow_smem(f.cluster_sort ? order_kernel<true> : order_kernel<false>, kOrderMost,
+                            order_ok[f.cluster_sort]));
     MOE_CUDA_TRY(allow_smem(shrink_tile_kernel<RN>, kShrinkSmem, shrink_ok));
     MOE_CUDA_TRY(allow_smem(expand_tile_kernel<RN, SWIGLU>, expand_smem<RN>(), expand_ok));
-    MOE_CUDA_TRY(launch_dependent(count_kernel, dim3(f.chunks), dim3(kSortThreads), buckets * 4, stream, p,
-                                  f.chunk_rows));
-    MOE_CUDA_TRY(launch_dependent(order_kernel, dim3(f.chunks), dim3(kSortThreads), order_smem, stream, p,
-                                  f.chunk_rows));
     const bool none = SWIGLU || p.out != p.base;
-    MOE_CUDA_TRY(launch_dependent(tiles_kernel, dim3(static_cast<unsigned>((p.rows + 255) / 256)), dim3(256), 0,
-                                  stream, p, none));
+    if (f.cluster_sort) {
+        MOE_CUDA_TRY(launch_clusters(order_kernel<true>, f.chunks, f.chunks, kSortThreads, order_smem, stream, p,
+                                     f.chunk_rows, none));
+    } else {
+        MOE_CUDA_TRY(launch_dependent(count_kernel, dim3(f.chunks), dim3(kSortThreads), buckets * 4, stream, p,
+                                      f.chunk_rows));
+        MOE_CUDA_TRY(launch_dependent(order_kernel<false>, dim3(f.chunks), dim3(kSortThreads), order_smem, stream,
+                                      p, f.chunk_rows, none));
+        MOE_CUDA_TRY(launch_dependent(tiles_kernel, dim3(static_cast<unsigned>((p.rows + 255) / 256)), dim3(256),
+                                      0, stream, p, none));
+    }
     const auto resident = [&](int smem_bytes, int threads_most) {
         const int fit = 227 * 1024 / (smem_bytes + 1024);
         return static_cast<int64_t>(sms) * (fit < threads_most ? fit : threads_most);
     };
-    const int64_t shrink_most = resident(kShrinkSmem, 4);
-    const int64_t shrink_items = p.rows * f.splits;
-    MOE_CUDA_TRY(launch_dependent(shrink_tile_kernel<RN>,
-                                  dim3(static_cast<unsigned>(shrink_items < shrink_most ? shrink_items : shrink_most)),
-                                  dim3(kTileThreads), kShrinkSmem, stream, p));
+    const int64_t most = resident(kShrinkSmem + RN * 256, 4) / f.splits;
+    MOE_CUDA_TRY(launch_clusters(shrink_tile_kernel<RN>, static_cast<int>((p.rows < most ? p.rows : most) * f.splits),
+                                 f.splits, kTileThreads, kShrinkSmem, stream, p));
     const int out_cols = SWIGLU ? kTileCols / 2 : kTileCols;
     const int blocks = static_cast<int>((p.cols + out_cols - 1) / out_cols);
     const int64_t expand_most = resident(expand_smem<RN>(), RN <= 32 ? 3 : (RN <= 64 ? 2 : 1));

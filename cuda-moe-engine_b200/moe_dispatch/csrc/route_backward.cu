@@ -13,9 +13,9 @@
 // (an fp32 result) takes all three parts of d; dx (a bf16 result) takes
 // d_mid W_hi + d_hi W_hi + d_hi W_lo, which leaves out terms of 2^-16 |d W|.
 //
-//   split_gradient_kernel  a warp per token writes d's parts, [T, 4 E8] bf16 with
-//                          columns lo | mid | hi | hi, E8 = E rounded up to 8
-//   split_weight_kernel    W^T parts, [H, 3 E8] bf16 with columns hi | hi | lo
+//   split_kernel           d's parts, [T, 4 E8] bf16 with columns lo | mid | hi | hi
+//                          (E8: E rounded up to 8), a warp per token; and W^T's parts,
+//                          [H, 3 E8] bf16 with columns hi | hi | lo
 //   dx                     the grouped GEMM with one group: columns mid | hi | hi
 //                          of the first against the second, K = 3 E8
 //   router_dw_kernel, router_dw_pair_kernel  dW: tcgen05 over tokens as K, both
@@ -51,19 +51,17 @@ __device__ __forceinline__ uint32_t bf16_part(float& rest) {
     return __bfloat16_as_ushort(h);
 }
 
-// A warp per token; lane holds experts 2 (lane + 32 i) and the next one.
+// d's parts of every token: a warp per token; lane holds experts 2 (lane + 32 i) and
+// the next one.
 template <int PAIRS>
-__global__ void __launch_bounds__(256)
-split_gradient_kernel(const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
-                      const float* __restrict__ weights, const float* __restrict__ grad_weights,
-                      uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded,
-                      int topk) {
+__device__ void split_gradient(const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
+                               const float* __restrict__ weights, const float* __restrict__ grad_weights,
+                               uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded, int topk,
+                               int block, int blocks) {
     const int lane = threadIdx.x & 31;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    pdl_trigger();
-    pdl_wait();
+    const int64_t warps = static_cast<int64_t>(blocks) * 8;
     const int half = padded / 2;  // 32-bit words of one part's columns
-    for (int64_t t = blockIdx.x * 8ll + (threadIdx.x >> 5); t < tokens; t += warps) {
+    for (int64_t t = block * 8ll + (threadIdx.x >> 5); t < tokens; t += warps) {
         float d[PAIRS][2];
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
@@ -109,22 +107,11 @@ split_gradient_kernel(const float* __restrict__ grad_logits, const int32_t* __re
     }
 }
 
-// W [E, H] fp32 -> [H, 3 E8] bf16: 32 x 32 tiles through shared memory.  Thread
-// 0 of the first CTA also writes the grouped GEMM's offsets {0, T}.
-__global__ void __launch_bounds__(256)
-split_weight_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ out,
-                    int32_t* __restrict__ offsets, int tokens, int experts, int padded,
-                    int64_t hidden) {
+// W [E, H] fp32 -> [H, 3 E8] bf16: one 32 x 32 tile through shared memory.
+__device__ void split_weight(const float* __restrict__ weight, __nv_bfloat16* __restrict__ out, int experts,
+                             int padded, int64_t hidden, int64_t h0, int e0) {
     __shared__ float tile[32][33];
-    pdl_trigger();
-    pdl_wait();
-    const int64_t h0 = blockIdx.x * 32ll;
-    const int e0 = blockIdx.y * 32;
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
-        offsets[0] = 0;
-        offsets[1] = tokens;
-    }
     for (int i = y; i < 32; i += 8)
         tile[i][x] = e0 + i < experts && h0 + x < hidden ? weight[(e0 + i) * hidden + h0 + x] : 0.0f;
     __syncthreads();
@@ -137,6 +124,30 @@ split_weight_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict_
         row[0] = hi;
         row[padded] = hi;
         row[2 * padded] = __float2bfloat16_rn(v - __bfloat162float(hi));
+    }
+}
+
+// Both splits in one launch: the first CTAs take a tile of W each (none without dx),
+// the others d.  Thread 0 of the first also writes the grouped GEMM's offsets {0, T}.
+template <int PAIRS>
+__global__ void __launch_bounds__(256)
+split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weight_parts,
+             int32_t* __restrict__ offsets, int64_t hidden, int tiles_h, int tiles,
+             const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
+             const float* __restrict__ weights, const float* __restrict__ grad_weights,
+             uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded, int topk) {
+    pdl_trigger();
+    pdl_wait();
+    const int block = blockIdx.x;
+    if (block < tiles) {
+        if (block == 0 && threadIdx.x == 0) {
+            offsets[0] = 0;
+            offsets[1] = static_cast<int32_t>(tokens);
+        }
+        split_weight(weight, weight_parts, experts, padded, hidden, block % tiles_h * 32ll, block / tiles_h * 32);
+    } else {
+        split_gradient<PAIRS>(grad_logits, ids, weights, grad_weights, parts, tokens, experts, padded, topk,
+                              block - tiles, gridDim.x - tiles);
     }
 }
 
@@ -956,20 +967,17 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
                            static_cast<__nv_bfloat16*>(grad_x), grad_weight, reinterpret_cast<float*>(base + l.sums),
                            tokens, hidden, experts, topk, sms, stream);
 
+    auto* wt = reinterpret_cast<__nv_bfloat16*>(base + l.weight);
+    auto* offsets = reinterpret_cast<int32_t*>(base + l.offsets);
+    const int tiles_h = static_cast<int>((hidden + 31) / 32);
+    const int weight_tiles = grad_x ? tiles_h * ((e8 + 31) / 32) : 0;
     const int64_t blocks = (tokens + 7) / 8;
-    const unsigned grid = static_cast<unsigned>(blocks < 8ll * sms ? blocks : 8ll * sms);
-    auto split = experts <= 64 ? split_gradient_kernel<1>
-                               : (experts <= 128 ? split_gradient_kernel<2> : split_gradient_kernel<4>);
-    MOE_CUDA_TRY(launch_dependent(split, dim3(grid), dim3(256), 0, stream, grad_logits, ids, weights,
-                                  grad_weights, reinterpret_cast<uint32_t*>(parts), tokens, experts, e8,
-                                  topk));
+    const int64_t grid = weight_tiles + (blocks < 8ll * sms ? blocks : 8ll * sms);
+    auto split = experts <= 64 ? split_kernel<1> : (experts <= 128 ? split_kernel<2> : split_kernel<4>);
+    MOE_CUDA_TRY(launch_dependent(split, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, weight, wt, offsets,
+                                  hidden, tiles_h, weight_tiles, grad_logits, ids, weights, grad_weights,
+                                  reinterpret_cast<uint32_t*>(parts), tokens, experts, e8, topk));
     if (grad_x) {
-        auto* wt = reinterpret_cast<__nv_bfloat16*>(base + l.weight);
-        auto* offsets = reinterpret_cast<int32_t*>(base + l.offsets);
-        MOE_CUDA_TRY(launch_dependent(split_weight_kernel,
-                                      dim3(static_cast<unsigned>((hidden + 31) / 32), (e8 + 31) / 32),
-                                      dim3(256), 0, stream, weight, wt, offsets,
-                                      static_cast<int>(tokens), experts, e8, hidden));
         MOE_CUDA_TRY(launch_grouped_gemm(parts + e8, wt, offsets, grad_x, tokens, hidden, 3 * e8, 1,
                                          false, stream, error, nullptr, nullptr, nullptr, 4 * e8));
     }

@@ -103,7 +103,8 @@ int moe_balance_loss_backward(const void* logits, int32_t dtype, const float* bi
  * on the tensor cores with d and the weight split into bf16 parts: d enters
  * grad_router_weight to 2^-24, and the products of grad_x are good to 2^-16 of
  * their size.
- * Gradients that are not finite give results that are not finite.  Fixed
+ * Gradients that are not finite (or above 3.38e38) give results that are not
+ * finite.  Fixed
  * summation order.  hidden % 8 == 0; x, router_weight and their gradients 16-byte
  * aligned.
  * scratch: 256-byte aligned, not initialised, its size for the current device;
@@ -205,8 +206,8 @@ int moe_grouped_gemm(const void* a, const void* weight, const int32_t* offsets, 
 /* out[r] = bf16(base[r] + scale[p] * (x[r] . a[p,e]^T) . b[p,e]^T) for every
  * row r of expert e's span [offsets[e], offsets[e+1]), p = row_adapters[r];
  * rows whose p is outside [0, adapters) get base[r].  Rows at or past
- * offsets[experts] are neither read nor written.  offsets NULL: one expert with
- * every row.  base, out [rows, n_cols] (out may be base itself, and must not
+ * offsets[experts] are neither read nor written.  offsets start at 0 and ascend;
+ * NULL: one expert with every row.  base, out [rows, n_cols] (out may be base itself, and must not
  * overlap any operand otherwise); x [rows, k_dim]; a [adapters, experts, rank,
  * k_dim]; b [adapters, experts, n_cols, rank]; scale [adapters] fp32 or NULL (1).
  * x . a^T is summed in fp32 and used to 2^-16 of its value or better; one

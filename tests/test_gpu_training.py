@@ -208,7 +208,8 @@ ROUTER_SHAPES = [
     (1, 8, 1, 1), (1, 64, 8, 2), (3, 72, 5, 2), (31, 136, 80, 8), (33, 128, 81, 3), (128, 512, 8, 2),
     (257, 520, 96, 6), (500, 2056, 200, 8), (1000, 1032, 256, 8), (5000, 256, 64, 6), (9000, 136, 16, 32),
     (4097, 264, 33, 1), (2111, 128, 128, 4), (64, 7168, 256, 8), (700, 4104, 8, 3), (3001, 1032, 9, 9),
-    (70000, 64, 4, 2), (1, 2056, 16, 16), (1000, 520, 17, 17), (129, 264, 32, 20)]
+    (70000, 64, 4, 2), (1, 2056, 16, 16), (1000, 520, 17, 17), (129, 264, 32, 20),
+    (40, 8, 20, 2), (40, 8, 100, 2), (70, 24, 40, 3), (2, 16, 256, 1), (35, 8, 8, 2)]
 
 
 @pytest.mark.parametrize("shape", ROUTER_SHAPES, ids=str)
