@@ -49,9 +49,8 @@ class MoEAdapters:
 def _check_pair(name, a, b, experts, k_dim, n_cols):
     if a.ndim != 4 or b.ndim != 4 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         raise ValueError(f"{name}: expected bf16 a[P,E,r,K] and b[P,E,N,r]")
-    adapters, _, rank = a.shape[:3]
-    if tuple(a.shape) != (adapters, experts, rank, k_dim) or tuple(b.shape) != (
-            adapters, experts, n_cols, rank):
+    adapters, a_experts, rank, a_dim = a.shape
+    if a_experts != experts or a_dim != k_dim or b.shape != (adapters, experts, n_cols, rank):
         raise ValueError(f"{name}: a and b do not match the projection")
     if not 1 <= adapters <= MAX_ADAPTERS:
         raise ValueError(f"{name}: adapters must be 1..{MAX_ADAPTERS}")
@@ -117,15 +116,16 @@ def _apply(base, x, a, b, row_adapters, offsets, scale, out, swiglu):
     _check_pair("adapter", a, b, experts, k_dim, n_cols)
     _check_scale(scale, a.shape[0])
     shape = (rows, n_cols // halves)
-    if out is not None and (tuple(out.shape) != shape or out.dtype != torch.bfloat16
-                            or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous bf16 tensor [{shape[0]},{shape[1]}]")
     device, grad = x.device, torch.is_grad_enabled()
     if out is not None:
-        low = out.data_ptr()
-        high = low + out.nbytes
+        if out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous bf16 tensor [{shape[0]},{shape[1]}]")
         if out.device != device:
             raise ValueError("all tensors must be on the same device")
+        if grad and out.requires_grad:
+            raise ValueError("CUDA operators are forward-only; detach inputs or use inference_mode")
+        low = out.data_ptr()
+        high = low + out.nbytes
     for t in (base, x, a, b, row_adapters, offsets, scale):
         if t is None:
             continue

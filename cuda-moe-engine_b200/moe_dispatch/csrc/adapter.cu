@@ -30,9 +30,9 @@
 // moved, far below what the tensor cores need to be the bound.  A tile holds one
 // adapter's rows only, so what is not finite in one adapter or row stays there.
 //
-// Nothing depends on where a row lands in a tile: its products are its own, so
-// results do not change with the batch around it, except between the two forms
-// (their summation orders differ).
+// Nothing depends on where a row lands in a tile: its products are its own, so for a
+// given number of rows (which decides the form and how K is split) a row's result does
+// not change with the rows around it.
 #include "common.cuh"
 #include "launch.h"
 
@@ -528,7 +528,6 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
     extern __shared__ __align__(128) uint8_t stages[];
     constexpr int kChunks = kShrinkK / 8, kPass = kTileThreads / kChunks;  // rows copied at a time
     constexpr int kRegs = RN / 2;                                          // accumulators of a lane
-    __shared__ float partial[kTileThreads / 32][kRegs][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c = tid % kChunks, i_first = tid / kChunks;  // this thread copies chunk c of every kPass-th row
     pdl_trigger();
@@ -607,15 +606,17 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
         }
         bool mine = warp * 16 < tile.y;
         if (splits > 1) {
+            float* partial = reinterpret_cast<float*>(stages) + warp * kRegs * 32 + lane;  // [warp][register][lane]
+            __syncthreads();  // the stages have been read
 #pragma unroll
-            for (int j = 0; j < kRegs; ++j) partial[warp][j][lane] = acc[j / 4][j % 4];
+            for (int j = 0; j < kRegs; ++j) partial[j * 32] = acc[j / 4][j % 4];
             cluster_barrier();
             mine = mine && warp % splits == split;
             if (mine) {
                 for (int z = 0; z < splits; ++z) {
                     float v[kRegs];  // all on their way before the first is added
 #pragma unroll
-                    for (int j = 0; j < kRegs; ++j) v[j] = __uint_as_float(load_peer(&partial[warp][j][lane], z));
+                    for (int j = 0; j < kRegs; ++j) v[j] = __uint_as_float(load_peer(partial + j * 32, z));
 #pragma unroll
                     for (int j = 0; j < kRegs; ++j)
                         acc[j / 4][j % 4] = z == 0 ? v[j] : acc[j / 4][j % 4] + v[j];
@@ -730,6 +731,10 @@ expand_tile_kernel(const Adapter p, int blocks) {
     const int c = (tid & 15) * 8, i_first = tid >> 4;
     const int c_col = SWIGLU ? c & 63 : c;  // its column inside the block
     const int b_q = tid % kChunks, b_n = tid / kChunks;
+    // this lane's first row of B for ldmatrix, and its first pair of base, inside a stage
+    const uint32_t b_lane = kTileRows * kBaseStride +
+                            (half * (kOut / 2) + (lane & 7) + ((lane >> 4) << 3)) * b_stride<RN>() + ((lane >> 3) & 1) * 16;
+    const int base_lane = (warp * 16 + (lane >> 2)) * kBaseStride + half * kOut + (lane & 3) * 4;
     const int r0 = warp * 16 + (lane >> 2);
     constexpr int kPieces = kOut / 16, kPer = 32 / kPieces;  // out: 16-byte pieces of a half row; rows at a time
     const int out_row = warp * 16 + lane / kPieces, out_col = half * (kOut / 2) + (lane % kPieces) * 8;
@@ -824,18 +829,17 @@ expand_tile_kernel(const Adapter p, int blocks) {
                 if (key >= 0) {
                     // 16 columns at a time (with SwiGLU 16 gate and the matching 16 up columns), so
                     // few accumulators live at once
-                    const uint32_t bs = smem_addr(base_s) + kTileRows * kBaseStride +
-                                        ((lane & 7) + ((lane >> 4) << 3)) * b_stride<RN>() + ((lane >> 3) & 1) * 16;
+                    const uint32_t bs = smem_addr(base_s) + b_lane;
+                    uint8_t* const mine = base_s + base_lane;
 #pragma unroll
                     for (int f = 0; f < kOut / 2; f += 16) {
-                        const int n0 = half * (kOut / 2) + f;
                         float acc[kHalves][2][4];
 #pragma unroll
                         for (int g = 0; g < kHalves; ++g)
 #pragma unroll
                             for (int kk = 0; kk < RK / 16; ++kk) {
                                 uint32_t bf[4];
-                                ldmatrix4(bs + (n0 + g * 64) * b_stride<RN>() + kk * 32, bf);
+                                ldmatrix4(bs + (f + g * 64) * b_stride<RN>() + kk * 32, bf);
                                 if (kk == 0) {
                                     mma16816_first(acc[g][0], lo[0], bf[0], bf[1]);
                                     mma16816_first(acc[g][1], lo[0], bf[2], bf[3]);
@@ -851,8 +855,7 @@ expand_tile_kernel(const Adapter p, int blocks) {
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
-                                uint32_t* at = reinterpret_cast<uint32_t*>(
-                                    base_s + (r0 + 8 * h) * kBaseStride + (n0 + q * 8) * 2 + (lane & 3) * 4);
+                                uint32_t* at = reinterpret_cast<uint32_t*>(mine + h * 8 * kBaseStride + (f + q * 8) * 2);
                                 const uint32_t v = *at;
                                 float2 y = add2(make_float2(bf16_lo(v), bf16_hi(v)),
                                                 make_float2(acc[0][q][2 * h], acc[0][q][2 * h + 1]));
@@ -864,13 +867,14 @@ expand_tile_kernel(const Adapter p, int blocks) {
                                 *at = pack2(y.x, y.y);
                             }
                     }
-                } else if constexpr (SWIGLU) {  // without an adapter: the bits of swiglu_kernel
+                } else if constexpr (SWIGLU) {
+                    // without an adapter: the bits of swiglu_kernel; two rows, a pair of columns a lane
+                    uint8_t* pair = base_s + (warp * 16 + (lane >> 4)) * kBaseStride + half * kOut + (lane & 15) * 4;
 #pragma unroll 4
-                    for (int i = 0; i < 16; ++i) {
-                        uint8_t* row = base_s + (warp * 16 + i) * kBaseStride + half * 64;
-                        const float g = __bfloat162float(reinterpret_cast<const bf16*>(row)[lane]);
-                        const float u = __bfloat162float(reinterpret_cast<const bf16*>(row + 128)[lane]);
-                        reinterpret_cast<bf16*>(row)[lane] = __float2bfloat16_rn(silu_times(g, u));
+                    for (int i = 0; i < 16; i += 2, pair += 2 * kBaseStride) {
+                        uint32_t* at = reinterpret_cast<uint32_t*>(pair);
+                        const uint32_t g = *at, u = at[32];
+                        *at = pack2(silu_times(bf16_lo(g), bf16_lo(u)), silu_times(bf16_hi(g), bf16_hi(u)));
                     }
                 }
                 __syncwarp();
@@ -1072,7 +1076,7 @@ cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream
         const int fit = 227 * 1024 / (smem_bytes + 1024);
         return static_cast<int64_t>(sms) * (fit < threads_most ? fit : threads_most);
     };
-    const int64_t most = resident(kShrinkSmem + RN * 256, 4) / f.splits;
+    const int64_t most = resident(kShrinkSmem, 4) / f.splits;
     MOE_CUDA_TRY(launch_clusters(shrink_tile_kernel<RN>, static_cast<int>((p.rows < most ? p.rows : most) * f.splits),
                                  f.splits, kTileThreads, kShrinkSmem, stream, p));
     const int out_cols = SWIGLU ? kTileCols / 2 : kTileCols;
