@@ -1008,10 +1008,13 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&configured)[64]) {
     return cudaSuccess;
 }
 
-// A dependent launch of `ctas` CTAs in clusters of `cluster`.
+// A dependent launch of `ctas` CTAs in clusters of `cluster`.  With `fit`, at most as
+// many clusters as the device holds at once (looked up once, into *fit): a walk with
+// the grid's stride would else leave shares to clusters that start when the others
+// are done, which doubled the shrink kernel's time at 443 small tiles.
 template <typename... Params, typename... Args>
 cudaError_t launch_clusters(void (*kernel)(Params...), int ctas, int cluster, int threads, int smem,
-                            cudaStream_t stream, Args&&... args) {
+                            cudaStream_t stream, int* fit, Args&&... args) {
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1026,6 +1029,10 @@ cudaError_t launch_clusters(void (*kernel)(Params...), int ctas, int cluster, in
     config.stream = stream;
     config.attrs = attribute;
     config.numAttrs = 2;
+    if (fit) {
+        if (*fit == 0) MOE_CUDA_TRY(cudaOccupancyMaxActiveClusters(fit, kernel, &config));
+        if (*fit > 0 && ctas > *fit * cluster) config.gridDim = dim3(static_cast<unsigned>(*fit * cluster));
+    }
     return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
 }
 
@@ -1062,8 +1069,8 @@ cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream
     MOE_CUDA_TRY(allow_smem(expand_tile_kernel<RN, SWIGLU>, expand_smem<RN>(), expand_ok));
     const bool none = SWIGLU || p.out != p.base;
     if (f.cluster_sort) {
-        MOE_CUDA_TRY(launch_clusters(order_kernel<true>, f.chunks, f.chunks, kSortThreads, order_smem, stream, p,
-                                     f.chunk_rows, none));
+        MOE_CUDA_TRY(launch_clusters(order_kernel<true>, f.chunks, f.chunks, kSortThreads, order_smem, stream,
+                                     nullptr, p, f.chunk_rows, none));
     } else {
         MOE_CUDA_TRY(launch_dependent(count_kernel, dim3(f.chunks), dim3(kSortThreads), buckets * 4, stream, p,
                                       f.chunk_rows));
@@ -1076,9 +1083,12 @@ cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream
         const int fit = 227 * 1024 / (smem_bytes + 1024);
         return static_cast<int64_t>(sms) * (fit < threads_most ? fit : threads_most);
     };
+    static int shrink_fit[5][64] = {};  // by splits
+    int device = 0;
+    MOE_CUDA_TRY(cudaGetDevice(&device));
     const int64_t most = resident(kShrinkSmem, 4) / f.splits;
     MOE_CUDA_TRY(launch_clusters(shrink_tile_kernel<RN>, static_cast<int>((p.rows < most ? p.rows : most) * f.splits),
-                                 f.splits, kTileThreads, kShrinkSmem, stream, p));
+                                 f.splits, kTileThreads, kShrinkSmem, stream, &shrink_fit[f.splits][device & 63], p));
     const int out_cols = SWIGLU ? kTileCols / 2 : kTileCols;
     const int blocks = static_cast<int>((p.cols + out_cols - 1) / out_cols);
     const int64_t expand_most = resident(expand_smem<RN>(), RN <= 32 ? 3 : (RN <= 64 ? 2 : 1));
