@@ -21,7 +21,7 @@
 //       come expert by expert, so the sorted rows are grouped by (p, e).
 //   tiles_kernel        cuts each group into tiles of up to 64 rows.  (Tiles over 64
 //       consecutive sorted rows, whatever groups they touch, were measured first: a
-//       few tiles with 26 small groups held everything up, 1080 us against 420 at
+//       few tiles with 26 small groups held everything up, 1080 us against 583 at
 //       16384 tokens, 64 experts, top-6, 32 adapters of rank 32.)
 //   shrink_tile_kernel  a tile's rows x rank, K in 128-wide cp.async stages
 //   expand_tile_kernel  a tile's rows x column blocks of 128; s enters the tensor
@@ -129,7 +129,7 @@ constexpr int kRowsSplitK = 2048;  // K elements per CTA
 
 // CTA: one row, eight rows of its A (a warp each), 2048 elements of K.  Everything is
 // copied to shared memory at once, so that all of it is in flight together; loads
-// into registers were used one by one (16.8 us against 11 at 134 rows of 14336).
+// into registers were used one by one (16.8 us against 12.3 at 134 rows of 14336).
 __global__ void __launch_bounds__(256) shrink_rows_kernel(const Adapter p) {
     __shared__ uint4 xs[kRowsSplitK / 8];
     __shared__ uint4 as[8][kRowsSplitK / 8];
@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const Adapter p, in
     int32_t* local = total + buckets;           // [buckets] this chunk's counts (cluster form)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int chunks = gridDim.x, me = blockIdx.x;
-    pdl_trigger();
+    // no early trigger: CTAs of the next kernel that start beside this one's end up crowded on
+    // the other SMs (1032 rows over 443 pairs: the call 179 us with it, 140 without)
     for (int i = tid; i < 32 * stride; i += kSortThreads) hist[i] = 0;
     if constexpr (kCluster)
         for (int i = tid; i < buckets; i += kSortThreads) local[i] = 0;
@@ -530,7 +531,6 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
     constexpr int kRegs = RN / 2;                                          // accumulators of a lane
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c = tid % kChunks, i_first = tid / kChunks;  // this thread copies chunk c of every kPass-th row
-    pdl_trigger();
     pdl_wait();
     const int splits = p.splits, split = blockIdx.x % splits;  // a cluster's CTAs are neighbours
     const int tile_count = *p.tile_count;
@@ -676,7 +676,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // of the value, against 2^-8 of the rounding to bf16.  Where 2^(-g log2 e) is
 // infinite the reciprocal is 0.  (With expf, a division and single lanes the
 // SwiGLU form of the expand kernel issued 36 instructions an element and was
-// bound by them: 309 us at 4096 tokens, 8 experts, top-2, against 195 with this.)
+// bound by them: 309 us at 4096 tokens, 8 experts, top-2, against 182 with this.)
 __device__ __forceinline__ float2 fast_silu_times(float2 g, float2 u) {
     const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
     float2 e, r;
@@ -932,9 +932,9 @@ int padded_rank(int rank) {
 }
 
 // Which form.  Measured in graphs (us, few-rows form / tiles), 8 experts, rank 16, down
-// projection 14336 -> 4096: one adapter, 128 rows 13 / 24, 256 rows 22 / 26, 512 rows
-// 41 / 31, 1024 rows 77 / 37; 64 adapters, a row's own each, 512 rows 46 / 129, 1024 rows
-// 83 / 159, 2048 rows 156 / 184.  (Rank 8 to 128 and 4096 -> 28672 cross over near the
+// projection 14336 -> 4096: one adapter, 128 rows 13 / 25, 256 rows 22 / 28, 512 rows
+// 41 / 31, 1024 rows 77 / 35; 64 adapters, a row's own each, 512 rows 47 / 125, 1024 rows
+// 83 / 140, 2048 rows 156 / 160.  (Rank 8 to 128 and 4096 -> 28672 cross over near the
 // same places.)  Where the rows are no more than twice the pairs that they may fall
 // on, tiles would hold few rows each.
 constexpr int64_t kFewRows = 256;

@@ -364,7 +364,7 @@ cudaError_t forward(const BalanceArgs& a) {
     MOE_CUDA_TRY(launch_dependent(balance_forward_kernel<DT, G, VPL, VEC>, dim3(parts), dim3(kThreads), 0,
                                   a.stream, static_cast<const T*>(a.logits), a.bias, a.ids, a.mask,
                                   sums, part_counts, a.tokens, a.experts, a.topk, per_cta));
-    // One CTA reads about 100 rows of 256 experts in 6 us, eight in 2 (each a slice of the parts).
+    // 148 rows of 256 experts took one CTA 8.8 us; eight take 6.8 for 296.
     const unsigned cluster = static_cast<int64_t>(parts) * a.experts > 2048 ? 8 : 1;
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute attribute[2];
