@@ -154,7 +154,7 @@ split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weigh
 // ----------------------------------------------------------------------- dW
 
 constexpr int kTileH = 128;   // rows of dW^T per CTA (M)
-constexpr int kTileT = 32;    // tokens per pipeline stage (K)
+constexpr int kTileT = 64;    // tokens per pipeline stage (K)
 constexpr int kBlock = kTileT * 128;  // bytes of 64 columns x kTileT tokens
 constexpr int kMaxStages = 8;
 constexpr int kDwThreads = 192;  // producer, issuer, four epilogue warps
@@ -347,7 +347,7 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 // one before into fp32 registers, 128 columns of one row per thread.
 constexpr int kPairThreads = 320;  // producer, issuer, eight epilogue warps
 constexpr int kChunk = 256;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 3;
 constexpr int kChunkSteps = kChunk / kTileT;
 
 __device__ __forceinline__ bool wait_bounded_cluster(uint64_t* bar, uint32_t parity,
