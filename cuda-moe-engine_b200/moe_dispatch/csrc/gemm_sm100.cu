@@ -1499,7 +1499,7 @@ cudaError_t launch_grouped_gemm(const void* a, const void* b, const int32_t* off
                                 int64_t rows, int64_t n_out, int64_t k_dim, int experts,
                                 bool swiglu, cudaStream_t stream, const char** error,
                                 const float* a_scale, const float* b_scale,
-                                const GemmArrival* arrival, int64_t a_stride) {
+                                const GemmArrival* arrival) {
     const bool fp8 = a_scale != nullptr;
     *error = nullptr;
     if (rows == 0 || experts == 0) return cudaSuccess;
@@ -1514,8 +1514,7 @@ cudaError_t launch_grouped_gemm(const void* a, const void* b, const int32_t* off
     if (info.sms == 0) MOE_CUDA_TRY(cudaDeviceGetAttribute(&info.sms, cudaDevAttrMultiProcessorCount, device));
     const int64_t b_rows = swiglu ? 2 * n_out : n_out;
     CUtensorMap map_a, map_b;
-    if (!make_tensor_map(&map_a, a, static_cast<uint64_t>(rows), static_cast<uint64_t>(k_dim), fp8,
-                         kBoxRows, static_cast<uint64_t>(a_stride)) ||
+    if (!make_tensor_map(&map_a, a, static_cast<uint64_t>(rows), static_cast<uint64_t>(k_dim), fp8) ||
         !make_tensor_map(&map_b, b, static_cast<uint64_t>(b_rows * experts), static_cast<uint64_t>(k_dim), fp8)) {
         *error = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
         return cudaErrorInvalidValue;

@@ -13,11 +13,10 @@
 // (an fp32 result) takes all three parts of d; dx (a bf16 result) takes
 // d_mid W_hi + d_hi W_hi + d_hi W_lo, which leaves out terms of 2^-16 |d W|.
 //
-//   split_kernel           d's parts, [T, 4 E8] bf16 with columns lo | mid | hi | hi
-//                          (E8: E rounded up to 8), a warp per token; and W^T's parts,
-//                          [H, 3 E8] bf16 with columns hi | hi | lo
-//   dx                     the grouped GEMM with one group: columns mid | hi | hi
-//                          of the first against the second, K = 3 E8
+//   split_kernel           d's parts, [T, 3 E8] bf16 with columns lo | mid | hi (E8: E
+//                          rounded up to 8), a warp per token; and W^T's parts,
+//                          [H, 2 E8] bf16 with columns hi | lo
+//   router_dx_kernel       dx: tcgen05 on CTA pairs, K = E, three MMAs per 16 experts
 //   router_dw_kernel, router_dw_pair_kernel  dW: tcgen05 over tokens as K, both
 //                          operands MN-major; up to 80 experts, and above
 //   add_parts_kernel       adds the token ranges' partial sums in order
@@ -33,6 +32,8 @@
 
 namespace moe {
 
+// gemm_sm100.cu: [rows, cols] bf16 whose rows lie `stride` elements apart (0: cols), in
+// boxes of box_rows x 64 columns, 128-byte swizzle.
 bool encode_bf16_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                             uint64_t stride, uint32_t box_rows);
 
@@ -91,7 +92,7 @@ __device__ void split_gradient(const float* __restrict__ grad_logits, const int3
                     else d[i][0] += v;
                 }
         }
-        uint32_t* row = parts + t * 4 * half;
+        uint32_t* row = parts + t * 3 * half;
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
             const int at = lane + 32 * i;
@@ -102,12 +103,11 @@ __device__ void split_gradient(const float* __restrict__ grad_logits, const int3
             row[at] = lo;
             row[half + at] = mid;
             row[2 * half + at] = hi;
-            row[3 * half + at] = hi;
         }
     }
 }
 
-// W [E, H] fp32 -> [H, 3 E8] bf16: one 32 x 32 tile through shared memory.
+// W [E, H] fp32 -> [H, 2 E8] bf16: one 32 x 32 tile through shared memory.
 __device__ void split_weight(const float* __restrict__ weight, __nv_bfloat16* __restrict__ out, int experts,
                              int padded, int64_t hidden, int64_t h0, int e0) {
     __shared__ float tile[32][33];
@@ -120,19 +120,17 @@ __device__ void split_weight(const float* __restrict__ weight, __nv_bfloat16* __
         if (h0 + i >= hidden) break;
         float v = tile[x][i];
         const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-        __nv_bfloat16* row = out + (h0 + i) * 3 * padded + e0 + x;
+        __nv_bfloat16* row = out + (h0 + i) * 2 * padded + e0 + x;
         row[0] = hi;
-        row[padded] = hi;
-        row[2 * padded] = __float2bfloat16_rn(v - __bfloat162float(hi));
+        row[padded] = __float2bfloat16_rn(v - __bfloat162float(hi));
     }
 }
 
 // Both splits in one launch: the first CTAs take a tile of W each (none without dx),
-// the others d.  Thread 0 of the first also writes the grouped GEMM's offsets {0, T}.
+// the others d.
 template <int PAIRS>
 __global__ void __launch_bounds__(256)
-split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weight_parts,
-             int32_t* __restrict__ offsets, int64_t hidden, int tiles_h, int tiles,
+split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weight_parts, int64_t hidden, int tiles_h, int tiles,
              const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
              const float* __restrict__ weights, const float* __restrict__ grad_weights,
              uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded, int topk) {
@@ -140,10 +138,6 @@ split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weigh
     pdl_wait();
     const int block = blockIdx.x;
     if (block < tiles) {
-        if (block == 0 && threadIdx.x == 0) {
-            offsets[0] = 0;
-            offsets[1] = static_cast<int32_t>(tokens);
-        }
         split_weight(weight, weight_parts, experts, padded, hidden, block % tiles_h * 32ll, block / tiles_h * 32);
     } else {
         split_gradient<PAIRS>(grad_logits, ids, weights, grad_weights, parts, tokens, experts, padded, topk,
@@ -338,12 +332,12 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 // dW^T tile [256 h, E] of one range of tokens on a CTA pair (cta_group::2), more
 // than 80 experts: each CTA loads its 128 columns of x and its half of every part's
 // E columns, the even CTA issues M = 256, N up to 256, one MMA per part and 16
-// tokens.  (On one CTA with M = 128 each SM is fed 112 KB per 64 tokens, which the
-// L2 cache delivers no faster than 49 bytes a cycle: 451 us at 32768 tokens, 256
-// experts, hidden 7168.)
+// tokens.  (One CTA with M = 128 needs 112 KB per 64 tokens and SM instead of 64: 451 us
+// at 32768 tokens, 256 experts, hidden 7168 against 283 for the pair, both with stages of
+// 32 tokens.)
 //
 // The tensor cores cut the sum of 16 products and the accumulator off below its last
-// bit, always downward, so long sums drift: with 500 MMAs into one accumulator dW was
+// bit, so long sums drift: with 500 MMAs into one accumulator dW was
 // 6.7e-6 of its norm off at this size, where plain fp32 products are 5.8e-7 off.  Here
 // an accumulator takes kChunk tokens (48 MMAs); meanwhile the epilogue warps add the
 // one before into fp32 registers, 128 columns of one row per thread.
@@ -518,6 +512,197 @@ router_dw_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             for (int j = 0; j < 128; ++j)
                 if (j < mine) out[j * p.hidden] = sum[j];
         }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while its peer may still touch its memory
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ----------------------------------------------------------------------- dx
+
+// dx tile [256 tokens, 256 h] on a CTA pair: each CTA loads mid and hi of its 128
+// tokens' d and hi and lo of its 128 rows of W^T, 64 experts at a time (a tensor map per
+// part, so that columns past E8 are zeros and not the next part's), the even CTA issues mid x hi, hi x hi and hi x lo, M = 256, N = 256.
+// The epilogue warps turn 32 tokens x 64 columns at a time into bf16 in shared memory
+// and store them as a tile while the next accumulator fills.  (221 us at 32768 tokens,
+// 256 experts, hidden 7168, 1.63 PFLOP/s of bf16 products, and 25 at 16384 tokens, 64
+// experts, hidden 2048.  The grouped GEMM over K = 3 E with d_hi and W_hi stored twice
+// took 295 and 36: 96 KB of operands per 64 experts where this loads 64.)
+constexpr int kDxTile = 128;                        // tokens, and rows of W^T, of a CTA
+constexpr int kDxPart = kDxTile * 128;              // bytes of one part's 64 columns
+constexpr int kDxStageBytes = 4 * kDxPart;
+constexpr int kDxStages = 3;
+constexpr int kDxThreads = 320;                     // producer, issuer, eight epilogue warps
+constexpr int kDxStaging = 32 * 128;                // bytes per epilogue warp
+constexpr int kDxSmem = kDxStages * kDxStageBytes + 8 * kDxStaging + 1024;
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDxThreads, 1)
+router_dx_kernel(const __grid_constant__ CUtensorMap map_mid, const __grid_constant__ CUtensorMap map_hi,
+                 const __grid_constant__ CUtensorMap map_w_hi, const __grid_constant__ CUtensorMap map_w_lo,
+                 const __grid_constant__ CUtensorMap map_out, int tokens, int64_t hidden, int padded) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t full[kDxStages], empty[kDxStages], acc_full[2], acc_empty[2], drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int k_blocks = (padded + 63) / 64;
+    const int tiles_h = static_cast<int>((hidden + 2 * kDxTile - 1) / (2 * kDxTile));
+    const int all = (tokens + 2 * kDxTile - 1) / (2 * kDxTile) * tiles_h;
+    const int first = blockIdx.x / 2, stride = gridDim.x / 2;
+
+    pdl_trigger();
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < kDxStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&acc_full[a], 1);
+            mbar_init(&acc_empty[a], 2 * (kDxThreads - 64));  // both CTAs' epilogue threads
+        }
+        mbar_init(&drain, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers are set up
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0, armed = 0, parity = 0;
+        bool ok = true;
+        for (int tile = first; tile < all && ok; tile += stride) {
+            const int t = tile / tiles_h * (2 * kDxTile) + static_cast<int>(rank) * kDxTile;
+            const int h = tile % tiles_h * (2 * kDxTile) + static_cast<int>(rank) * kDxTile;
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                if (!wait_bounded(&empty[stage], phase ^ 1u, &abort_flag, kWaitLimitNs)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* at = tiles + stage * kDxStageBytes;
+                const uint32_t leader_full = map_to_cta(smem_u32(&full[stage]), 0);
+                if (leader) mbar_expect_tx(&full[stage], 2 * kDxStageBytes);
+                tma_load_2d_pair(at, &map_mid, leader_full, kb * 64, t);
+                tma_load_2d_pair(at + kDxPart, &map_hi, leader_full, kb * 64, t);
+                tma_load_2d_pair(at + 2 * kDxPart, &map_w_hi, leader_full, kb * 64, h);
+                tma_load_2d_pair(at + 3 * kDxPart, &map_w_lo, leader_full, kb * 64, h);
+                armed |= 1u << stage;
+                parity = (parity & ~(1u << stage)) | (phase << stage);
+                if (++stage == kDxStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (abort_flag && leader) {  // every copy in flight lands before the pair exits
+            volatile int never = 0;
+            for (int s = 0; s < kDxStages; ++s)
+                if (armed & (1u << s)) wait_bounded(&full[s], (parity >> s) & 1u, &never, kDrainLimitNs);
+        }
+    } else if (warp == 1 && lane == 0 && leader) {
+        constexpr uint32_t idesc = make_idesc(2 * kDxTile, 2 * kDxTile);
+        int stage = 0, local = 0;
+        uint32_t phase = 0;
+        bool issued = false, ok = true;
+        for (int tile = first; tile < all && ok; tile += stride, ++local) {
+            const int acc = local & 1;
+            if (!wait_bounded_cluster(&acc_empty[acc], ((local >> 1) & 1) ^ 1u, &abort_flag, kWaitLimitNs)) break;
+            tc_fence_after();
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                if (!wait_bounded(&full[stage], phase, &abort_flag, kWaitLimitNs)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_at = smem_u32(tiles + stage * kDxStageBytes);
+                const uint32_t w_at = d_at + 2 * kDxPart;
+                const int steps = (min(64, padded - kb * 64) + 15) / 16;  // the rest is zeros
+                for (int k = 0; k < steps; ++k) {
+                    const uint64_t mid = smem_desc_sw128(d_at + k * 32), hi = smem_desc_sw128(d_at + kDxPart + k * 32);
+                    const uint64_t w_hi = smem_desc_sw128(w_at + k * 32), w_lo = smem_desc_sw128(w_at + kDxPart + k * 32);
+                    umma_bf16_pair(tmem + acc * 256, mid, w_hi, idesc, (kb | k) != 0 ? 1u : 0u);
+                    umma_bf16_pair(tmem + acc * 256, hi, w_lo, idesc, 1u);
+                    umma_bf16_pair(tmem + acc * 256, hi, w_hi, idesc, 1u);
+                }
+                issued = true;
+                umma_commit_pair(&empty[stage]);
+                if (++stage == kDxStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (ok) umma_commit_pair(&acc_full[acc]);
+        }
+        if (issued) {  // no MMA outlives this wait, whatever the epilogue does
+            umma_commit_pair(&drain);
+            volatile int never = 0;
+            wait_bounded(&drain, 0, &never, kWaitLimitNs);
+        }
+    } else if (warp >= 2) {
+        // TMEM lane = token; each warp takes 32 tokens and half of the columns, 64 at a time
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        uint8_t* staging = tiles + kDxStages * kDxStageBytes + (warp - 2) * kDxStaging;
+        const uint32_t staged = smem_u32(staging);
+        const uint32_t row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+        const uint32_t leader_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
+        const uint32_t leader_empty1 = map_to_cta(smem_u32(&acc_empty[1]), 0);
+        int local = 0;
+        for (int tile = first; tile < all; tile += stride, ++local) {
+            const int acc = local & 1;
+            const int t = tile / tiles_h * (2 * kDxTile) + static_cast<int>(rank) * kDxTile + quarter * 32;
+            const int h = tile % tiles_h * (2 * kDxTile) + half * 128;
+            if (!wait_bounded(&acc_full[acc], (local >> 1) & 1, &abort_flag, kWaitLimitNs)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 64) {
+                uint32_t v[2][32];
+                tmem_ld32(row + acc * 256 + c, v[0]);
+                tmem_ld32(row + acc * 256 + c + 32, v[1]);
+                tmem_wait_ld();
+                if (c == 64) {  // the accumulator has been read
+                    tc_fence_before();
+                    mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+                }
+                // the tile stored before has left the staging
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {  // 16-byte piece q of this token's 128, swizzled
+                    uint32_t piece[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        piece[j] = pack_bf16x2(__uint_as_float(v[q / 4][q % 4 * 8 + 2 * j]),
+                                               __uint_as_float(v[q / 4][q % 4 * 8 + 2 * j + 1]));
+                    *reinterpret_cast<uint4*>(staging + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                        make_uint4(piece[0], piece[1], piece[2], piece[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0 && t < tokens && h + c < hidden) {
+                    tma_store_2d(&map_out, staged, h + c, t);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -875,7 +1060,7 @@ FewShape few_shape(int64_t tokens, int64_t hidden, int sms) {
 }
 
 struct Layout {
-    int64_t parts, weight, offsets, sums, total;
+    int64_t parts, weight, sums, total;
 };
 Layout layout(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw, int sms) {
     const int64_t e8 = pad8(experts);
@@ -887,9 +1072,8 @@ Layout layout(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw, int
         return l;
     }
     l.parts = 0;
-    l.weight = round256(tokens * 4 * e8 * 2);
-    l.offsets = l.weight + (dx ? round256(hidden * 3 * e8 * 2) : 0);
-    l.sums = l.offsets + 256;
+    l.weight = round256(tokens * 3 * e8 * 2);
+    l.sums = l.weight + (dx ? round256(hidden * 2 * e8 * 2) : 0);
     const int ranges = token_ranges(tokens, hidden, experts, sms);
     l.total = l.sums + (dw && ranges > 1 ? round256(ranges * experts * hidden * 4) : 0);
     return l;
@@ -970,18 +1154,37 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
                            tokens, hidden, experts, topk, sms, stream);
 
     auto* wt = reinterpret_cast<__nv_bfloat16*>(base + l.weight);
-    auto* offsets = reinterpret_cast<int32_t*>(base + l.offsets);
     const int tiles_h = static_cast<int>((hidden + 31) / 32);
     const int weight_tiles = grad_x ? tiles_h * ((e8 + 31) / 32) : 0;
     const int64_t blocks = (tokens + 7) / 8;
     const int64_t grid = weight_tiles + (blocks < 8ll * sms ? blocks : 8ll * sms);
     auto split = experts <= 64 ? split_kernel<1> : (experts <= 128 ? split_kernel<2> : split_kernel<4>);
-    MOE_CUDA_TRY(launch_dependent(split, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, weight, wt, offsets,
-                                  hidden, tiles_h, weight_tiles, grad_logits, ids, weights, grad_weights,
+    MOE_CUDA_TRY(launch_dependent(split, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, weight, wt, hidden,
+                                  tiles_h, weight_tiles, grad_logits, ids, weights, grad_weights,
                                   reinterpret_cast<uint32_t*>(parts), tokens, experts, e8, topk));
+    int device = 0;
+    MOE_CUDA_TRY(cudaGetDevice(&device));
+    const char* rejected = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
     if (grad_x) {
-        MOE_CUDA_TRY(launch_grouped_gemm(parts + e8, wt, offsets, grad_x, tokens, hidden, 3 * e8, 1,
-                                         false, stream, error, nullptr, nullptr, nullptr, 4 * e8));
+        CUtensorMap map_mid, map_hi, map_w_hi, map_w_lo, map_out;
+        if (!encode_bf16_tensor_map(&map_mid, parts + e8, tokens, e8, 3 * e8, kDxTile) ||
+            !encode_bf16_tensor_map(&map_hi, parts + 2 * e8, tokens, e8, 3 * e8, kDxTile) ||
+            !encode_bf16_tensor_map(&map_w_hi, wt, hidden, e8, 2 * e8, kDxTile) ||
+            !encode_bf16_tensor_map(&map_w_lo, wt + e8, hidden, e8, 2 * e8, kDxTile) ||
+            !encode_bf16_tensor_map(&map_out, grad_x, tokens, hidden, 0, 32)) {
+            *error = rejected;
+            return cudaErrorInvalidValue;
+        }
+        static bool configured[64] = {};
+        if (!configured[device & 63]) {
+            MOE_CUDA_TRY(cudaFuncSetAttribute(router_dx_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDxSmem));
+            configured[device & 63] = true;
+        }
+        const int64_t pairs = ((tokens + 2 * kDxTile - 1) / (2 * kDxTile)) * ((hidden + 2 * kDxTile - 1) / (2 * kDxTile));
+        const int64_t ctas = 2 * (pairs < sms / 2 ? pairs : sms / 2);
+        MOE_CUDA_TRY(launch_dependent(router_dx_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kDxThreads), kDxSmem,
+                                      stream, map_mid, map_hi, map_w_hi, map_w_lo, map_out, static_cast<int>(tokens),
+                                      hidden, e8));
     }
     if (grad_weight) {
         DwParams p;
@@ -1013,13 +1216,11 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
         p.out = used > 1 ? reinterpret_cast<float*>(base + l.sums) : grad_weight;
         CUtensorMap map_x, map_d;
         if (!encode_bf16_tensor_map(&map_x, x, tokens, hidden, 0, kTileT) ||
-            !encode_bf16_tensor_map(&map_d, parts, tokens, 4 * e8, 0, kTileT)) {
-            *error = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
+            !encode_bf16_tensor_map(&map_d, parts, tokens, 3 * e8, 0, kTileT)) {
+            *error = rejected;
             return cudaErrorInvalidValue;
         }
         static bool configured[2][64] = {};
-        int device = 0;
-        MOE_CUDA_TRY(cudaGetDevice(&device));
         auto kernel = pair ? router_dw_pair_kernel : router_dw_kernel;
         if (!configured[pair][device & 63]) {
             MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDwSmem + 1024));
