@@ -14,7 +14,7 @@
 // d_mid W_hi + d_hi W_hi + d_hi W_lo, which leaves out terms of 2^-16 |d W|.
 //
 //   split_kernel           d's parts, [T, 3 E8] bf16 with columns lo | mid | hi (E8: E
-//                          rounded up to 8), a warp per token; and W^T's parts,
+//                          rounded up to 8), and W^T's parts,
 //                          [H, 2 E8] bf16 with columns hi | lo
 //   router_dx_kernel       dx: tcgen05 on CTA pairs, K = E, three MMAs per 16 experts
 //   router_dw_kernel, router_dw_pair_kernel  dW: tcgen05 over tokens as K, both
@@ -52,57 +52,87 @@ __device__ __forceinline__ uint32_t bf16_part(float& rest) {
     return __bfloat16_as_ushort(h);
 }
 
-// d's parts of every token: a warp per token; lane holds experts 2 (lane + 32 i) and
-// the next one.
-template <int PAIRS>
+// d's parts of every token.  LANES lanes share a token, eight neighbouring experts each:
+// two 16-byte loads of grad_logits (`wide`: rows and pointer on 16 bytes) and a 16-byte
+// store per part.  The scatter goes through a row in shared memory, one lane per
+// selected expert; where ids repeat they add one after the other, in order.
+template <int LANES>
 __device__ void split_gradient(const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
                                const float* __restrict__ weights, const float* __restrict__ grad_weights,
-                               uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded, int topk,
-                               int block, int blocks) {
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = static_cast<int64_t>(blocks) * 8;
-    const int half = padded / 2;  // 32-bit words of one part's columns
-    for (int64_t t = block * 8ll + (threadIdx.x >> 5); t < tokens; t += warps) {
-        float d[PAIRS][2];
+                               __nv_bfloat16* __restrict__ parts, int64_t tokens, int experts, int padded, int topk,
+                               bool wide, int block, int blocks) {
+    constexpr int kTokens = 32 / LANES;  // per warp
+    __shared__ __align__(16) float rows[8][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LANES - 1);
+    const int slot = (threadIdx.x & 31) / LANES;
+    float* row = rows[warp] + slot * (LANES * 8);
+    const int e0 = lane * 8;
+    const int64_t stride = static_cast<int64_t>(blocks) * 8 * kTokens;
+    for (int64_t first = (block * 8ll + warp) * kTokens; first < tokens; first += stride) {  // same for the warp
+        const int64_t t = first + slot;
+        const bool live = t < tokens;
+        float d[8] = {};
+        if (grad_logits && live && e0 < experts) {
+            const float* from = grad_logits + t * experts + e0;
+            if (wide) {
+                const float4 v = *reinterpret_cast<const float4*>(from);
+                d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+                if (e0 + 4 < experts) {
+                    const float4 u = *reinterpret_cast<const float4*>(from + 4);
+                    d[4] = u.x, d[5] = u.y, d[6] = u.z, d[7] = u.w;
+                }
+            } else {
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-            const int e = 2 * (lane + 32 * i);
-            d[i][0] = grad_logits && e < experts ? grad_logits[t * experts + e] : 0.0f;
-            d[i][1] = grad_logits && e + 1 < experts ? grad_logits[t * experts + e + 1] : 0.0f;
+                for (int j = 0; j < 8; ++j)
+                    if (e0 + j < experts) d[j] = from[j];
+            }
         }
         int id = -1;
         float w = 0.0f, g = 0.0f;
-        if (lane < topk) {
+        if (live && lane < topk) {
             id = ids[t * topk + lane];
             w = weights[t * topk + lane];
             g = grad_weights[t * topk + lane];
         }
         float dot = w * g;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+        for (int off = LANES / 2; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
         const float ds = w * (g - dot);
-        for (int k = 0; k < topk; ++k) {  // in order: a repeated id adds the same way every time
-            const int e = __shfl_sync(0xffffffffu, id, k);
-            const float v = __shfl_sync(0xffffffffu, ds, k);
-            if (e < 0 || e >= experts) continue;
-#pragma unroll
-            for (int i = 0; i < PAIRS; ++i)
-                if (lane + 32 * i == e >> 1) {
-                    if (e & 1) d[i][1] += v;
-                    else d[i][0] += v;
-                }
+        *reinterpret_cast<float4*>(row + e0) = make_float4(d[0], d[1], d[2], d[3]);
+        *reinterpret_cast<float4*>(row + e0 + 4) = make_float4(d[4], d[5], d[6], d[7]);
+        const bool mine = id >= 0 && id < experts;
+        // one key per expert of this token; lanes without one differ from all others
+        const int key = mine ? slot << 16 | id : -1 - static_cast<int>(threadIdx.x & 31);
+        const unsigned same = __match_any_sync(0xffffffffu, key);
+        if (__any_sync(0xffffffffu, __popc(same) > 1)) {
+            for (int k = 0; k < topk; ++k) {
+                __syncwarp();
+                if (mine && lane == k) row[id] += ds;
+            }
+        } else {
+            __syncwarp();
+            if (mine) row[id] += ds;
         }
-        uint32_t* row = parts + t * 3 * half;
+        __syncwarp();
+        const float4 v = *reinterpret_cast<const float4*>(row + e0);
+        const float4 u = *reinterpret_cast<const float4*>(row + e0 + 4);
+        __syncwarp();  // read before the next token's row is written
+        d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+        d[4] = u.x, d[5] = u.y, d[6] = u.z, d[7] = u.w;
+        if (live && e0 < padded) {
+            __nv_bfloat16* to = parts + t * 3 * padded + e0;
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-            const int at = lane + 32 * i;
-            if (at >= half) continue;
-            const uint32_t hi = bf16_part(d[i][0]) | bf16_part(d[i][1]) << 16;
-            const uint32_t mid = bf16_part(d[i][0]) | bf16_part(d[i][1]) << 16;
-            const uint32_t lo = bf16_part(d[i][0]) | bf16_part(d[i][1]) << 16;
-            row[at] = lo;
-            row[half + at] = mid;
-            row[2 * half + at] = hi;
+            for (int part = 2; part >= 0; --part) {  // hi, mid, lo
+                uint32_t piece[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 both = __floats2bfloat162_rn(d[2 * j], d[2 * j + 1]);
+                    piece[j] = *reinterpret_cast<const uint32_t*>(&both);
+                    d[2 * j] -= __uint_as_float(piece[j] << 16);
+                    d[2 * j + 1] -= __uint_as_float(piece[j] & 0xffff0000u);
+                }
+                *reinterpret_cast<uint4*>(to + part * padded) = make_uint4(piece[0], piece[1], piece[2], piece[3]);
+            }
         }
     }
 }
@@ -128,19 +158,20 @@ __device__ void split_weight(const float* __restrict__ weight, __nv_bfloat16* __
 
 // Both splits in one launch: the first CTAs take a tile of W each (none without dx),
 // the others d.
-template <int PAIRS>
+template <int LANES>
 __global__ void __launch_bounds__(256)
-split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weight_parts, int64_t hidden, int tiles_h, int tiles,
+split_kernel(const float* __restrict__ weight, __nv_bfloat16* __restrict__ weight_parts, int64_t hidden,
+             int tiles_h, int tiles,
              const float* __restrict__ grad_logits, const int32_t* __restrict__ ids,
              const float* __restrict__ weights, const float* __restrict__ grad_weights,
-             uint32_t* __restrict__ parts, int64_t tokens, int experts, int padded, int topk) {
+             __nv_bfloat16* __restrict__ parts, int64_t tokens, int experts, int padded, int topk, bool wide) {
     pdl_trigger();
     pdl_wait();
     const int block = blockIdx.x;
     if (block < tiles) {
         split_weight(weight, weight_parts, experts, padded, hidden, block % tiles_h * 32ll, block / tiles_h * 32);
     } else {
-        split_gradient<PAIRS>(grad_logits, ids, weights, grad_weights, parts, tokens, experts, padded, topk,
+        split_gradient<LANES>(grad_logits, ids, weights, grad_weights, parts, tokens, experts, padded, topk, wide,
                               block - tiles, gridDim.x - tiles);
     }
 }
@@ -1156,12 +1187,15 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
     auto* wt = reinterpret_cast<__nv_bfloat16*>(base + l.weight);
     const int tiles_h = static_cast<int>((hidden + 31) / 32);
     const int weight_tiles = grad_x ? tiles_h * ((e8 + 31) / 32) : 0;
-    const int64_t blocks = (tokens + 7) / 8;
+    // as few lanes per token as hold its experts, eight each, and its ids, one each
+    const int lanes = experts <= 64 && topk <= 8 ? 8 : (experts <= 128 && topk <= 16 ? 16 : 32);
+    const bool wide = experts % 4 == 0 && reinterpret_cast<uintptr_t>(grad_logits) % 16 == 0;
+    const int64_t blocks = (tokens * lanes + 255) / 256;
     const int64_t grid = weight_tiles + (blocks < 8ll * sms ? blocks : 8ll * sms);
-    auto split = experts <= 64 ? split_kernel<1> : (experts <= 128 ? split_kernel<2> : split_kernel<4>);
+    auto split = lanes == 8 ? split_kernel<8> : (lanes == 16 ? split_kernel<16> : split_kernel<32>);
     MOE_CUDA_TRY(launch_dependent(split, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, weight, wt, hidden,
                                   tiles_h, weight_tiles, grad_logits, ids, weights, grad_weights,
-                                  reinterpret_cast<uint32_t*>(parts), tokens, experts, e8, topk));
+                                  parts, tokens, experts, e8, topk, wide));
     int device = 0;
     MOE_CUDA_TRY(cudaGetDevice(&device));
     const char* rejected = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
