@@ -644,11 +644,12 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
     copy_wait<0>();
 }
 
-constexpr int kExpandThreads = 256;                   // 4 x 16 rows, 2 halves of the columns
+constexpr int kExpandThreads = 128;                   // 4 x 16 rows
 constexpr int kExpandStages = 2;
-constexpr int kTileCols = 128;                        // rows of B per step: 128 columns, or 64 gate + 64 up
+constexpr int kTileCols = 64;                         // rows of B per step: 64 columns, or 32 gate + 32 up
 constexpr int kBaseStride = kTileCols * 2 + 16;       // bytes; the pads keep ldmatrix and row stores conflict-free
 template <int RN> constexpr int b_stride() { return rank_k<RN>() * 2 + 16; }
+template <int RN> constexpr int expand_ctas() { return RN <= 32 ? 6 : (RN <= 64 ? 4 : 2); }  // per SM
 template <int RN> constexpr int expand_smem() {
     return kExpandStages * (kTileRows * kBaseStride + kTileCols * b_stride<RN>());
 }
@@ -718,7 +719,7 @@ __device__ __forceinline__ Stretch stretch_of(int64_t q, int64_t all) {
 // tile form one cp.async pipeline whose stages hold the tile's base rows and the
 // pair's rows of B; s stays in registers as bf16 fragments.
 template <int RN, bool SWIGLU>
-__global__ void __launch_bounds__(kExpandThreads, RN <= 32 ? 3 : (RN <= 64 ? 2 : 1))
+__global__ void __launch_bounds__(kExpandThreads, expand_ctas<RN>())
 expand_tile_kernel(const Adapter p, int blocks) {
     constexpr int RK = rank_k<RN>();
     constexpr int kOut = SWIGLU ? kTileCols / 2 : kTileCols;  // output columns of a block
@@ -726,18 +727,18 @@ expand_tile_kernel(const Adapter p, int blocks) {
     constexpr int kStage = kTileRows * kBaseStride + kTileCols * b_stride<RN>();
     constexpr int kChunks = RK / 8, kBRows = kExpandThreads / kChunks, kBCopies = kTileCols / kBRows;
     extern __shared__ __align__(128) uint8_t smem[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, half = tid >> 7;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // this thread's share of the base rows: one 16-byte chunk of rows i_first + 16 j
-    const int c = (tid & 15) * 8, i_first = tid >> 4;
-    const int c_col = SWIGLU ? c & 63 : c;  // its column inside the block
+    const int c = (tid & 7) * 8, i_first = tid >> 3;
+    const int c_col = SWIGLU ? c & 31 : c;  // its column inside the block
     const int b_q = tid % kChunks, b_n = tid / kChunks;
     // this lane's first row of B for ldmatrix, and its first pair of base, inside a stage
     const uint32_t b_lane = kTileRows * kBaseStride +
-                            (half * (kOut / 2) + (lane & 7) + ((lane >> 4) << 3)) * b_stride<RN>() + ((lane >> 3) & 1) * 16;
-    const int base_lane = (warp * 16 + (lane >> 2)) * kBaseStride + half * kOut + (lane & 3) * 4;
+                            ((lane & 7) + ((lane >> 4) << 3)) * b_stride<RN>() + ((lane >> 3) & 1) * 16;
+    const int base_lane = (warp * 16 + (lane >> 2)) * kBaseStride + (lane & 3) * 4;
     const int r0 = warp * 16 + (lane >> 2);
-    constexpr int kPieces = kOut / 16, kPer = 32 / kPieces;  // out: 16-byte pieces of a half row; rows at a time
-    const int out_row = warp * 16 + lane / kPieces, out_col = half * (kOut / 2) + (lane % kPieces) * 8;
+    constexpr int kPieces = kOut / 8, kPer = 32 / kPieces;  // out: 16-byte pieces of a row; rows at a time
+    const int out_row = warp * 16 + lane / kPieces, out_col = (lane % kPieces) * 8;
     pdl_trigger();
     pdl_wait();
     __shared__ int claimed[2];
@@ -755,7 +756,7 @@ expand_tile_kernel(const Adapter p, int blocks) {
         for (int j = 0; j < kTileRows / 16; ++j) {
             const int i = i_first + 16 * j;
             base[j] = p.base + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.n +
-                      static_cast<int64_t>(first_block) * kOut + c_col + (SWIGLU && c >= 64 ? p.cols : 0);
+                      static_cast<int64_t>(first_block) * kOut + c_col + (SWIGLU && c >= 32 ? p.cols : 0);
         }
         // and its share of B: chunk b_q of rows b_n + kBRows j
         const int64_t col0 = static_cast<int64_t>(first_block) * kOut;
@@ -763,7 +764,7 @@ expand_tile_kernel(const Adapter p, int blocks) {
 #pragma unroll
         for (int j = 0; j < kBCopies; ++j) {
             const int n = b_n + kBRows * j;
-            const int64_t column = col0 + (SWIGLU ? (n & 63) + (n >= 64 ? p.cols : 0) : n);
+            const int64_t column = col0 + (SWIGLU ? (n & 31) + (n >= 32 ? p.cols : 0) : n);
             b[j] = p.b + (key < 0 ? 0 : (static_cast<int64_t>(key) * p.n + column) * p.rank + b_q * 8);
         }
         int64_t left = p.cols - col0;  // columns from the next block to load on
@@ -782,7 +783,7 @@ expand_tile_kernel(const Adapter p, int blocks) {
 #pragma unroll
                 for (int j = 0; j < kBCopies; ++j) {
                     const int n = b_n + kBRows * j;
-                    const bool in = b_q * 8 < p.rank && (SWIGLU ? n & 63 : n) < left;
+                    const bool in = b_q * 8 < p.rank && (SWIGLU ? n & 31 : n) < left;
                     copy16(b_at + j * kBRows * b_stride<RN>(), in ? b[j] : p.b, in);
                     b[j] += kOut * p.rank;
                 }
@@ -832,14 +833,14 @@ expand_tile_kernel(const Adapter p, int blocks) {
                     const uint32_t bs = smem_addr(base_s) + b_lane;
                     uint8_t* const mine = base_s + base_lane;
 #pragma unroll
-                    for (int f = 0; f < kOut / 2; f += 16) {
+                    for (int f = 0; f < kOut; f += 16) {
                         float acc[kHalves][2][4];
 #pragma unroll
                         for (int g = 0; g < kHalves; ++g)
 #pragma unroll
                             for (int kk = 0; kk < RK / 16; ++kk) {
                                 uint32_t bf[4];
-                                ldmatrix4(bs + (f + g * 64) * b_stride<RN>() + kk * 32, bf);
+                                ldmatrix4(bs + (f + g * 32) * b_stride<RN>() + kk * 32, bf);
                                 if (kk == 0) {
                                     mma16816_first(acc[g][0], lo[0], bf[0], bf[1]);
                                     mma16816_first(acc[g][1], lo[0], bf[2], bf[3]);
@@ -860,7 +861,7 @@ expand_tile_kernel(const Adapter p, int blocks) {
                                 float2 y = add2(make_float2(bf16_lo(v), bf16_hi(v)),
                                                 make_float2(acc[0][q][2 * h], acc[0][q][2 * h + 1]));
                                 if constexpr (SWIGLU) {
-                                    const uint32_t u = at[32];  // 128 bytes further
+                                    const uint32_t u = at[16];  // 64 bytes further
                                     y = fast_silu_times(y, add2(make_float2(bf16_lo(u), bf16_hi(u)),
                                                                 make_float2(acc[1][q][2 * h], acc[1][q][2 * h + 1])));
                                 }
@@ -869,11 +870,11 @@ expand_tile_kernel(const Adapter p, int blocks) {
                     }
                 } else if constexpr (SWIGLU) {
                     // without an adapter: the bits of swiglu_kernel; two rows, a pair of columns a lane
-                    uint8_t* pair = base_s + (warp * 16 + (lane >> 4)) * kBaseStride + half * kOut + (lane & 15) * 4;
+                    uint8_t* pair = base_s + (warp * 16 + (lane >> 4)) * kBaseStride + (lane & 15) * 4;
 #pragma unroll 4
                     for (int i = 0; i < 16; i += 2, pair += 2 * kBaseStride) {
                         uint32_t* at = reinterpret_cast<uint32_t*>(pair);
-                        const uint32_t g = *at, u = at[32];
+                        const uint32_t g = *at, u = at[16];
                         *at = pack2(silu_times(bf16_lo(g), bf16_lo(u)), silu_times(bf16_hi(g), bf16_hi(u)));
                     }
                 }
@@ -1091,7 +1092,7 @@ cudaError_t tiles(const Adapter& p, const Shape& f, int sms, cudaStream_t stream
                                  f.splits, kTileThreads, kShrinkSmem, stream, &shrink_fit[f.splits][device & 63], p));
     const int out_cols = SWIGLU ? kTileCols / 2 : kTileCols;
     const int blocks = static_cast<int>((p.cols + out_cols - 1) / out_cols);
-    const int64_t expand_most = resident(expand_smem<RN>(), RN <= 32 ? 3 : (RN <= 64 ? 2 : 1));
+    const int64_t expand_most = resident(expand_smem<RN>(), expand_ctas<RN>());
     return launch_dependent(expand_tile_kernel<RN, SWIGLU>, dim3(static_cast<unsigned>(expand_most)),
                             dim3(kExpandThreads), expand_smem<RN>(), stream, p, blocks);
 }
