@@ -481,16 +481,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The same with c = 0 before it.
-__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%10, %10, %10, %10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-}
-
-
 constexpr int kShrinkStages = 3;
 constexpr int kShrinkK = 128;                   // K elements per stage: 256 bytes of each row
 constexpr int kShrinkRow = kShrinkK * 2;
@@ -728,17 +718,28 @@ expand_tile_kernel(const Adapter p, int blocks) {
     constexpr int kChunks = RK / 8, kBRows = kExpandThreads / kChunks, kBCopies = kTileCols / kBRows;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int cols = static_cast<int>(p.cols);
     // this thread's share of the base rows: one 16-byte chunk of rows i_first + 16 j
     const int c = (tid & 7) * 8, i_first = tid >> 3;
     const int c_col = SWIGLU ? c & 31 : c;  // its column inside the block
-    const int b_q = tid % kChunks, b_n = tid / kChunks;
+    const int b_q = tid % kChunks, b_n = tid / kChunks;  // and of B: chunk b_q of rows b_n + kBRows j
+    const uint32_t base_to = i_first * kBaseStride + c * 2;
+    const uint32_t b_to = kTileRows * kBaseStride + b_n * b_stride<RN>() + b_q * 16;
     // this lane's first row of B for ldmatrix, and its first pair of base, inside a stage
     const uint32_t b_lane = kTileRows * kBaseStride +
                             ((lane & 7) + ((lane >> 4) << 3)) * b_stride<RN>() + ((lane >> 3) & 1) * 16;
-    const int base_lane = (warp * 16 + (lane >> 2)) * kBaseStride + (lane & 3) * 4;
     const int r0 = warp * 16 + (lane >> 2);
+    const int base_lane = r0 * kBaseStride + (lane & 3) * 4;
     constexpr int kPieces = kOut / 8, kPer = 32 / kPieces;  // out: 16-byte pieces of a row; rows at a time
     const int out_row = warp * 16 + lane / kPieces, out_col = (lane % kPieces) * 8;
+    const int out_lane = out_row * kBaseStride + out_col * 2;
+    if (b_q * 8 >= p.rank) {  // past the rank B is zero: written once, never copied over
+#pragma unroll
+        for (int s = 0; s < kExpandStages; ++s)
+#pragma unroll
+            for (int j = 0; j < kBCopies; ++j)
+                *reinterpret_cast<uint4*>(smem + s * kStage + b_to + j * kBRows * b_stride<RN>()) = make_uint4(0, 0, 0, 0);
+    }
     pdl_trigger();
     pdl_wait();
     __shared__ int claimed[2];
@@ -751,57 +752,53 @@ expand_tile_kernel(const Adapter p, int blocks) {
         const int first_block = static_cast<int>(stretch.x % blocks);
         const int count = static_cast<int>(min(static_cast<int64_t>(blocks - first_block), stretch.y - stretch.x));
         const int key = p.keys[tile.x];
+        // Blocks in which a column of this thread's lies inside the row: its copies and stores
+        // stop there, so a step compares step numbers only.
+        const int col0 = first_block * kOut, width = cols - col0;
+        const auto blocks_with = [&](int column) { return width > column ? (width - column + kOut - 1) / kOut : 0; };
+        const int base_blocks = blocks_with(c_col), base_rows = (tile.y - i_first + 15) / 16;
         const bf16* base[kTileRows / 16];
 #pragma unroll
         for (int j = 0; j < kTileRows / 16; ++j) {
             const int i = i_first + 16 * j;
-            base[j] = p.base + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.n +
-                      static_cast<int64_t>(first_block) * kOut + c_col + (SWIGLU && c >= 32 ? p.cols : 0);
+            base[j] = p.base + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.n + col0 + c_col +
+                      (SWIGLU && c >= 32 ? cols : 0);
         }
-        // and its share of B: chunk b_q of rows b_n + kBRows j
-        const int64_t col0 = static_cast<int64_t>(first_block) * kOut;
         const bf16* b[kBCopies];
+        int b_blocks[kBCopies];
 #pragma unroll
         for (int j = 0; j < kBCopies; ++j) {
-            const int n = b_n + kBRows * j;
-            const int64_t column = col0 + (SWIGLU ? (n & 31) + (n >= 32 ? p.cols : 0) : n);
-            b[j] = p.b + (key < 0 ? 0 : (static_cast<int64_t>(key) * p.n + column) * p.rank + b_q * 8);
+            const int n = b_n + kBRows * j, column = SWIGLU ? n & 31 : n;
+            b[j] = p.b + (key < 0 ? 0 : (static_cast<int64_t>(key) * p.n + col0 + column + (SWIGLU && n >= 32 ? cols : 0)) *
+                                            p.rank + b_q * 8);
+            b_blocks[j] = key < 0 || b_q * 8 >= p.rank ? 0 : blocks_with(column);
         }
-        int64_t left = p.cols - col0;  // columns from the next block to load on
-        auto load = [&](int slot) {
-            const uint32_t at = smem_addr(smem) + slot * kStage;
-            if (c_col < left) {
+        auto load = [&](uint32_t stage, int step) {
+            const uint32_t at = smem_addr(smem) + stage;
+            if (step < base_blocks) {
 #pragma unroll
-                for (int j = 0; j < kTileRows / 16; ++j) {
-                    if (i_first + 16 * j < tile.y)
-                        copy16(at + (i_first + 16 * j) * kBaseStride + c * 2, base[j], true);
-                    base[j] += kOut;
-                }
+                for (int j = 0; j < kTileRows / 16; ++j)
+                    if (j < base_rows) copy16(at + base_to + 16 * j * kBaseStride, base[j], true);
             }
-            if (key >= 0) {
-                const uint32_t b_at = at + kTileRows * kBaseStride + b_n * b_stride<RN>() + b_q * 16;
 #pragma unroll
-                for (int j = 0; j < kBCopies; ++j) {
-                    const int n = b_n + kBRows * j;
-                    const bool in = b_q * 8 < p.rank && (SWIGLU ? n & 31 : n) < left;
-                    copy16(b_at + j * kBRows * b_stride<RN>(), in ? b[j] : p.b, in);
-                    b[j] += kOut * p.rank;
-                }
+            for (int j = 0; j < kTileRows / 16; ++j) base[j] += kOut;
+#pragma unroll
+            for (int j = 0; j < kBCopies; ++j) {
+                if (step < b_blocks[j]) copy16(at + b_to + j * kBRows * b_stride<RN>(), b[j], true);
+                b[j] += kOut * p.rank;
             }
-            left -= kOut;
         };
         __syncthreads();  // the item before is done with its stages
-#pragma unroll
-        for (int s = 0; s < kExpandStages - 1; ++s) {
-            if (s < count) load(s);
-            copy_commit();
-        }
+        load(0, 0);
+        copy_commit();
 
         bf16* out[16 / kPer];
+        int out_blocks[16 / kPer];
 #pragma unroll
         for (int j = 0; j < 16 / kPer; ++j) {
             const int i = out_row + j * kPer;
-            out[j] = p.out + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.cols + out_col;
+            out[j] = p.out + static_cast<int64_t>(i < tile.y ? p.order[tile.x + i] : 0) * p.cols + col0 + out_col;
+            out_blocks[j] = i < tile.y ? blocks_with(out_col) : 0;
         }
 
         // s of this warp's 16 rows as fragments
@@ -818,54 +815,54 @@ expand_tile_kernel(const Adapter p, int blocks) {
                 }
         }
 
-        int slot = 0, load_slot = kExpandStages - 1;
+        uint32_t stage = 0;
         for (int step = 0; step < count; ++step) {
-            copy_wait<kExpandStages - 2>();
+            copy_wait<0>();
             __syncthreads();  // this stage has landed everywhere, and the one before is done with
-            if (step + kExpandStages - 1 < count) load(load_slot);
+            if (step + 1 < count) load(kStage - stage, step + 1);
             copy_commit();
-            uint8_t* base_s = smem + slot * kStage;
-            const int64_t c0 = static_cast<int64_t>(first_block + step) * kOut;
+            uint8_t* const base_s = smem + stage;
             if (warp * 16 < tile.y) {
                 if (key >= 0) {
                     // 16 columns at a time (with SwiGLU 16 gate and the matching 16 up columns), so
-                    // few accumulators live at once
+                    // few accumulators live at once; they start from base and end in its place
+                    // (conflict-free)
                     const uint32_t bs = smem_addr(base_s) + b_lane;
                     uint8_t* const mine = base_s + base_lane;
 #pragma unroll
                     for (int f = 0; f < kOut; f += 16) {
                         float acc[kHalves][2][4];
+                        const auto word = [&](int h, int q) {
+                            return reinterpret_cast<uint32_t*>(mine + h * 8 * kBaseStride + (f + q * 8) * 2);
+                        };
+#pragma unroll
+                        for (int g = 0; g < kHalves; ++g)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t v = word(h, q)[g * 16];  // up: 64 bytes further
+                                    acc[g][q][2 * h] = bf16_lo(v), acc[g][q][2 * h + 1] = bf16_hi(v);
+                                }
 #pragma unroll
                         for (int g = 0; g < kHalves; ++g)
 #pragma unroll
                             for (int kk = 0; kk < RK / 16; ++kk) {
                                 uint32_t bf[4];
                                 ldmatrix4(bs + (f + g * 32) * b_stride<RN>() + kk * 32, bf);
-                                if (kk == 0) {
-                                    mma16816_first(acc[g][0], lo[0], bf[0], bf[1]);
-                                    mma16816_first(acc[g][1], lo[0], bf[2], bf[3]);
-                                } else {
-                                    mma16816(acc[g][0], lo[kk], bf[0], bf[1]);
-                                    mma16816(acc[g][1], lo[kk], bf[2], bf[3]);
-                                }
+                                mma16816(acc[g][0], lo[kk], bf[0], bf[1]);
+                                mma16816(acc[g][1], lo[kk], bf[2], bf[3]);
                                 mma16816(acc[g][0], hi[kk], bf[0], bf[1]);
                                 mma16816(acc[g][1], hi[kk], bf[2], bf[3]);
                             }
-                        // y = base + delta in place (conflict-free), in this warp's rows and columns
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
-                                uint32_t* at = reinterpret_cast<uint32_t*>(mine + h * 8 * kBaseStride + (f + q * 8) * 2);
-                                const uint32_t v = *at;
-                                float2 y = add2(make_float2(bf16_lo(v), bf16_hi(v)),
-                                                make_float2(acc[0][q][2 * h], acc[0][q][2 * h + 1]));
-                                if constexpr (SWIGLU) {
-                                    const uint32_t u = at[16];  // 64 bytes further
-                                    y = fast_silu_times(y, add2(make_float2(bf16_lo(u), bf16_hi(u)),
-                                                                make_float2(acc[1][q][2 * h], acc[1][q][2 * h + 1])));
-                                }
-                                *at = pack2(y.x, y.y);
+                                float2 y = make_float2(acc[0][q][2 * h], acc[0][q][2 * h + 1]);
+                                if constexpr (SWIGLU)
+                                    y = fast_silu_times(y, make_float2(acc[1][q][2 * h], acc[1][q][2 * h + 1]));
+                                *word(h, q) = pack2(y.x, y.y);
                             }
                     }
                 } else if constexpr (SWIGLU) {
@@ -881,14 +878,13 @@ expand_tile_kernel(const Adapter p, int blocks) {
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 16 / kPer; ++j) {
-                    const int i = out_row + j * kPer;
-                    if (i < tile.y && c0 + out_col < p.cols)
-                        *reinterpret_cast<uint4*>(out[j] + c0) =
-                            *reinterpret_cast<const uint4*>(base_s + i * kBaseStride + out_col * 2);
+                    if (step < out_blocks[j])
+                        *reinterpret_cast<uint4*>(out[j]) =
+                            *reinterpret_cast<const uint4*>(base_s + out_lane + j * kPer * kBaseStride);
+                    out[j] += kOut;
                 }
             }
-            if (++slot == kExpandStages) slot = 0;
-            if (++load_slot == kExpandStages) load_slot = 0;
+            stage = kStage - stage;
         }
         stretch.x += count;
         if (stretch.x == stretch.y) {  // the claim was made a stretch ago; make the next one now
