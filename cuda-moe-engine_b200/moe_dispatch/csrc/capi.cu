@@ -322,8 +322,9 @@ int moe_swiglu(const void* projection, int32_t dtype, const int32_t* valid_rows,
 
 static int check_adapter_shape(int64_t rows, int64_t k, int32_t rank, int32_t adapters, int32_t experts) {
     if (rows < 0 || rows > INT_MAX / 4) return fail(MOE_ERR_INVALID, "rows must be in 0..INT_MAX / 4");
-    if (k < 8 || k % 8 || k > INT_MAX / 8)
-        return fail(MOE_ERR_INVALID, "adapter dimensions must be positive multiples of 8");
+    // above 2^26 a single row's pieces of K would not fit the launch grid
+    if (k < 8 || k % 8 || k > 1 << 26)
+        return fail(MOE_ERR_INVALID, "adapter dimensions must be positive multiples of 8, K up to 2^26");
     if (rank < 8 || rank % 8 || rank > moe::kMaxAdapterRank)
         return fail(MOE_ERR_INVALID, "rank must be a multiple of 8 up to %d", moe::kMaxAdapterRank);
     if (adapters < 1 || adapters > moe::kMaxAdapters)

@@ -130,3 +130,10 @@ def test_library_refuses_bad_row_maps_and_queries():
     assert "null" in lib.moe_last_error().decode()
     assert lib.moe_adapter_scratch_bytes(4, 12, 8, 2, 1) == -1
     assert lib.moe_adapter_scratch_bytes(4, 16, 8, 600, 1) == -1
+
+
+def test_library_refuses_rows_too_long_for_the_grid():
+    lib = load_library()
+    assert adapter_call(lib, k=2**26 + 8) == 1
+    assert "2^26" in lib.moe_last_error().decode()
+    assert lib.moe_adapter_scratch_bytes(4, 2**26 + 8, 8, 2, 1) == -1

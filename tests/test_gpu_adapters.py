@@ -199,6 +199,30 @@ def test_long_projections_pass_32_bit_offsets():
         assert bool(((out[r].double().cpu() - want[0]).abs() <= bound[0]).all())
 
 
+@pytest.mark.parametrize("rows", [60, 700])
+def test_extreme_base_values_pass_through(rows):
+    """A product of zero leaves every base value as it is: subnormals, the largest, infinities."""
+    p, used = make_problem([rows // 2, rows // 2], 136, 200, 3, 24, False, 8)
+    p["b"].zero_()
+    values = torch.tensor([2.0**-133, -2.0**-130, 2.0**-126, 3.3895e38, -3.3895e38, float("inf"), -float("inf"), 1.0])
+    p["base"].copy_(values.repeat(25).to(torch.bfloat16))
+    p["base"][5, 17] = float("nan")
+    out = run(p, False).cpu()
+    same = out == p["base"]
+    assert not bool(same[5, 17]) and bool(torch.isnan(out[5, 17]))
+    same[5, 17] = True
+    assert bool(same.all())
+
+
+@pytest.mark.parametrize("rows", [60, 700])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_inference_mode_gives_the_same_rows(rows, swiglu):
+    p, used = make_problem([rows // 2, rows // 2], 136, 72, 6, 16, swiglu, 3)
+    want = run(p, swiglu)
+    with torch.inference_mode():
+        assert torch.equal(run(p, swiglu), want)
+
+
 def test_no_rows():
     p, _ = make_problem([0, 0], 64, 64, 2, 8, True, 6)
     assert run(p, True).shape == (0, 64)

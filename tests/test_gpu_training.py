@@ -418,3 +418,46 @@ def test_balance_loss_with_every_expert_chosen(experts):
     assert counts.cpu().tolist() == want_counts.tolist()
     assert abs(loss.item() - want) <= 268 * U * want
     check_gradient(grad, want_grad, terms)
+
+
+@pytest.mark.parametrize("shape", [(33, 264, 40, 12), (50, 136, 100, 20), (29, 72, 130, 17), (300, 2312, 66, 3),
+                                   (70, 64, 252, 32), (5, 40, 64, 8)], ids=str)
+def test_route_backward_of_repeated_ids_and_unaligned_logit_gradients(shape):
+    from moe_dispatch import route_backward
+
+    tokens, hidden, experts, topk = shape
+    x, weight, ids, weights, gw, gl = router_problem(tokens, hidden, experts, topk, seed=sum(shape))
+    ids[1] = ids[1, 0]                           # one expert topk times
+    ids[2, 1:] = -1
+    ids[3, :2] = torch.tensor([experts, experts - 1])
+    buffer = torch.empty(tokens * experts + 1, device="cuda")
+    shifted = buffer[1:].view(tokens, experts)   # contiguous rows off every 16-byte boundary
+    shifted.copy_(gl)
+    aligned = [t.cuda() for t in (x, weight, ids, weights, gw, gl)]
+    got = route_backward(*aligned[:5], shifted)
+    check_router((x, weight, ids, weights, gw, gl), *got)
+    assert all(torch.equal(a, b) for a, b in zip(got, route_backward(*aligned)))
+
+
+def test_balance_loss_of_strided_ids_and_masks():
+    from moe_dispatch import balance_loss
+
+    logits, ids, _ = make_logits(500, 12, 3, torch.float32, 9)
+    mask = torch.arange(500) % 3 != 1
+    want = balance_loss(logits.cuda(), ids.to(torch.int32).cuda(), token_mask=mask.cuda())
+    wide_ids = torch.stack([ids.long(), -ids.long()], -1).cuda()[..., 0]
+    wide_mask = torch.stack([mask, ~mask], -1).cuda()[:, 0]
+    assert not wide_ids.is_contiguous() and not wide_mask.is_contiguous()
+    got = balance_loss(logits.cuda(), wide_ids, token_mask=wide_mask)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_inference_mode_gives_the_same_values():
+    from moe_dispatch import balance_loss, route, route_backward
+
+    problem = [t.cuda() for t in router_problem(300, 264, 24, 4, seed=5)]
+    x, weight, ids, _, _, logits = problem
+    want = (*route(x, weight, topk=4), *route_backward(*problem), *balance_loss(logits, ids))
+    with torch.inference_mode():
+        got = (*route(x, weight, topk=4), *route_backward(*problem), *balance_loss(logits, ids))
+    assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
