@@ -666,8 +666,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // once (|g| 2^-24), both are good to a few steps, so it is within (|g| + 8) 2^-23
 // of the value, against 2^-8 of the rounding to bf16.  Where 2^(-g log2 e) is
 // infinite the reciprocal is 0.  (With expf, a division and single lanes the
-// SwiGLU form of the expand kernel issued 36 instructions an element and was
-// bound by them: 309 us at 4096 tokens, 8 experts, top-2, against 182 with this.)
+// SwiGLU form of the expand kernel was bound by its instructions and took 1.7 times as
+// long at 4096 tokens, 8 experts, top-2.)
 __device__ __forceinline__ float2 fast_silu_times(float2 g, float2 u) {
     const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
     float2 e, r;
@@ -704,10 +704,18 @@ __device__ __forceinline__ Stretch stretch_of(int64_t q, int64_t all) {
 
 // CTAs claim stretches of the (tile, column block) pairs, long ones first, and walk
 // them tile by tile: tiles differ in their rows, so equal shares end far apart
-// (one share per CTA: 306 us instead of 186 at 4096 tokens, 8 experts of 14336,
+// (one share per CTA took 1.6 times as long at 4096 tokens, 8 experts of 14336,
 // top-2), and short stretches alone pay for many starts.  A CTA's blocks of one
 // tile form one cp.async pipeline whose stages hold the tile's base rows and the
-// pair's rows of B; s stays in registers as bf16 fragments.
+// pair's rows of B; s stays in registers as bf16 fragments, and the accumulators
+// start from base.
+//
+// Measured: 163-168 us at that size (8192 rows -> 2 x 14336, rank 16: 710 MB through
+// memory in this kernel, 108 us), 259-262 at 98304 rows of 2 x 1408, 2048 pairs, rank 32.
+// Bound by instruction issue (58 %) and the warps' dependent chains.  Four warps a CTA
+// and six CTAs an SM, because a barrier then holds up 64 columns and not 128 (175 and
+// 300 us with eight warps).  B in the warps' registers instead of shared memory, with no
+// barrier: 180 and 376.  Three stages: the same as two.
 template <int RN, bool SWIGLU>
 __global__ void __launch_bounds__(kExpandThreads, expand_ctas<RN>())
 expand_tile_kernel(const Adapter p, int blocks) {

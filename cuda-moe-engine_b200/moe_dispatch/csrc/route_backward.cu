@@ -559,8 +559,8 @@ router_dw_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 // tokens' d and hi and lo of its 128 rows of W^T, 64 experts at a time (a tensor map per
 // part, so that columns past E8 are zeros and not the next part's), the even CTA issues mid x hi, hi x hi and hi x lo, M = 256, N = 256.
 // The epilogue warps turn 32 tokens x 64 columns at a time into bf16 in shared memory
-// and store them as a tile while the next accumulator fills.  (221 us at 32768 tokens,
-// 256 experts, hidden 7168, 1.63 PFLOP/s of bf16 products, and 25 at 16384 tokens, 64
+// and store them as a tile while the next accumulator fills.  (221-229 us at 32768 tokens,
+// 256 experts, hidden 7168, 1.57-1.63 PFLOP/s of bf16 products, and 25 at 16384 tokens, 64
 // experts, hidden 2048.  The grouped GEMM over K = 3 E with d_hi and W_hi stored twice
 // took 295 and 36: 96 KB of operands per 64 experts where this loads 64.)
 constexpr int kDxTile = 128;                        // tokens, and rows of W^T, of a CTA
