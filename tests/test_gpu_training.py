@@ -461,3 +461,40 @@ def test_inference_mode_gives_the_same_values():
     with torch.inference_mode():
         got = (*route(x, weight, topk=4), *route_backward(*problem), *balance_loss(logits, ids))
     assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("shape", [(20000, 1032, 40, 4), (12001, 2056, 130, 4), (40000, 520, 256, 8)], ids=str)
+def test_route_backward_of_several_tiles_per_sm(shape):
+    from moe_dispatch import route_backward
+
+    problem = router_problem(*shape, seed=3)
+    check_router(problem, *route_backward(*(t.cuda() for t in problem)))
+
+
+@pytest.mark.parametrize("experts", [12, 24, 96])
+def test_route_backward_passes_32_bit_offsets(experts):
+    """x and dx of more than 2^31 elements: rows around that border, and dW of all tokens."""
+    from moe_dispatch import route_backward
+
+    tokens, hidden, topk = 300_100, 7168, 2
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(tokens, hidden, device="cuda", generator=g, dtype=torch.bfloat16)
+    _, weight, ids, weights, gw, gl = router_problem(tokens, 8, experts, topk, seed=4)
+    weight = torch.randn(experts, hidden, generator=torch.Generator().manual_seed(8)) / hidden**0.5
+    grad_x, grad_weight = route_backward(x, *(t.cuda() for t in (weight, ids, weights, gw, gl)))
+    border = 2**31 // hidden
+    rows = torch.tensor([0, 1, border - 1, border, border + 1, tokens - 1])
+    check_router((x[rows.cuda()].cpu(), weight, ids[rows], weights[rows], gw[rows], gl[rows]), grad_x[rows.cuda()], None)
+    w, u = weights.double(), gw.double()
+    ds = w * (u - (w * u).sum(-1, keepdim=True))
+    d = gl.double().scatter_add_(1, ids.long(), ds).cuda()
+    # d itself is within (topk + 4) U of |ds| and |w| sum |w u|, and topk U of its sum
+    slack = gl.double().abs().scatter_add_(1, ids.long(), ds.abs() + w * (u.abs() + (w * u).abs().sum(-1, keepdim=True))).cuda()
+    want = torch.zeros(experts, hidden, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(want)
+    for first in range(0, tokens, 50_000):
+        part = x[first:first + 50_000].double()
+        want += d[first:first + 50_000].T @ part
+        size += slack[first:first + 50_000].T @ part.abs()
+    bound = (2 * 4096 / 16 + 24 + topk + 4) * 2.0**-23 * size
+    assert bool(((grad_weight.double() - want).abs() <= bound).all())
