@@ -402,3 +402,40 @@ def test_block_refuses_ids_that_do_not_fit():
     with pytest.raises(ValueError, match="set_adapters"):
         block(x, adapter_ids=ids)
     assert block(x[:0]).shape == (0, 64)
+
+
+def test_calls_in_a_row_see_what_the_one_before_wrote():
+    """In place, ids from the device, small forms back to back: each call reads the base and the
+    ids that the kernels just before it have written, eagerly and in a graph."""
+    from moe_dispatch import adapter_add
+
+    p, _ = make_problem([40, 0, 30], 264, 1032, 5, 16, False, 12)
+    p = {k: None if v is None else v.cuda() for k, v in p.items()}
+    rounds = 8
+    ids = torch.randint(-1, 5, (rounds, 70), device="cuda", dtype=torch.int32)
+
+    def chain(row_ids, base, sync):
+        for i in range(rounds):
+            row_ids.copy_(ids[i])
+            base.mul_(0.5)
+            if sync:
+                torch.cuda.synchronize()
+            adapter_add(base, p["x"], p["a"], p["b"], row_ids, offsets=p["offsets"], scale=p["scale"], out=base)
+            if sync:
+                torch.cuda.synchronize()
+
+    want = p["base"].clone()
+    chain(torch.empty_like(ids[0]), want, True)
+    for _ in range(20):
+        got = p["base"].clone()
+        chain(torch.empty_like(ids[0]), got, False)
+        assert torch.equal(got, want)
+    row_ids, got = torch.empty_like(ids[0]), p["base"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(row_ids, got, False)
+    for _ in range(20):
+        got.copy_(p["base"])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
