@@ -10,13 +10,16 @@
 // every fp32 operand is split into bf16 parts whose sum is the value: hi =
 // bf16(v), mid = bf16(v - hi), lo = bf16(v - hi - mid), each within half a step
 // (2^-8) of the rest, so hi + mid + lo is v to 2^-24.  x is bf16 already.  dW
-// (an fp32 result) takes all three parts of d; dx (a bf16 result) takes
-// d_mid W_hi + d_hi W_hi + d_hi W_lo, which leaves out terms of 2^-16 |d W|.
+// takes all three parts of d.  dx takes the six products whose parts' ranks add up
+// to hi lo or less: what is left out (mid lo, lo mid, lo lo) is 2^-23 |d W|, as much as
+// the two splits are off, so dx is an fp32 product before its one rounding to bf16.
+// (Three products, without mid mid, hi lo and lo hi, are 2^-16 |d W| off; at 32768 tokens,
+// 256 experts, hidden 7168 the splits and dx then take 256 us and not 434.)
 //
 //   split_kernel           d's parts, [T, 3 E8] bf16 with columns lo | mid | hi (E8: E
 //                          rounded up to 8), and W^T's parts,
-//                          [H, 2 E8] bf16 with columns hi | lo
-//   router_dx_kernel       dx: tcgen05 on CTA pairs, K = E, three MMAs per 16 experts
+//                          [H, 3 E8] bf16 with columns hi | mid | lo
+//   router_dx_kernel       dx: tcgen05 on CTA pairs, K = E, six MMAs per 16 experts
 //   router_dw_kernel, router_dw_pair_kernel  dW: tcgen05 over tokens as K, both
 //                          operands MN-major; up to 80 experts, and above
 //   add_parts_kernel       adds the token ranges' partial sums in order
@@ -25,7 +28,7 @@
 // x once (router_few_kernel).
 //
 // Bound: for few experts by x and dx through memory; for 256 experts by the tensor
-// cores (6 bf16 flop per fp32 multiply-add).
+// cores (dx six bf16 products per fp32 multiply-add, dW three).
 #include "common.cuh"
 #include "launch.h"
 #include "tcgen05.cuh"
@@ -137,7 +140,7 @@ __device__ void split_gradient(const float* __restrict__ grad_logits, const int3
     }
 }
 
-// W [E, H] fp32 -> [H, 2 E8] bf16: one 32 x 32 tile through shared memory.
+// W [E, H] fp32 -> [H, 3 E8] bf16: one 32 x 32 tile through shared memory.
 __device__ void split_weight(const float* __restrict__ weight, __nv_bfloat16* __restrict__ out, int experts,
                              int padded, int64_t hidden, int64_t h0, int e0) {
     __shared__ float tile[32][33];
@@ -149,10 +152,9 @@ __device__ void split_weight(const float* __restrict__ weight, __nv_bfloat16* __
     for (int i = y; i < 32; i += 8) {
         if (h0 + i >= hidden) break;
         float v = tile[x][i];
-        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-        __nv_bfloat16* row = out + (h0 + i) * 2 * padded + e0 + x;
-        row[0] = hi;
-        row[padded] = __float2bfloat16_rn(v - __bfloat162float(hi));
+        __nv_bfloat16* row = out + (h0 + i) * 3 * padded + e0 + x;
+#pragma unroll
+        for (int part = 0; part < 3; ++part) row[part * padded] = __ushort_as_bfloat16(static_cast<unsigned short>(bf16_part(v)));
     }
 }
 
@@ -555,26 +557,32 @@ router_dw_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 
 // ----------------------------------------------------------------------- dx
 
-// dx tile [256 tokens, 256 h] on a CTA pair: each CTA loads mid and hi of its 128
-// tokens' d and hi and lo of its 128 rows of W^T, 64 experts at a time (a tensor map per
-// part, so that columns past E8 are zeros and not the next part's), the even CTA issues mid x hi, hi x hi and hi x lo, M = 256, N = 256.
+// dx tile [256 tokens, 256 h] on a CTA pair: each CTA loads the three parts of its 128
+// tokens' d and of its 128 rows of W^T, 64 experts at a time (a tensor map per part, so
+// that columns past E8 are zeros and not the next part's), the even CTA issues the six
+// products, M = 256, N = 256, the small ones of all 64 experts first: what an MMA cuts off
+// goes by the sum that it finds.
 // The epilogue warps turn 32 tokens x 64 columns at a time into bf16 in shared memory
-// and store them as a tile while the next accumulator fills.  (221-229 us at 32768 tokens,
-// 256 experts, hidden 7168, 1.57-1.63 PFLOP/s of bf16 products, and 25 at 16384 tokens, 64
-// experts, hidden 2048.  The grouped GEMM over K = 3 E with d_hi and W_hi stored twice
-// took 295 and 36: 96 KB of operands per 64 experts where this loads 64.)
+// and store them as a tile while the next accumulator fills.
+// With the splits before it 434 us at 32768 tokens, 256 experts, hidden 7168 (1.7
+// PFLOP/s of bf16 products: bound by the tensor cores), and 32 at 16384 tokens, 64
+// experts, hidden 2048 (the epilogue and its stores).
 constexpr int kDxTile = 128;                        // tokens, and rows of W^T, of a CTA
 constexpr int kDxPart = kDxTile * 128;              // bytes of one part's 64 columns
-constexpr int kDxStageBytes = 4 * kDxPart;
-constexpr int kDxStages = 3;
+constexpr int kDxStageBytes = 6 * kDxPart;
+constexpr int kDxStages = 2;
 constexpr int kDxThreads = 320;                     // producer, issuer, eight epilogue warps
 constexpr int kDxStaging = 32 * 128;                // bytes per epilogue warp
 constexpr int kDxSmem = kDxStages * kDxStageBytes + 8 * kDxStaging + 1024;
+constexpr int kDxProducts = 6;
+
+struct DxMaps {
+    CUtensorMap d[3], w[3];  // lo, mid, hi of d; hi, mid, lo of W^T
+    CUtensorMap out;
+};
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDxThreads, 1)
-router_dx_kernel(const __grid_constant__ CUtensorMap map_mid, const __grid_constant__ CUtensorMap map_hi,
-                 const __grid_constant__ CUtensorMap map_w_hi, const __grid_constant__ CUtensorMap map_w_lo,
-                 const __grid_constant__ CUtensorMap map_out, int tokens, int64_t hidden, int padded) {
+router_dx_kernel(const __grid_constant__ DxMaps maps, int tokens, int64_t hidden, int padded) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~static_cast<uintptr_t>(1023));
@@ -631,10 +639,10 @@ router_dx_kernel(const __grid_constant__ CUtensorMap map_mid, const __grid_const
                 uint8_t* at = tiles + stage * kDxStageBytes;
                 const uint32_t leader_full = map_to_cta(smem_u32(&full[stage]), 0);
                 if (leader) mbar_expect_tx(&full[stage], 2 * kDxStageBytes);
-                tma_load_2d_pair(at, &map_mid, leader_full, kb * 64, t);
-                tma_load_2d_pair(at + kDxPart, &map_hi, leader_full, kb * 64, t);
-                tma_load_2d_pair(at + 2 * kDxPart, &map_w_hi, leader_full, kb * 64, h);
-                tma_load_2d_pair(at + 3 * kDxPart, &map_w_lo, leader_full, kb * 64, h);
+                for (int part = 0; part < 3; ++part) {  // lo and W's hi first: the first product's
+                    tma_load_2d_pair(at + part * kDxPart, &maps.d[part], leader_full, kb * 64, t);
+                    tma_load_2d_pair(at + (3 + part) * kDxPart, &maps.w[part], leader_full, kb * 64, h);
+                }
                 armed |= 1u << stage;
                 parity = (parity & ~(1u << stage)) | (phase << stage);
                 if (++stage == kDxStages) {
@@ -664,15 +672,17 @@ router_dx_kernel(const __grid_constant__ CUtensorMap map_mid, const __grid_const
                 }
                 tc_fence_after();
                 const uint32_t d_at = smem_u32(tiles + stage * kDxStageBytes);
-                const uint32_t w_at = d_at + 2 * kDxPart;
+                const uint32_t w_at = d_at + 3 * kDxPart;
                 const int steps = (min(64, padded - kb * 64) + 15) / 16;  // the rest is zeros
-                for (int k = 0; k < steps; ++k) {
-                    const uint64_t mid = smem_desc_sw128(d_at + k * 32), hi = smem_desc_sw128(d_at + kDxPart + k * 32);
-                    const uint64_t w_hi = smem_desc_sw128(w_at + k * 32), w_lo = smem_desc_sw128(w_at + kDxPart + k * 32);
-                    umma_bf16_pair(tmem + acc * 256, mid, w_hi, idesc, (kb | k) != 0 ? 1u : 0u);
-                    umma_bf16_pair(tmem + acc * 256, hi, w_lo, idesc, 1u);
-                    umma_bf16_pair(tmem + acc * 256, hi, w_hi, idesc, 1u);
-                }
+                // product q: d's part (lo, mid, hi: 0, 1, 2) and W's (hi, mid, lo: 0, 1, 2)
+                constexpr int kOfD[kDxProducts] = {0, 1, 2, 1, 2, 2};
+                constexpr int kOfW[kDxProducts] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+                for (int q = 0; q < kDxProducts; ++q)
+                    for (int k = 0; k < steps; ++k)
+                        umma_bf16_pair(tmem + acc * 256, smem_desc_sw128(d_at + kOfD[q] * kDxPart + k * 32),
+                                       smem_desc_sw128(w_at + kOfW[q] * kDxPart + k * 32), idesc,
+                                       (kb | q | k) != 0 ? 1u : 0u);
                 issued = true;
                 umma_commit_pair(&empty[stage]);
                 if (++stage == kDxStages) {
@@ -728,7 +738,7 @@ router_dx_kernel(const __grid_constant__ CUtensorMap map_mid, const __grid_const
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0 && t < tokens && h + c < hidden) {
-                    tma_store_2d(&map_out, staged, h + c, t);
+                    tma_store_2d(&maps.out, staged, h + c, t);
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
             }
@@ -755,21 +765,26 @@ router_dx_kernel(const __grid_constant__ CUtensorMap map_mid, const __grid_const
 // the ring on its way out.  d's parts are made for 256 tokens at a time, a row of
 // hi | mid | lo per token; the one layout serves both products, transposed and not.
 // The sums hi and mid + lo of dW are kept apart until the end.
-// (17 us at 4096 tokens, 8 experts, hidden 4096; fp32 multiply-adds on the CUDA cores,
-// two lanes an instruction, took 24, the split products of more experts 36.)
+// (21 us with the ranges' sum at 4096 tokens, 8 experts, hidden 4096, 34 with 16 experts;
+// for 8, fp32 multiply-adds on the CUDA cores, two lanes an instruction, took 7 us more,
+// the split products of more experts 19 more.)
 constexpr int kFewExperts = 16;
 constexpr int kFewThreads = 256;
 constexpr int kFewCols = 512;     // of a CTA
 constexpr int kFewWarpCols = kFewCols / (kFewThreads / 32);
 constexpr int kFewTile = 16;      // tokens
 constexpr int kFewStages = 4;
-constexpr int kFewTokens = 256;   // of d at a time
 constexpr int kFewRow = kFewWarpCols * 2 + 16;  // bytes of a token in a warp's ring; the pad spreads the banks
 constexpr int kFewStage = kFewTile * kFewRow;
 template <int EP> constexpr int few_d_row() { return 3 * EP * 2 + (EP == 8 ? 32 : 16); }  // 80 or 112: likewise
+template <int EP> constexpr int few_tokens() { return EP == 8 ? 256 : 224; }  // of d at a time (224: two CTAs fit an SM)
+// lo of W's fragments in shared memory, not in registers: 16 experts' accumulators take 64 of the 128
+template <int EP> constexpr bool few_w_staged() { return EP == 16; }
+template <int EP> constexpr int few_w_bytes() { return few_w_staged<EP>() ? kFewThreads * (kFewWarpCols / 8) * 8 : 0; }
 template <int EP> constexpr int few_smem() {
-    return (kFewThreads / 32) * kFewStages * kFewStage + kFewTokens * few_d_row<EP>();
+    return (kFewThreads / 32) * kFewStages * kFewStage + few_tokens<EP>() * few_d_row<EP>() + few_w_bytes<EP>();
 }
+static_assert(2 * (few_smem<8>() + 1024) <= 228 * 1024 && 2 * (few_smem<16>() + 1024) <= 228 * 1024, "two CTAs an SM");
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
@@ -843,7 +858,8 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
     }
 
     // W's parts as B fragments: experts k = 2 (lane % 4) and the next (and 8 further), column lane / 4
-    uint32_t w_hi[kFrags][EP / 8], w_lo[kFrags][EP / 8];
+    uint32_t w_hi[kFrags][EP / 8], w_mid[kFrags][EP / 8], w_lo[few_w_staged<EP>() ? 1 : kFrags][EP / 8];
+    uint2* w_staged = reinterpret_cast<uint2*>(d_rows + few_tokens<EP>() * few_d_row<EP>()) + tid;  // [fragment][thread]
     if (grad_x) {
 #pragma unroll
         for (int f = 0; f < kFrags; ++f)
@@ -854,16 +870,19 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
                 float a = h < hidden && e < experts ? weight[e * hidden + h] : 0.0f;
                 float b = h < hidden && e + 1 < experts ? weight[(e + 1) * hidden + h] : 0.0f;
                 w_hi[f][g] = bf16_part(a) | bf16_part(b) << 16;
-                w_lo[f][g] = bf16_part(a) | bf16_part(b) << 16;
+                w_mid[f][g] = bf16_part(a) | bf16_part(b) << 16;
+                const uint32_t lo = bf16_part(a) | bf16_part(b) << 16;
+                if constexpr (few_w_staged<EP>()) (g ? w_staged[f * kFewThreads].y : w_staged[f * kFewThreads].x) = lo;
+                else w_lo[f][g] = lo;
             }
     }
 
     // dW: EP = 8: rows 0..7 of the fragment are hi, 8..15 mid and lo; EP = 16: one fragment each
     float acc[kFrags][EP / 8][4] = {};
     int slot = 0, load_slot = kFewStages - 1;
-    for (int batch = t0; batch < t1; batch += kFewTokens) {
+    for (int batch = t0; batch < t1; batch += few_tokens<EP>()) {
         if (batch > t0) __syncthreads();  // d of the batch before has been used
-        const int count = min(kFewTokens, t1 - batch);
+        const int count = min(few_tokens<EP>(), t1 - batch);
         for (int i = tid; i < (count + kFewTile - 1) / kFewTile * kFewTile; i += kFewThreads) {
             float d[EP];
 #pragma unroll
@@ -938,19 +957,26 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
                 }
                 if (grad_x) {
                     // A = d: {tokens 0-7, tokens 8-15} x {k 0-7, k 8-15}
-                    uint32_t hi[4], mid[4];
+                    uint32_t hi[4], mid[4], lo[4];
                     const uint32_t at_d = at + (m & 1) * 8 * few_d_row<EP>() + (m >> 1) * 16;
-                    ldmatrix4(at_d, hi);  // EP 8: hi, mid; EP 16: hi
-                    if constexpr (EP == 16) ldmatrix4(at_d + 2 * EP, mid);
+                    ldmatrix4(at_d, hi);           // EP 8: hi, mid; EP 16: hi
+                    ldmatrix4(at_d + 2 * EP, mid);  // EP 8: mid, lo; EP 16: mid
+                    if constexpr (EP == 16) ldmatrix4(at_d + 4 * EP, lo);
                     __syncwarp();  // x of these tokens has been read: dx may take its place
 #pragma unroll
                     for (int f = 0; f < kFrags; ++f) {
                         float c[4];
+                        // the six products, small ones first
                         if constexpr (EP == 8) {
-                            mma_k16_first(c, hi[0], hi[1], 0, 0, w_lo[f][0], 0);
+                            mma_k16_first(c, hi[0], hi[1], mid[2], mid[3], w_lo[f][0], w_hi[f][0]);
+                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_mid[f][0], w_mid[f][0]);
                             mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_hi[f][0], w_hi[f][0]);
                         } else {
-                            mma_k16_first(c, hi[0], hi[1], hi[2], hi[3], w_lo[f][0], w_lo[f][1]);
+                            const uint2 w = w_staged[f * kFewThreads];
+                            mma_k16_first(c, hi[0], hi[1], hi[2], hi[3], w.x, w.y);
+                            mma_k16(c, mid[0], mid[1], mid[2], mid[3], w_mid[f][0], w_mid[f][1]);
+                            mma_k16(c, lo[0], lo[1], lo[2], lo[3], w_hi[f][0], w_hi[f][1]);
+                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_mid[f][0], w_mid[f][1]);
                             mma_k16(c, mid[0], mid[1], mid[2], mid[3], w_hi[f][0], w_hi[f][1]);
                             mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_hi[f][0], w_hi[f][1]);
                         }
@@ -1104,7 +1130,7 @@ Layout layout(int64_t tokens, int64_t hidden, int experts, bool dx, bool dw, int
     }
     l.parts = 0;
     l.weight = round256(tokens * 3 * e8 * 2);
-    l.sums = l.weight + (dx ? round256(hidden * 2 * e8 * 2) : 0);
+    l.sums = l.weight + (dx ? round256(hidden * 3 * e8 * 2) : 0);
     const int ranges = token_ranges(tokens, hidden, experts, sms);
     l.total = l.sums + (dw && ranges > 1 ? round256(ranges * experts * hidden * 4) : 0);
     return l;
@@ -1200,12 +1226,12 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
     MOE_CUDA_TRY(cudaGetDevice(&device));
     const char* rejected = "cuTensorMapEncodeTiled rejected an operand (pointer alignment or shape)";
     if (grad_x) {
-        CUtensorMap map_mid, map_hi, map_w_hi, map_w_lo, map_out;
-        if (!encode_bf16_tensor_map(&map_mid, parts + e8, tokens, e8, 3 * e8, kDxTile) ||
-            !encode_bf16_tensor_map(&map_hi, parts + 2 * e8, tokens, e8, 3 * e8, kDxTile) ||
-            !encode_bf16_tensor_map(&map_w_hi, wt, hidden, e8, 2 * e8, kDxTile) ||
-            !encode_bf16_tensor_map(&map_w_lo, wt + e8, hidden, e8, 2 * e8, kDxTile) ||
-            !encode_bf16_tensor_map(&map_out, grad_x, tokens, hidden, 0, 32)) {
+        DxMaps maps;
+        bool encoded = encode_bf16_tensor_map(&maps.out, grad_x, tokens, hidden, 0, 32);
+        for (int part = 0; part < 3; ++part)
+            encoded = encoded && encode_bf16_tensor_map(&maps.d[part], parts + part * e8, tokens, e8, 3 * e8, kDxTile) &&
+                      encode_bf16_tensor_map(&maps.w[part], wt + part * e8, hidden, e8, 3 * e8, kDxTile);
+        if (!encoded) {
             *error = rejected;
             return cudaErrorInvalidValue;
         }
@@ -1217,8 +1243,7 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
         const int64_t pairs = ((tokens + 2 * kDxTile - 1) / (2 * kDxTile)) * ((hidden + 2 * kDxTile - 1) / (2 * kDxTile));
         const int64_t ctas = 2 * (pairs < sms / 2 ? pairs : sms / 2);
         MOE_CUDA_TRY(launch_dependent(router_dx_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kDxThreads), kDxSmem,
-                                      stream, map_mid, map_hi, map_w_hi, map_w_lo, map_out, static_cast<int>(tokens),
-                                      hidden, e8));
+                                      stream, maps, static_cast<int>(tokens), hidden, e8));
     }
     if (grad_weight) {
         DwParams p;

@@ -100,9 +100,9 @@ int moe_balance_loss_backward(const void* logits, int32_t dtype, const float* bi
  *             a repeated id adds each time)
  *   grad_x [tokens, hidden] bf16 = d . router_weight  (rounded once; NULL: not computed)
  *   grad_router_weight [experts, hidden] fp32 = d^T . x  (written; NULL: not computed)
- * on the tensor cores with d and the weight split into bf16 parts: d enters
- * grad_router_weight to 2^-24, and the products of grad_x are good to 2^-16 of
- * their size.
+ * on the tensor cores with d and the weight split into three bf16 parts each, to
+ * fp32 accuracy: both are their parts' sum to 2^-24, and what the products of
+ * grad_x leave out is 2^-23 of their size.
  * Gradients that are not finite (or above 3.38e38) give results that are not
  * finite.  Fixed
  * summation order.  hidden % 8 == 0; x, router_weight and their gradients 16-byte
