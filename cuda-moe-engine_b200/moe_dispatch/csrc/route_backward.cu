@@ -187,6 +187,13 @@ constexpr int kTileT = 64;
 constexpr int kBlock = kTileT * 128;  // bytes of 64 columns x kTileT tokens
 constexpr int kMaxStages = 8;
 constexpr int kDwThreads = 192;  // producer, issuer, four epilogue warps
+// The tensor cores cut the sum of 16 products and the accumulator off below its last
+// bit, so long sums drift: with 500 MMAs into one accumulator dW of 32768 tokens, 256
+// experts was 6.7e-6 of its norm off, where plain fp32 products are 5.8e-7 off.  So in
+// every dW kernel an accumulator takes kChunk tokens (16 MMAs per part of d), and is then
+// added to an fp32 sum, rounded to nearest.
+constexpr int kChunk = 256;
+constexpr int kChunkSteps = kChunk / kTileT;
 constexpr int kDwSmem = 224 * 1024;
 
 struct DwParams {
@@ -196,9 +203,13 @@ struct DwParams {
     int range;            // tokens per CTA or CTA pair (a multiple of kTileT)
     int n;                // MMA N
     int blocks;           // 64-column boxes of d per stage (pair: per part and CTA)
-    int tmem_cols;
     int stages;
 };
+
+// Up to this many (padded) experts d's parts fit side by side into one MMA.
+constexpr int kSideBySide = 80;
+constexpr int kSideBySide32 = (kSideBySide + 31) / 32 * 32;  // read 32 columns at a time
+static_assert(2 * kSideBySide + kSideBySide32 <= 256, "the last part's columns lie in its accumulator");
 
 __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                              uint64_t limit) {
@@ -228,17 +239,17 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
 
 // dW^T tile [128 h, E] of one range of tokens, up to 80 experts.  Warp 0 loads x
 // [64 tokens, 128] and d's parts by TMA, warp 1 issues the MMAs (M = 128, K = 16),
-// warps 2-5 store the tile.  The three parts stand side by side in N (3 E8 <= 240):
-// one MMA per 16 tokens, and the epilogue adds the three column groups.  A CTA's
-// range bounds the additions in one accumulator (at most 2048 tokens, see the pair
-// kernel on why); ranges are added in a launch of their own.
+// warps 2-5 add the accumulators into registers (two accumulators in turn, 256 columns of
+// tensor memory each; a thread has all experts of one row) and store the tile.  The three
+// parts stand side by side in N (3 E8 <= 240): one MMA per 16 tokens, and the epilogue
+// adds the three column groups.  Ranges are added in a launch of their own.
 __global__ void __launch_bounds__(kDwThreads, 1)
 router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_d,
                  const DwParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -246,6 +257,7 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const int t0 = blockIdx.y * p.range;
     const int t1 = min(t0 + p.range, p.tokens);
     const int steps = (t1 - t0 + kTileT - 1) / kTileT;  // >= 1
+    const int chunks = (steps + kChunkSteps - 1) / kChunkSteps;
     const int stage_bytes = (2 + p.blocks) * kBlock;
 
     pdl_trigger();
@@ -254,7 +266,10 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(&done, 1);
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&acc_full[a], 1);
+            mbar_init(&acc_empty[a], kDwThreads - 64);  // the epilogue's threads
+        }
         mbar_init(&drain, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -262,7 +277,7 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&tmem_slot)),
-                     "r"(p.tmem_cols));
+                     "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     pdl_wait();
@@ -300,65 +315,81 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         const uint32_t idesc = make_idesc(kTileH, p.n) | (1u << 15) | (1u << 16);  // both MN-major
         int stage = 0;
         uint32_t phase = 0;
-        bool issued = false;
-        for (int i = 0; i < steps; ++i) {
-            if (!wait_bounded(&full[stage], phase, &abort_flag, kWaitLimitNs)) break;
+        bool issued = false, ok = true;
+        for (int chunk = 0; chunk < chunks && ok; ++chunk) {
+            const int acc = chunk & 1;
+            if (!wait_bounded(&acc_empty[acc], ((chunk >> 1) & 1) ^ 1u, &abort_flag, kWaitLimitNs)) break;
             tc_fence_after();
-            const uint32_t x_at = smem_u32(tiles + stage * stage_bytes);
-            const uint32_t d_at = x_at + 2 * kBlock;
-            for (int k = 0; k < kTileT / 16; ++k)
-                umma_bf16(tmem, mn_desc(x_at + k * 2048), mn_desc(d_at + k * 2048), idesc, (i | k) != 0 ? 1u : 0u);
-            issued = true;
-            umma_commit(&empty[stage]);
-            if (++stage == p.stages) {
-                stage = 0;
-                phase ^= 1u;
+            const int here = min(kChunkSteps, steps - chunk * kChunkSteps);
+            for (int i = 0; i < here; ++i) {
+                if (!wait_bounded(&full[stage], phase, &abort_flag, kWaitLimitNs)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t x_at = smem_u32(tiles + stage * stage_bytes);
+                const uint32_t d_at = x_at + 2 * kBlock;
+                for (int k = 0; k < kTileT / 16; ++k)
+                    umma_bf16(tmem + acc * 256, mn_desc(x_at + k * 2048), mn_desc(d_at + k * 2048), idesc,
+                              (i | k) != 0 ? 1u : 0u);
+                issued = true;
+                umma_commit(&empty[stage]);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
+            if (ok) umma_commit(&acc_full[acc]);
         }
-        if (!abort_flag) {
-            umma_commit(&done);
-            volatile int never = 0;  // whatever the epilogue does, no MMA outlives this wait
-            wait_bounded(&done, 0, &never, kWaitLimitNs);
-        } else if (issued) {  // MMAs in flight end before the tensor memory is freed
+        if (issued) {  // no MMA outlives this wait, whatever the epilogue does
             umma_commit(&drain);
             volatile int never = 0;
-            wait_bounded(&drain, 0, &never, kDrainLimitNs);
+            wait_bounded(&drain, 0, &never, kWaitLimitNs);
         }
     } else if (warp >= 2) {
         // TMEM lane = row of the tile (h), column = expert: a warp stores 32 neighbours of one
         // expert's row.  Lanes past H (only in the last tile) store nothing.
-        if (wait_bounded(&done, 0, &abort_flag, 2 * kWaitLimitNs)) {
-            tc_fence_after();
-            const int quarter = warp & 3;
-            const int64_t h = h0 + quarter * 32 + lane;
-            const uint32_t row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-            float* out = p.out + static_cast<int64_t>(blockIdx.y) * p.experts * p.hidden + h;
-            for (int c = 0; c < p.experts; c += 32) {
-                uint32_t v[32];
-                float sum[32];
-                tmem_ld32(row + c, v);
-                tmem_wait_ld();
+        const int quarter = warp & 3;
+        const int64_t h = h0 + quarter * 32 + lane;
+        const uint32_t row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        float sum[kSideBySide32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) sum[j] = __uint_as_float(v[j]);
-                for (int s = 1; s < 3; ++s) {  // the small parts first: lo + mid + hi
-                    tmem_ld32(row + s * p.padded + c, v);
+        for (int j = 0; j < kSideBySide32; ++j) sum[j] = 0.0f;
+        bool ok = true;
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            const int acc = chunk & 1;
+            if (!wait_bounded(&acc_full[acc], (chunk >> 1) & 1, &abort_flag, kWaitLimitNs)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kSideBySide32; c += 32) {
+                if (c < p.experts) {
+                    uint32_t v[3][32];
+#pragma unroll
+                    for (int s = 0; s < 3; ++s) tmem_ld32(row + acc * 256 + s * p.padded + c, v[s]);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(v[j]);
-                }
-                if (h < p.hidden) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c + j < p.experts) out[(c + j) * p.hidden] = sum[j];
+                    for (int j = 0; j < 32; ++j)  // the small parts first: lo + mid + hi
+                        sum[c + j] += (__uint_as_float(v[0][j]) + __uint_as_float(v[1][j])) + __uint_as_float(v[2][j]);
                 }
             }
             tc_fence_before();
+            mbar_arrive(&acc_empty[acc]);
+        }
+        if (ok && h < p.hidden) {
+            float* out = p.out + static_cast<int64_t>(blockIdx.y) * p.experts * p.hidden + h;
+#pragma unroll
+            for (int j = 0; j < kSideBySide32; ++j)
+                if (j < p.experts) out[j * p.hidden] = sum[j];
         }
     }
+    tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
@@ -368,16 +399,10 @@ router_dw_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 // tokens.  (One CTA with M = 128 needs 112 KB per 64 tokens and SM instead of 64: 451 us
 // at 32768 tokens, 256 experts, hidden 7168 against 283 for the pair, both with stages of
 // 32 tokens.)
-//
-// The tensor cores cut the sum of 16 products and the accumulator off below its last
-// bit, so long sums drift: with 500 MMAs into one accumulator dW was
-// 6.7e-6 of its norm off at this size, where plain fp32 products are 5.8e-7 off.  Here
-// an accumulator takes kChunk tokens (48 MMAs); meanwhile the epilogue warps add the
-// one before into fp32 registers, 128 columns of one row per thread.
+// While an accumulator takes its kChunk tokens (48 MMAs) the epilogue warps add the
+// one before into fp32 registers, 128 columns of one row per thread (7.4e-7 of dW's norm).
 constexpr int kPairThreads = 320;  // producer, issuer, eight epilogue warps
-constexpr int kChunk = 256;
 constexpr int kPairStages = 3;
-constexpr int kChunkSteps = kChunk / kTileT;
 
 __device__ __forceinline__ bool wait_bounded_cluster(uint64_t* bar, uint32_t parity,
                                                      volatile int* abort_flag, uint64_t limit) {
@@ -764,8 +789,10 @@ router_dx_kernel(const __grid_constant__ DxMaps maps, int tokens, int64_t hidden
 // parts of d, N = columns, against W's parts in registers), which takes x's place in
 // the ring on its way out.  d's parts are made for 256 tokens at a time, a row of
 // hi | mid | lo per token; the one layout serves both products, transposed and not.
-// The sums hi and mid + lo of dW are kept apart until the end.
-// (21 us with the ranges' sum at 4096 tokens, 8 experts, hidden 4096, 34 with 16 experts;
+// The sums hi and mid + lo of dW are kept apart; after every batch of d (256 tokens at most,
+// see kChunk) they are added to this CTA's fp32 sums in memory, each by the thread that
+// wrote it before, and start again from zero.
+// (21 us with the ranges' sum at 4096 tokens, 8 experts, hidden 4096, 28 with 16 experts;
 // for 8, fp32 multiply-adds on the CUDA cores, two lanes an instruction, took 7 us more,
 // the split products of more experts 19 more.)
 constexpr int kFewExperts = 16;
@@ -773,14 +800,14 @@ constexpr int kFewThreads = 256;
 constexpr int kFewCols = 512;     // of a CTA
 constexpr int kFewWarpCols = kFewCols / (kFewThreads / 32);
 constexpr int kFewTile = 16;      // tokens
-constexpr int kFewStages = 4;
+constexpr int kFewStages = 3;
 constexpr int kFewRow = kFewWarpCols * 2 + 16;  // bytes of a token in a warp's ring; the pad spreads the banks
 constexpr int kFewStage = kFewTile * kFewRow;
 template <int EP> constexpr int few_d_row() { return 3 * EP * 2 + (EP == 8 ? 32 : 16); }  // 80 or 112: likewise
 template <int EP> constexpr int few_tokens() { return EP == 8 ? 256 : 224; }  // of d at a time (224: two CTAs fit an SM)
-// lo of W's fragments in shared memory, not in registers: 16 experts' accumulators take 64 of the 128
-template <int EP> constexpr bool few_w_staged() { return EP == 16; }
-template <int EP> constexpr int few_w_bytes() { return few_w_staged<EP>() ? kFewThreads * (kFewWarpCols / 8) * 8 : 0; }
+static_assert(few_tokens<8>() <= kChunk && few_tokens<16>() <= kChunk, "dW's accumulators are emptied after each");
+// mid and lo of W's fragments wait in shared memory: of the 128 registers 16 experts' accumulators take 64
+template <int EP> constexpr int few_w_bytes() { return kFewThreads * (kFewWarpCols / 8) * EP; }
 template <int EP> constexpr int few_smem() {
     return (kFewThreads / 32) * kFewStages * kFewStage + few_tokens<EP>() * few_d_row<EP>() + few_w_bytes<EP>();
 }
@@ -858,8 +885,9 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
     }
 
     // W's parts as B fragments: experts k = 2 (lane % 4) and the next (and 8 further), column lane / 4
-    uint32_t w_hi[kFrags][EP / 8], w_mid[kFrags][EP / 8], w_lo[few_w_staged<EP>() ? 1 : kFrags][EP / 8];
-    uint2* w_staged = reinterpret_cast<uint2*>(d_rows + few_tokens<EP>() * few_d_row<EP>()) + tid;  // [fragment][thread]
+    uint32_t w_hi[kFrags][EP / 8];
+    struct alignas(EP) Staged { uint32_t mid[EP / 8], lo[EP / 8]; };
+    Staged* w_staged = reinterpret_cast<Staged*>(d_rows + few_tokens<EP>() * few_d_row<EP>()) + tid;  // [fragment][thread]
     if (grad_x) {
 #pragma unroll
         for (int f = 0; f < kFrags; ++f)
@@ -870,10 +898,8 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
                 float a = h < hidden && e < experts ? weight[e * hidden + h] : 0.0f;
                 float b = h < hidden && e + 1 < experts ? weight[(e + 1) * hidden + h] : 0.0f;
                 w_hi[f][g] = bf16_part(a) | bf16_part(b) << 16;
-                w_mid[f][g] = bf16_part(a) | bf16_part(b) << 16;
-                const uint32_t lo = bf16_part(a) | bf16_part(b) << 16;
-                if constexpr (few_w_staged<EP>()) (g ? w_staged[f * kFewThreads].y : w_staged[f * kFewThreads].x) = lo;
-                else w_lo[f][g] = lo;
+                w_staged[f * kFewThreads].mid[g] = bf16_part(a) | bf16_part(b) << 16;
+                w_staged[f * kFewThreads].lo[g] = bf16_part(a) | bf16_part(b) << 16;
             }
     }
 
@@ -967,16 +993,16 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
                     for (int f = 0; f < kFrags; ++f) {
                         float c[4];
                         // the six products, small ones first
+                        const Staged w = w_staged[f * kFewThreads];
                         if constexpr (EP == 8) {
-                            mma_k16_first(c, hi[0], hi[1], mid[2], mid[3], w_lo[f][0], w_hi[f][0]);
-                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_mid[f][0], w_mid[f][0]);
+                            mma_k16_first(c, hi[0], hi[1], mid[2], mid[3], w.lo[0], w_hi[f][0]);
+                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w.mid[0], w.mid[0]);
                             mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_hi[f][0], w_hi[f][0]);
                         } else {
-                            const uint2 w = w_staged[f * kFewThreads];
-                            mma_k16_first(c, hi[0], hi[1], hi[2], hi[3], w.x, w.y);
-                            mma_k16(c, mid[0], mid[1], mid[2], mid[3], w_mid[f][0], w_mid[f][1]);
+                            mma_k16_first(c, hi[0], hi[1], hi[2], hi[3], w.lo[0], w.lo[1]);
+                            mma_k16(c, mid[0], mid[1], mid[2], mid[3], w.mid[0], w.mid[1]);
                             mma_k16(c, lo[0], lo[1], lo[2], lo[3], w_hi[f][0], w_hi[f][1]);
-                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_mid[f][0], w_mid[f][1]);
+                            mma_k16(c, hi[0], hi[1], hi[2], hi[3], w.mid[0], w.mid[1]);
                             mma_k16(c, mid[0], mid[1], mid[2], mid[3], w_hi[f][0], w_hi[f][1]);
                             mma_k16(c, hi[0], hi[1], hi[2], hi[3], w_hi[f][0], w_hi[f][1]);
                         }
@@ -1002,28 +1028,33 @@ router_few_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__
             if (++slot == kFewStages) slot = 0;
             if (++load_slot == kFewStages) load_slot = 0;
         }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (!active || !sums) return;
+        if (sums) {
+            float* at = sums + (static_cast<int64_t>(blockIdx.y) * experts + (lane >> 2)) * hidden + h0 + 2 * (lane & 3);
 #pragma unroll
-    for (int f = 0; f < kFrags; ++f) {
-        const int64_t h = h0 + f * 8 + 2 * (lane & 3);
-        if (h >= hidden) continue;
-        float* at = sums + static_cast<int64_t>(blockIdx.y) * experts * hidden + h;
-        const int e = lane >> 2;
-        if constexpr (EP == 8) {  // expert e: rows e and e + 8
-            if (e < experts)
-                *reinterpret_cast<float2*>(at + e * hidden) =
-                    make_float2(acc[f][0][0] + acc[f][0][2], acc[f][0][1] + acc[f][0][3]);
-        } else {
-            if (e < experts)
-                *reinterpret_cast<float2*>(at + e * hidden) =
-                    make_float2(acc[f][0][0] + acc[f][1][0], acc[f][0][1] + acc[f][1][1]);
-            if (e + 8 < experts)
-                *reinterpret_cast<float2*>(at + (e + 8) * hidden) =
-                    make_float2(acc[f][0][2] + acc[f][1][2], acc[f][0][3] + acc[f][1][3]);
+            for (int g = 0; g < EP / 8; ++g, at += 8 * hidden) {
+                const int e = g * 8 + (lane >> 2);
+                const auto here = [&](int f) { return e < experts && h0 + f * 8 < hidden; };  // 8 divides hidden
+                float2 before[kFrags];  // all on their way before the first is used
+#pragma unroll
+                for (int f = 0; f < kFrags; ++f)
+                    before[f] = batch > t0 && here(f) ? *reinterpret_cast<const float2*>(at + f * 8) : make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int f = 0; f < kFrags; ++f) {
+                    // expert e: EP 8: rows e and e + 8; EP 16: the same row of both fragments
+                    const float a = EP == 8 ? acc[f][0][0] + acc[f][0][2] : acc[f][0][2 * g] + acc[f][EP / 8 - 1][2 * g];
+                    const float b = EP == 8 ? acc[f][0][1] + acc[f][0][3] : acc[f][0][2 * g + 1] + acc[f][EP / 8 - 1][2 * g + 1];
+                    if (here(f)) *reinterpret_cast<float2*>(at + f * 8) = make_float2(before[f].x + a, before[f].y + b);
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+                for (int g = 0; g < EP / 8; ++g)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[f][g][j] = 0.0f;
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // out = the parts' sum, in a fixed order: SLICES threads per vector add a stretch of
@@ -1068,28 +1099,24 @@ add_parts_kernel(const float4* __restrict__ parts, float4* __restrict__ out, int
 
 int pad8(int experts) { return (experts + 7) / 8 * 8; }
 
-// Up to this many (padded) experts d's parts fit side by side into one MMA.
-constexpr int kSideBySide = 80;
-
 // Ranges of tokens for dW: those that take the least time, as waves of CTAs (or
 // pairs) over the SMs, each as long as its tokens and a start of about 64, plus the
 // partial sums' way through memory.  A token costs an SM of the first kernel about
 // 6 ns (x read at the memory's rate), a pair of the second 12.6 ns at N = 256 (6
 // MMAs of 128 cycles per 32 tokens); the partial sums of a range cost
 // 8 E H bytes at 6500 bytes/ns.
-constexpr int64_t kMinRange = 256, kMaxRange = 2048;
+constexpr int64_t kMinRange = 256;
 int token_ranges(int64_t tokens, int64_t hidden, int experts, int sms) {
     const bool pair = pad8(experts) > kSideBySide;
     const int64_t tiles = pair ? (hidden + 2 * kTileH - 1) / (2 * kTileH) : (hidden + kTileH - 1) / kTileH;
     const int64_t slots = pair ? sms / 2 : sms;
     const double token_ns = pair ? 12.6 * experts / 256 : 6.0;
     const double part_tokens = 8.0 * experts * hidden / 6500.0 / token_ns;
-    const int64_t least = pair ? 1 : (tokens + kMaxRange - 1) / kMaxRange;
     int64_t most = (tokens + kMinRange - 1) / kMinRange;
-    if (most > least + 31) most = least + 31;
-    int64_t best = least;
+    if (most > 32) most = 32;
+    int64_t best = 1;
     double best_time = 1e30;
-    for (int64_t r = least; r <= most; ++r) {
+    for (int64_t r = 1; r <= most; ++r) {
         const double waves = static_cast<double>((tiles * r + slots - 1) / slots);
         const double time = waves * (static_cast<double>(tokens) / r + 64.0) + (r > 1 ? r * part_tokens : 0.0);
         if (time < best_time) {
@@ -1255,15 +1282,10 @@ cudaError_t launch_route_backward(const void* x, const float* weight, const int3
         if (pair) {
             p.n = (experts + 63) / 64 * 64;
             p.blocks = (p.n / 2 + 63) / 64;
-            p.tmem_cols = 512;
             p.stages = kPairStages;
         } else {
             p.n = (3 * e8 + 15) / 16 * 16;
             p.blocks = (3 * e8 + 63) / 64;
-            // the epilogue reads 32 columns at a time from each column group
-            const int reach = 2 * e8 + (e8 + 31) / 32 * 32;
-            p.tmem_cols = 32;
-            while (p.tmem_cols < (reach > p.n ? reach : p.n)) p.tmem_cols *= 2;
             const int fit = kDwSmem / ((2 + p.blocks) * kBlock);
             p.stages = fit < kMaxStages ? fit : kMaxStages;
         }
