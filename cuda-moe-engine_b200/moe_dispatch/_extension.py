@@ -172,6 +172,7 @@ class Extension:
             self._scratch_sizes[key] = size
         scratch = torch.empty(size or 1, dtype=torch.uint8, device=device)
         self._run(function(*args, scratch.data_ptr(), size, _stream(index)))
+        return scratch
 
     def scratch_bytes(self, tokens, topk, experts):
         return int(self.lib.moe_dispatch_scratch_bytes(tokens, topk, experts))
@@ -372,9 +373,10 @@ class Extension:
         self.launch_balance_loss(logits, ids, bias, token_mask, coefficient, loss, counts, counted)
 
     def launch_balance_loss(self, logits, ids, bias, token_mask, coefficient, loss, counts, counted):
-        """balance_loss_out without its tensor checks (callers have made them)."""
+        """balance_loss_out without its tensor checks (callers have made them).  Returns the scratch,
+        which begins with counts[E] and the counted tokens once more."""
         tokens, experts = logits.shape
-        self._call_with_scratch(
+        return self._call_with_scratch(
             logits.device, "moe_balance_loss_scratch_bytes", (experts,),
             self.lib.moe_balance_loss,
             logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), ids.data_ptr(),
@@ -393,18 +395,18 @@ class Extension:
                  "expected int32 counts[E] and counted[1]")
         _require(grad_loss.numel() == 1 and grad_loss.dtype == torch.float32,
                  "expected one FP32 grad_loss")
-        self.launch_balance_loss_backward(logits, bias, token_mask, counts, counted, grad_loss,
-                                          coefficient, topk, grad_logits)
+        self.launch_balance_loss_backward(logits, bias, token_mask, counts.data_ptr(),
+                                          counted.data_ptr(), grad_loss, coefficient, topk, grad_logits)
 
     def launch_balance_loss_backward(self, logits, bias, token_mask, counts, counted, grad_loss,
                                      coefficient, topk, grad_logits):
-        """balance_loss_backward_out without its tensor checks."""
+        """balance_loss_backward_out without its tensor checks; counts and counted are addresses."""
         tokens, experts = logits.shape
         self._call(
             logits.device, self.lib.moe_balance_loss_backward,
             logits.data_ptr(), _DTYPE_CODES[logits.dtype], _ptr(bias), _ptr(token_mask),
-            counts.data_ptr(), counted.data_ptr(), grad_loss.data_ptr(), coefficient,
-            grad_logits.data_ptr(), tokens, experts, topk,
+            counts, counted, grad_loss.data_ptr(), coefficient, grad_logits.data_ptr(), tokens,
+            experts, topk,
         )
 
     def route_backward_out(self, x, router_weight, ids, weights, grad_weights, grad_logits, grad_x,

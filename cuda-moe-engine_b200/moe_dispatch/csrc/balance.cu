@@ -191,11 +191,12 @@ __device__ __forceinline__ void cluster_barrier() {
 
 // One cluster (of one CTA for few parts): every CTA adds a stretch of the parts in
 // order, the first adds the CTAs' sums in order from their shared memory and writes
-// counts[E], counted[0] = V and the loss.
+// counts[E], counted[0] = V, both once more into kept, and the loss.
 __global__ void __launch_bounds__(kFinishThreads)
 balance_finish_kernel(const float* __restrict__ sums, const int32_t* __restrict__ part_counts,
                       int parts, int experts, int topk, float coefficient, float* __restrict__ loss,
-                      int32_t* __restrict__ counts, int32_t* __restrict__ counted) {
+                      int32_t* __restrict__ counts, int32_t* __restrict__ counted,
+                      int32_t* __restrict__ kept) {
     constexpr int kMax = kFinishThreads;
     __shared__ float s_sum[kMax];
     __shared__ int32_t s_count[kMax];
@@ -235,6 +236,7 @@ balance_finish_kernel(const float* __restrict__ sums, const int32_t* __restrict_
                 total += __uint_as_float(load_peer(&s_sum[e], c));
                 count += static_cast<int32_t>(load_peer(&s_count[e], c));
             }
+            kept[e] = count;
             if (e < experts) counts[e] = count;
             else {
                 counted[0] = count;
@@ -327,6 +329,10 @@ cudaError_t sm_count(int* sms) {
     return cudaSuccess;
 }
 
+// The scratch: counts and V once more for the backward pass (the caller may change its
+// counts before that), then the CTAs' sums and counts.
+int64_t kept_bytes(int experts) { return (4 * (experts + 1) + 15) / 16 * 16; }
+
 // CTAs of the forward pass: two per SM at most (each costs the finishing launch a
 // row to add), at least one token per group of lanes each.
 constexpr int kMaxParts = 512;
@@ -359,7 +365,8 @@ cudaError_t forward(const BalanceArgs& a) {
     MOE_CUDA_TRY(sm_count(&sms));
     const int parts = balance_parts(a.tokens, G, sms);
     const int64_t per_cta = (a.tokens + parts - 1) / parts;
-    float* sums = static_cast<float*>(a.scratch);
+    int32_t* kept = static_cast<int32_t*>(a.scratch);
+    float* sums = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kept_bytes(a.experts));
     int32_t* part_counts = reinterpret_cast<int32_t*>(sums + static_cast<int64_t>(kMaxParts) * a.experts);
     MOE_CUDA_TRY(launch_dependent(balance_forward_kernel<DT, G, VPL, VEC>, dim3(parts), dim3(kThreads), 0,
                                   a.stream, static_cast<const T*>(a.logits), a.bias, a.ids, a.mask,
@@ -381,7 +388,7 @@ cudaError_t forward(const BalanceArgs& a) {
     config.numAttrs = 2;
     return cudaLaunchKernelEx(&config, balance_finish_kernel, static_cast<const float*>(sums),
                               static_cast<const int32_t*>(part_counts), parts, a.experts, a.topk,
-                              a.coefficient, a.loss, a.counts, a.counted);
+                              a.coefficient, a.loss, a.counts, a.counted, kept);
 }
 
 template <int DT, int G, int VPL, int VEC>
@@ -433,7 +440,7 @@ cudaError_t by_dtype(int dtype, const BalanceArgs& a) {
 }  // namespace
 
 int64_t balance_scratch_bytes(int experts) {
-    return static_cast<int64_t>(kMaxParts) * (2 * experts + 1) * 4;
+    return kept_bytes(experts) + static_cast<int64_t>(kMaxParts) * (2 * experts + 1) * 4;
 }
 
 cudaError_t launch_balance_loss(const void* logits, int dtype, const float* bias,

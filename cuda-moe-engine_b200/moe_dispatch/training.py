@@ -61,11 +61,13 @@ class _BalanceLoss(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=logits.device)
         counts = torch.empty(experts, dtype=torch.int32, device=logits.device)
         counted = torch.empty(1, dtype=torch.int32, device=logits.device)
-        extension.launch_balance_loss(logits, expert_ids, bias, token_mask, coefficient, loss, counts,
-                                      counted)
+        # kept begins with counts and counted: the caller may sum its own counts over ranks in
+        # place before the backward pass
+        kept = extension.launch_balance_loss(logits, expert_ids, bias, token_mask, coefficient, loss,
+                                             counts, counted)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, bias, token_mask, counts, counted)
+        ctx.save_for_backward(logits, bias, token_mask, kept)
         ctx.coefficient, ctx.topk = coefficient, expert_ids.shape[1]
         return loss, counts
 
@@ -74,11 +76,12 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         if grad_loss is None or not ctx.needs_input_grad[0]:
             return None, None, None, None, None
-        logits, bias, token_mask, counts, counted = ctx.saved_tensors
+        logits, bias, token_mask, kept = ctx.saved_tensors
         grad = torch.empty_like(logits)
+        counts = kept.data_ptr()
         get_extension().launch_balance_loss_backward(
-            logits, bias, token_mask, counts, counted, grad_loss.contiguous(), ctx.coefficient,
-            ctx.topk, grad)
+            logits, bias, token_mask, counts, counts + 4 * logits.shape[1], grad_loss.contiguous(),
+            ctx.coefficient, ctx.topk, grad)
         return grad, None, None, None, None
 
 
@@ -96,7 +99,7 @@ def balance_loss(logits, expert_ids, *, bias=None, token_mask=None, coefficient=
 
     which is ``coefficient`` when every expert gets its share.  Returns the fp32
     scalar loss, differentiable in ``logits`` (f is a constant), and counts [E]
-    int32.  Ids outside 0..E-1 (dropped assignments) count for nothing; without
+    int32, the caller's own: what is written there does not change the gradient.  Ids outside 0..E-1 (dropped assignments) count for nothing; without
     a token that counts the loss is 0.
     """
     if logits.ndim != 2:

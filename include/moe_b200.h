@@ -75,7 +75,9 @@ int moe_route(const void* x_bf16, const float* router_weight, const float* bias,
  * number V) are device memory.  V = 0 gives loss 0.  A row whose scores are
  * all -inf has p = 0.  Sums in fp32 in a fixed order: same bits on every run.
  * scratch: moe_balance_loss_scratch_bytes(experts), 16-byte aligned, not
- * initialised; calls that may overlap in time need one each. */
+ * initialised; calls that may overlap in time need one each.  Afterwards it begins
+ * with the int32 counts[experts] and V once more: who changes counts before the
+ * backward pass (a sum over ranks) keeps the scratch and gives that pass these. */
 int64_t moe_balance_loss_scratch_bytes(int32_t experts);
 int moe_balance_loss(const void* logits, int32_t dtype, const float* bias, const int32_t* ids,
                      const uint8_t* token_mask, float coefficient, float* loss, int32_t* counts,
