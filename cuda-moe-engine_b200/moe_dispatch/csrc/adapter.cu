@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(256) expand_rows_kernel(const Adapter p) {
             }
 #pragma unroll
             for (int off = LANES / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            y[h] = c < cols ? __bfloat162float(reinterpret_cast<const bf16*>(base_s[h])[c]) + sum * scale : 0.0f;
+            y[h] = c < cols ? __bfloat162float(reinterpret_cast<const bf16*>(base_s[h])[c]) : 0.0f;
+            if (key >= 0) y[h] += sum * scale;  // without an adapter a zero keeps its sign
         }
         if constexpr (SWIGLU) y[0] = silu_times(y[0], y[1]);
         if (chunk == 0 && c < cols) p.out[row * p.cols + c0 + c] = __float2bfloat16_rn(y[0]);
