@@ -646,11 +646,12 @@ template <int RN> constexpr int expand_smem() {
 }
 
 // Two fp32 lanes in one register pair: one instruction for both.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     uint64_t x, y, z;
     asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
     asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(x), "l"(y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(z) : "l"(x), "l"(y));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(z));
     return a;
 }
@@ -665,8 +666,10 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 // silu(g) u from the hardware's exponential and reciprocal: g log2 e is rounded
 // once (|g| 2^-24), both are good to a few steps, so it is within (|g| + 8) 2^-23
-// of the value, against 2^-8 of the rounding to bf16.  Where 2^(-g log2 e) is
-// infinite the reciprocal is 0.  (With expf, a division and single lanes the
+// of the value, against 2^-8 of the rounding to bf16.  The sum 1 + e is taken a quarter
+// as large: the reciprocal of more than 2^126 would be flushed to zero, for gates between
+// -88.72 and -87.33.  Below, where e is infinite, the value is 0, as g / (1 + expf(-g)) is.
+// (With expf, a division and single lanes the
 // SwiGLU form of the expand kernel was bound by its instructions and took 1.7 times as
 // long at 4096 tokens, 8 experts, top-2.)
 __device__ __forceinline__ float2 fast_silu_times(float2 g, float2 u) {
@@ -674,10 +677,10 @@ __device__ __forceinline__ float2 fast_silu_times(float2 g, float2 u) {
     float2 e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-    e = add2(e, make_float2(1.0f, 1.0f));
+    e = fma2(e, make_float2(0.25f, 0.25f), make_float2(0.25f, 0.25f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
-    return mul2(mul2(g, r), u);
+    return mul2(mul2(mul2(g, make_float2(0.25f, 0.25f)), r), u);
 }
 
 // Stretch q of the (tile, column block) pairs: the first gridDim.x stretches cover

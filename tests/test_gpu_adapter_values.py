@@ -37,3 +37,33 @@ def test_rows_without_an_adapter_keep_the_sign_of_zero(rows):
     want = torch.empty(rows, 72, dtype=BF16, device="cuda")
     get_extension().swiglu_out(base, torch.tensor([rows], dtype=torch.int32, device="cuda"), want)
     assert torch.equal(bits(adapter_swiglu(base, x, a, b, ids)), bits(want))
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_swiglu_of_gates_whose_exponential_is_near_the_largest_number(rows):
+    """Every bf16 gate from -88.5 (e^88.5 is below the largest fp32 number) to 90.
+
+    Rows with an adapter whose product is zero; 2^-8 of the value for the rounding to
+    bf16 and (|g| + 8) 2^-23 for g log2 e rounded once, the exponential, the
+    reciprocal and the products."""
+    from moe_dispatch import adapter_swiglu
+
+    patterns = torch.arange(-2**15, 2**15, dtype=torch.int32).to(torch.int16)
+    gates = patterns.view(BF16)
+    gates = gates[(gates.float() >= -88.5) & (gates.float() <= 90.0)]
+    half = (gates.numel() + rows * 8 - 1) // (rows * 8) * 8
+    gate = torch.zeros(rows * half, dtype=BF16)
+    gate[:gates.numel()] = gates
+    gate = gate.view(rows, half)
+    for up in (1.0, -3.0, 2.0**20):
+        projection = torch.cat([gate, torch.full_like(gate, up)], 1).cuda()
+        x = torch.ones(rows, 8, dtype=BF16, device="cuda")
+        a = torch.ones(1, 1, 8, 8, dtype=BF16, device="cuda")
+        b = torch.zeros(1, 1, 2 * half, 8, dtype=BF16, device="cuda")
+        out = adapter_swiglu(projection, x, a, b, torch.zeros(rows, dtype=torch.int32, device="cuda"))
+        g = gate.double()
+        exact = g / (1.0 + torch.exp(-g)) * up
+        # half a step of bf16 is 2^-134 at least
+        bound = (2.0**-8 + 1.01 * (g.abs() + 8) * 2.0**-23) * exact.abs() + 2.0**-134
+        error = (out.double().cpu() - exact).abs()
+        assert bool((error <= bound).all()), (up, float((error / bound).max()))
