@@ -24,8 +24,8 @@
 //       few tiles with 26 small groups held everything up, 1080 us against 583 at
 //       16384 tokens, 64 experts, top-6, 32 adapters of rank 32.)
 //   shrink_tile_kernel  a tile's rows x rank, K in 128-wide cp.async stages
-//   expand_tile_kernel  a tile's rows x column blocks of 128; s enters the tensor
-//       cores as two bf16 parts (s to 2^-16), base is added in fp32
+//   expand_tile_kernel  a tile's rows x column blocks of 64; s enters the tensor
+//       cores as three bf16 parts (s to 2^-24), base is added in fp32
 // Both use mma.sync: at rank <= 64 a 64-row tile does at most 64 flop per byte
 // moved, far below what the tensor cores need to be the bound.  A tile holds one
 // adapter's rows only, so what is not finite in one adapter or row stays there.
@@ -55,7 +55,7 @@ struct Adapter {
     int32_t *table, *order, *keys;
     int32_t* tile_count;          // [0] tiles, [1] stretches claimed by the expand kernel
     int2* tiles;                  // {first sorted row, rows} of each tile
-    float* s;                     // few rows: [splits][rows][rank]; tiles: pieces (s_piece)
+    float* s;                     // few rows: [splits][rows][rank]; tiles: pieces (s_pieces)
     int splits;                   // of K
     int64_t split_k;              // K elements per split
 };
@@ -493,22 +493,29 @@ __device__ __forceinline__ uint32_t stage_at(int i, int c) { return i * kShrinkR
 
 template <int RN> constexpr int rank_k() { return RN < 16 ? 16 : RN; }
 
-// s of a sorted row as the tensor cores take it: for every 16 of its elements four
-// pieces of 16 bytes, piece q = bf16 {hi(2q, 2q + 1), hi(2q + 8, 2q + 9), lo of the same}.
-// A lane's part of an accumulator fragment is a piece, and so is its part of an operand.
-template <int RN> __device__ __forceinline__ uint4* s_piece(const Adapter& p, int64_t row, int kk, int q) {
-    return reinterpret_cast<uint4*>(p.s) + (row * (rank_k<RN>() / 16) + kk) * 4 + q;
+// s of a sorted row as the tensor cores take it: three bf16 parts, each the rest of those
+// before it, rounded, so their sum is s to 2^-24.  For every 16 of its elements four pieces
+// of 16 bytes, piece q = bf16 {hi(2q, 2q + 1), hi(2q + 8, 2q + 9), mid of the same}, and four
+// of 8, lo of the same.  A lane's part of an accumulator fragment is a piece of both, and so
+// is its part of an operand.
+constexpr int kPieceBytes = 96;
+template <int RN> __device__ __forceinline__ char* s_pieces(const Adapter& p, int64_t row, int kk) {
+    return reinterpret_cast<char*>(p.s) + (row * (rank_k<RN>() / 16) + kk) * kPieceBytes;
 }
+__device__ __forceinline__ uint4* piece_hi_mid(char* pieces, int q) { return reinterpret_cast<uint4*>(pieces) + q; }
+__device__ __forceinline__ uint2* piece_lo(char* pieces, int q) { return reinterpret_cast<uint2*>(pieces + 64) + q; }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Two floats as bf16 hi parts, and the rests' as a second register.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+// Two floats as three bf16 parts.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
     hi = pack2(a, b);
-    lo = pack2(a - bf16_lo(hi), b - bf16_hi(hi));
+    a -= bf16_lo(hi), b -= bf16_hi(hi);
+    mid = pack2(a, b);
+    lo = pack2(a - bf16_lo(mid), b - bf16_hi(mid));
 }
 
 // RN: rank rounded up to 8, 16, 32, 64 or 128; columns past the rank are zero.
@@ -624,10 +631,13 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
 #pragma unroll
                 for (int kk = 0; kk < rank_k<RN>() / 16; ++kk) {
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    split2(acc[2 * kk][2 * h] * scale, acc[2 * kk][2 * h + 1] * scale, v.x, v.z);
+                    uint2 lo = make_uint2(0, 0);
+                    split2(acc[2 * kk][2 * h] * scale, acc[2 * kk][2 * h + 1] * scale, v.x, v.z, lo.x);
                     if constexpr (RN > 8)
-                        split2(acc[2 * kk + 1][2 * h] * scale, acc[2 * kk + 1][2 * h + 1] * scale, v.y, v.w);
-                    *s_piece<RN>(p, tile.x + i, kk, lane & 3) = v;
+                        split2(acc[2 * kk + 1][2 * h] * scale, acc[2 * kk + 1][2 * h + 1] * scale, v.y, v.w, lo.y);
+                    char* const to = s_pieces<RN>(p, tile.x + i, kk);
+                    *piece_hi_mid(to, lane & 3) = v;
+                    *piece_lo(to, lane & 3) = lo;
                 }
             }
         }
@@ -642,7 +652,7 @@ constexpr int kBaseStride = kTileCols * 2 + 16;       // bytes; the pads keep ld
 template <int RN> constexpr int b_stride() { return rank_k<RN>() * 2 + 16; }
 template <int RN> constexpr int expand_ctas() { return RN <= 32 ? 6 : (RN <= 64 ? 4 : 2); }  // per SM
 template <int RN> constexpr int expand_smem() {
-    return kExpandStages * (kTileRows * kBaseStride + kTileCols * b_stride<RN>());
+    return kExpandStages * (kTileRows * kBaseStride + kTileCols * b_stride<RN>()) + rank_k<RN>() / 16 * kExpandThreads * 16;
 }
 
 // Two fp32 lanes in one register pair: one instruction for both.
@@ -711,8 +721,9 @@ __device__ __forceinline__ Stretch stretch_of(int64_t q, int64_t all) {
 // (one share per CTA took 1.6 times as long at 4096 tokens, 8 experts of 14336,
 // top-2), and short stretches alone pay for many starts.  A CTA's blocks of one
 // tile form one cp.async pipeline whose stages hold the tile's base rows and the
-// pair's rows of B; s stays in registers as bf16 fragments, and the accumulators
-// start from base.
+// pair's rows of B; s stays as bf16 fragments in registers (hi and mid) and in shared
+// memory (lo, written and read by the same lane: the registers decide how many CTAs an SM
+// holds), and the accumulators start from base.
 //
 // Measured: 163-168 us at that size (8192 rows -> 2 x 14336, rank 16: 710 MB through
 // memory in this kernel, 108 us), 259-262 at 98304 rows of 2 x 1408, 2048 pairs, rank 32.
@@ -745,6 +756,7 @@ expand_tile_kernel(const Adapter p, int blocks) {
     constexpr int kPieces = kOut / 8, kPer = 32 / kPieces;  // out: 16-byte pieces of a row; rows at a time
     const int out_row = warp * 16 + lane / kPieces, out_col = (lane % kPieces) * 8;
     const int out_lane = out_row * kBaseStride + out_col * 2;
+    uint4* const lo_s = reinterpret_cast<uint4*>(smem + kExpandStages * kStage) + tid;  // [kk][thread]
     if (b_q * 8 >= p.rank) {  // past the rank B is zero: written once, never copied over
 #pragma unroll
         for (int s = 0; s < kExpandStages; ++s)
@@ -814,17 +826,22 @@ expand_tile_kernel(const Adapter p, int blocks) {
         }
 
         // s of this warp's 16 rows as fragments
-        uint32_t hi[RK / 16][4] = {}, lo[RK / 16][4] = {};
+        uint32_t hi[RK / 16][4] = {}, mid[RK / 16][4] = {};
         if (key >= 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (r0 + 8 * h < tile.y) {
+            for (int kk = 0; kk < RK / 16; ++kk) {
+                uint32_t lo[4] = {};
 #pragma unroll
-                    for (int kk = 0; kk < RK / 16; ++kk) {
-                        const uint4 v = *s_piece<RN>(p, static_cast<int64_t>(tile.x) + r0 + 8 * h, kk, lane & 3);
-                        hi[kk][h] = v.x, hi[kk][2 + h] = v.y, lo[kk][h] = v.z, lo[kk][2 + h] = v.w;
+                for (int h = 0; h < 2; ++h)
+                    if (r0 + 8 * h < tile.y) {
+                        char* const from = s_pieces<RN>(p, static_cast<int64_t>(tile.x) + r0 + 8 * h, kk);
+                        const uint4 v = *piece_hi_mid(from, lane & 3);
+                        const uint2 w = *piece_lo(from, lane & 3);
+                        hi[kk][h] = v.x, hi[kk][2 + h] = v.y, mid[kk][h] = v.z, mid[kk][2 + h] = v.w;
+                        lo[h] = w.x, lo[2 + h] = w.y;
                     }
-                }
+                lo_s[kk * kExpandThreads] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
         }
 
         uint32_t stage = 0;
@@ -857,16 +874,21 @@ expand_tile_kernel(const Adapter p, int blocks) {
                                     acc[g][q][2 * h] = bf16_lo(v), acc[g][q][2 * h + 1] = bf16_hi(v);
                                 }
 #pragma unroll
-                        for (int g = 0; g < kHalves; ++g)
+                        for (int kk = 0; kk < RK / 16; ++kk) {
+                            const uint4 w = lo_s[kk * kExpandThreads];
+                            const uint32_t lo[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                            for (int kk = 0; kk < RK / 16; ++kk) {
+                            for (int g = 0; g < kHalves; ++g) {
                                 uint32_t bf[4];
                                 ldmatrix4(bs + (f + g * 32) * b_stride<RN>() + kk * 32, bf);
-                                mma16816(acc[g][0], lo[kk], bf[0], bf[1]);
-                                mma16816(acc[g][1], lo[kk], bf[2], bf[3]);
+                                mma16816(acc[g][0], lo, bf[0], bf[1]);
+                                mma16816(acc[g][1], lo, bf[2], bf[3]);
+                                mma16816(acc[g][0], mid[kk], bf[0], bf[1]);
+                                mma16816(acc[g][1], mid[kk], bf[2], bf[3]);
                                 mma16816(acc[g][0], hi[kk], bf[0], bf[1]);
                                 mma16816(acc[g][1], hi[kk], bf[2], bf[3]);
                             }
+                        }
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -992,7 +1014,7 @@ Shape shape_of(int64_t rows, int64_t k, int rank, int adapters, int experts, int
     f.keys = f.order + round256(rows * 4);
     f.tiles = f.keys + round256(rows * 4);
     f.s = f.tiles + round256(rows * 8 + 256);  // the count, then at most one tile per row
-    f.total = f.s + round256(rows * (padded_rank(rank) < 16 ? 16 : padded_rank(rank)) * 4);
+    f.total = f.s + round256(rows * (padded_rank(rank) < 16 ? 1 : padded_rank(rank) / 16) * kPieceBytes);
     return f;
 }
 

@@ -212,7 +212,7 @@ int moe_grouped_gemm(const void* a, const void* weight, const int32_t* offsets, 
  * NULL: one expert with every row.  base, out [rows, n_cols] (out may be base itself, and must not
  * overlap any operand otherwise); x [rows, k_dim]; a [adapters, experts, rank,
  * k_dim]; b [adapters, experts, n_cols, rank]; scale [adapters] fp32 or NULL (1).
- * x . a^T is summed in fp32 and used to 2^-16 of its value or better; one
+ * x . a^T is summed in fp32 and used to 2^-24 of its value; one
  * rounding to bf16 at the end.  What is not finite in one adapter or row does
  * not reach rows of others.  k_dim (<= 2^26), n_cols multiples of 8; rank a multiple of 8
  * up to 128; adapters <= 512.  scratch: 256-byte aligned, not initialised, sized

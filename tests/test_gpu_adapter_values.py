@@ -67,3 +67,35 @@ def test_swiglu_of_gates_whose_exponential_is_near_the_largest_number(rows):
         bound = (2.0**-8 + 1.01 * (g.abs() + 8) * 2.0**-23) * exact.abs() + 2.0**-134
         error = (out.double().cpu() - exact).abs()
         assert bool((error <= bound).all()), (up, float((error / bound).max()))
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("rank", [8, 16, 24, 64, 128])
+def test_the_inner_product_enters_in_fp32(rows, rank):
+    """s = (1 + 2^-9 + 2^-18, 1 + 2^-9, 0, ...) and B = (1, -1, ...): 2^-18 is left.
+
+    Every product and partial sum is a multiple of 2^-18 below 4 (times a power of
+    two that the row and the column share), so nothing is ever rounded."""
+    from moe_dispatch import adapter_add, adapter_swiglu
+
+    k, n = 136, 80
+    row = torch.exp2((torch.arange(rows) % 3).float())
+    column = torch.exp2((torch.arange(n) % 4).float())
+    x = torch.zeros(rows, k)
+    x[:, 1], x[:, 50], x[:, 135] = row, 2.0**-9 * row, 2.0**-18 * row
+    a = torch.zeros(1, 1, rank, k)
+    a[0, 0, 0], a[0, 0, 1, :135] = 1.0, 1.0
+    b = torch.zeros(1, 1, n, rank)
+    b[0, 0, :, 0], b[0, 0, :, 1] = column, -column
+    ids = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    x, a, b = (t.to(BF16).cuda() for t in (x, a, b))
+    want = 2.0**-18 * row[:, None] * column
+    out = adapter_add(torch.zeros(rows, n, dtype=BF16, device="cuda"), x, a, b, ids)
+    assert torch.equal(out.float().cpu(), want)
+
+    base = torch.zeros(rows, 2 * n, dtype=BF16, device="cuda")
+    base[:, :n] = 4.0
+    b = torch.cat([torch.zeros_like(b), b], 2)
+    out = adapter_swiglu(base, x, a, b, ids)
+    exact = 4.0 / (1.0 + torch.exp(torch.tensor(-4.0, dtype=torch.float64))) * want.double()
+    assert bool(((out.double().cpu() - exact).abs() <= (2.0**-8 + 12 * 2.0**-23) * exact).all())
