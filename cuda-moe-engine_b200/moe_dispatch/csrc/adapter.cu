@@ -493,8 +493,9 @@ __device__ __forceinline__ uint32_t stage_at(int i, int c) { return i * kShrinkR
 
 template <int RN> constexpr int rank_k() { return RN < 16 ? 16 : RN; }
 
-// s of a sorted row as the tensor cores take it: three bf16 parts, each the rest of those
-// before it, rounded, so their sum is s to 2^-24.  For every 16 of its elements four pieces
+// s of a sorted row as the tensor cores take it: three bf16 parts, each the leading eight
+// bits of what those before it leave, so their sum is s.  An infinity is the first part alone
+// (and its product what the formula says), as no part of a finite s is infinite.  For every 16 of its elements four pieces
 // of 16 bytes, piece q = bf16 {hi(2q, 2q + 1), hi(2q + 8, 2q + 9), mid of the same}, and four
 // of 8, lo of the same.  A lane's part of an accumulator fragment is a piece of both, and so
 // is its part of an operand.
@@ -512,10 +513,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // Two floats as three bf16 parts.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-    hi = pack2(a, b);
-    a -= bf16_lo(hi), b -= bf16_hi(hi);
-    mid = pack2(a, b);
-    lo = pack2(a - bf16_lo(mid), b - bf16_hi(mid));
+    const auto take = [&] {
+        const uint32_t x = __float_as_uint(a) & 0xffff0000u, y = __float_as_uint(b) & 0xffff0000u;
+        a = fabsf(a) < INFINITY ? a - __uint_as_float(x) : 0.0f;
+        b = fabsf(b) < INFINITY ? b - __uint_as_float(y) : 0.0f;
+        return x >> 16 | y;
+    };
+    hi = take(), mid = take(), lo = take();
 }
 
 // RN: rank rounded up to 8, 16, 32, 64 or 128; columns past the rank are zero.
@@ -632,9 +636,11 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
                 for (int kk = 0; kk < rank_k<RN>() / 16; ++kk) {
                     uint4 v = make_uint4(0, 0, 0, 0);
                     uint2 lo = make_uint2(0, 0);
-                    split2(acc[2 * kk][2 * h] * scale, acc[2 * kk][2 * h + 1] * scale, v.x, v.z, lo.x);
+                    if (kk * 16 < p.rank)  // past the rank: zeros, not an infinite x times a zero
+                        split2(acc[2 * kk][2 * h] * scale, acc[2 * kk][2 * h + 1] * scale, v.x, v.z, lo.x);
                     if constexpr (RN > 8)
-                        split2(acc[2 * kk + 1][2 * h] * scale, acc[2 * kk + 1][2 * h + 1] * scale, v.y, v.w, lo.y);
+                        if (kk * 16 + 8 < p.rank)
+                            split2(acc[2 * kk + 1][2 * h] * scale, acc[2 * kk + 1][2 * h + 1] * scale, v.y, v.w, lo.y);
                     char* const to = s_pieces<RN>(p, tile.x + i, kk);
                     *piece_hi_mid(to, lane & 3) = v;
                     *piece_lo(to, lane & 3) = lo;

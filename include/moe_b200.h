@@ -214,7 +214,8 @@ int moe_grouped_gemm(const void* a, const void* weight, const int32_t* offsets, 
  * k_dim]; b [adapters, experts, n_cols, rank]; scale [adapters] fp32 or NULL (1).
  * x . a^T is summed in fp32 and used to 2^-24 of its value; one
  * rounding to bf16 at the end.  What is not finite in one adapter or row does
- * not reach rows of others.  k_dim (<= 2^26), n_cols multiples of 8; rank a multiple of 8
+ * not reach rows of others; an infinite x . a^T gives the infinities of the
+ * formula, an infinite element of b may give NaN where the formula has one.  k_dim (<= 2^26), n_cols multiples of 8; rank a multiple of 8
  * up to 128; adapters <= 512.  scratch: 256-byte aligned, not initialised, sized
  * for the current device; calls that may overlap in time need one each. */
 int64_t moe_adapter_scratch_bytes(int64_t rows, int64_t k_dim, int32_t rank, int32_t adapters,

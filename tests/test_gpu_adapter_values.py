@@ -99,3 +99,38 @@ def test_the_inner_product_enters_in_fp32(rows, rank):
     out = adapter_swiglu(base, x, a, b, ids)
     exact = 4.0 / (1.0 + torch.exp(torch.tensor(-4.0, dtype=torch.float64))) * want.double()
     assert bool(((out.double().cpu() - exact).abs() <= (2.0**-8 + 12 * 2.0**-23) * exact).all())
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 72, 128])
+def test_infinite_and_very_large_inner_products(rows, rank):
+    """An infinite s gives the infinity of the formula (a, b, up > 0: no inf - inf, no 0 inf), and an s
+    past the largest bf16 value is still a number."""
+    from moe_dispatch import adapter_add, adapter_swiglu
+
+    g = torch.Generator().manual_seed(rank)
+    k, n = 264, 72
+    x = torch.rand(rows, k, generator=g)
+    x[7, 5] = float("inf")
+    x[20, 5] = -float("inf")
+    x[33] = 0.0
+    x[33, 0], x[33, 1] = 2.0**127, 2.0**127
+    a = torch.rand(2, 1, rank, k, generator=g) + 0.5
+    a[:, :, :, 0], a[:, :, :, 1] = 0.0, 0.0
+    a[:, :, 0, 0], a[:, :, 0, 1] = 1.0, 1.0 - 2.0**-8  # s[33] = (2^127 (2 - 2^-8), 0, ...): a tie, up to infinity in bf16
+    b = torch.rand(2, 1, n, rank, generator=g) + 0.5
+    b[:, :, :, 0] = 2.0**-20
+    ids = (torch.arange(rows) % 2).to(torch.int32)
+    x, a, b = (t.to(BF16).cuda() for t in (x, a, b))
+    out = adapter_add(torch.ones(rows, n, dtype=BF16, device="cuda"), x, a, b, ids.cuda()).cpu()
+    assert bool((out[7] == float("inf")).all()) and bool((out[20] == -float("inf")).all())
+    assert bool((out[33] == 2.0**108).all())  # 2^107 (2 - 2^-8), rounded to bf16
+    rest = torch.ones(rows, dtype=torch.bool)
+    rest[[7, 20]] = False
+    assert bool(torch.isfinite(out[rest]).all())
+
+    base = torch.ones(rows, 2 * n, dtype=BF16, device="cuda")
+    b = torch.cat([b, torch.full_like(b, 2.0**-20)], 2)
+    out = adapter_swiglu(base, x, a, b, ids.cuda()).cpu()
+    rest[33] = False                             # its gate times its up is past the largest number
+    assert bool((out[7] == float("inf")).all()) and bool(torch.isfinite(out[rest]).all())
