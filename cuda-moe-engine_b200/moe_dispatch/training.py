@@ -203,9 +203,14 @@ def route_backward(x, router_weight, expert_ids, weights, grad_weights, grad_log
     [T,K] and ``grad_logits`` [T,E] (optional) the fp32 gradients of its outputs:
     with ds = weights * (grad_weights - sum_k weights * grad_weights) and
     d = grad_logits + ds at the ids, grad_x = d router_weight (rounded once) and
-    grad_router_weight = d^T x to fp32 accuracy.
+    grad_router_weight = d^T x, both products to fp32 accuracy.  The results carry no
+    graph: with gradients enabled, inputs that require them are refused.
     """
     _check_router(x, router_weight)
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad
+            for t in (x, router_weight, weights, grad_weights, grad_logits)):
+        raise ValueError("route_backward has no gradient of its own; detach inputs or use no_grad")
     tokens, experts = x.shape[0], router_weight.shape[0]
     _check_ids(expert_ids, tokens, x)
     for name, tensor, shape in (("weights", weights, expert_ids.shape),
