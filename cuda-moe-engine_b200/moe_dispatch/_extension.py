@@ -387,6 +387,7 @@ class Extension:
     def balance_loss_backward_out(self, logits, bias, token_mask, counts, counted, grad_loss,
                                   coefficient, topk, grad_logits):
         """d loss / d logits times the scalar grad_loss (include/moe_b200.h)."""
+        _require(grad_logits is not None, "expected grad_logits[T,E]")
         tokens, experts = self._balance_checks(logits, bias, token_mask, grad_logits)
         for tensor in (counts, counted, grad_loss):
             _check_cuda(tensor, logits, "balance_loss")
