@@ -485,6 +485,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 constexpr int kShrinkStages = 3;
 constexpr int kShrinkK = 128;                   // K elements per stage: 256 bytes of each row
 constexpr int kShrinkRow = kShrinkK * 2;
+// The tensor cores cut a sum off below the accumulator's last bit at every MMA, so long sums
+// drift (s of K = 14336 lost 1e-4 of a sum whose first term is the largest).  After this many
+// stages (256 elements, 16 MMAs) an accumulator is added to an fp32 sum, rounded to nearest.
+constexpr int kShrinkChunk = 2;
 template <int RN> constexpr int shrink_stage_bytes() { return (kTileRows + RN) * kShrinkRow; }
 
 // 16-byte chunk c of row i of a stage: the low three bits are swizzled by the
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
             if (s < steps) load(s, s);
             copy_commit();
         }
-        float acc[RN / 8][4] = {};
+        float acc[RN / 8][4] = {}, sum[RN / 8][4] = {};
         int slot = 0, load_slot = kShrinkStages - 1;
         for (int step = 0; step < steps; ++step) {
             copy_wait<kShrinkStages - 2>();
@@ -602,10 +606,19 @@ __global__ void __launch_bounds__(kTileThreads) shrink_tile_kernel(const Adapter
                         }
                     }
                 }
+                if (step % kShrinkChunk == kShrinkChunk - 1) {
+#pragma unroll
+                    for (int j = 0; j < kRegs; ++j) {
+                        sum[j / 4][j % 4] += acc[j / 4][j % 4];
+                        acc[j / 4][j % 4] = 0.0f;
+                    }
+                }
             }
             if (++slot == kShrinkStages) slot = 0;
             if (++load_slot == kShrinkStages) load_slot = 0;
         }
+#pragma unroll
+        for (int j = 0; j < kRegs; ++j) acc[j / 4][j % 4] += sum[j / 4][j % 4];
         bool mine = warp * 16 < tile.y;
         if (splits > 1) {
             float* partial = reinterpret_cast<float*>(stages) + warp * kRegs * 32 + lane;  // [warp][register][lane]

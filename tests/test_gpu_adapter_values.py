@@ -134,3 +134,27 @@ def test_infinite_and_very_large_inner_products(rows, rank):
     out = adapter_swiglu(base, x, a, b, ids.cuda()).cpu()
     rest[33] = False                             # its gate times its up is past the largest number
     assert bool((out[7] == float("inf")).all()) and bool(torch.isfinite(out[rest]).all())
+
+
+@pytest.mark.parametrize("rows", ROWS + [12000])
+def test_small_terms_of_a_long_inner_product_are_not_lost(rows):
+    """s = 1 + (K - 1) 7 2^-30, base = -1, b = 1: what is left are the small terms, 7/8 of 2^-23 per 16.
+
+    A sum that stands at 1 may lose the terms of 256 elements (16 cuts of at most 2^-23); then
+    half a step (2^-24) for each of at most K / 256 + 8 additions, and three cuts of 2^-23 for the
+    parts of s in the second product."""
+    from moe_dispatch import adapter_add
+
+    k, rank = 14336, 16
+    a = torch.zeros(1, 1, rank, k)
+    a[0, 0, 0] = 7 * 2.0**-30
+    a[0, 0, 0, 0] = 1.0
+    b = torch.zeros(1, 1, 8, rank)
+    b[..., 0] = 1.0
+    x = torch.ones(rows, k, dtype=BF16, device="cuda")
+    base = torch.full((rows, 8), -1.0, dtype=BF16, device="cuda")
+    out = adapter_add(base, x, a.to(BF16).cuda(), b.to(BF16).cuda(), torch.zeros(rows, dtype=torch.int32, device="cuda"))
+    exact = (k - 1) * 7 * 2.0**-30
+    bound = 19 * 2.0**-23 + (k // 256 + 8) * 2.0**-24 + 2.0**-8 * exact
+    error = float((out.double() - exact).abs().max())
+    assert error <= bound, error / bound
