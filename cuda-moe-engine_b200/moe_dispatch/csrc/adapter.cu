@@ -744,12 +744,15 @@ __device__ __forceinline__ Stretch stretch_of(int64_t q, int64_t all) {
 // memory (lo, written and read by the same lane: the registers decide how many CTAs an SM
 // holds), and the accumulators start from base.
 //
-// Measured: 163-168 us at that size (8192 rows -> 2 x 14336, rank 16: 710 MB through
-// memory in this kernel, 108 us), 259-262 at 98304 rows of 2 x 1408, 2048 pairs, rank 32.
-// Bound by instruction issue (58 %) and the warps' dependent chains.  Four warps a CTA
-// and six CTAs an SM, because a barrier then holds up 64 columns and not 128 (175 and
-// 300 us with eight warps).  B in the warps' registers instead of shared memory, with no
-// barrier: 180 and 376.  Three stages: the same as two.
+// Measured (a call less the same call with 8 columns): 172 us at that size (8192 rows
+// -> 2 x 14336, rank 16: 710 MB through memory in this kernel, 108 us), 305 at 98304 rows
+// of 2 x 1408, 2048 pairs, rank 32.  No unit is saturated (instruction issue 51-56 %, DRAM
+// 42-49 %, tensor cores 13-35 %): the warps wait for their own chains and at the barrier.
+// Five CTAs an SM at rank 32 or three at rank 64, with lo in registers' reach: the same or
+// slower.  Measured with two parts of s (160 and 280 us): four warps a CTA and six CTAs an
+// SM, because a barrier then holds up 64 columns and not 128 (4 and 20 us more with eight
+// warps); B in the warps' registers instead of shared memory, with no barrier, 9 and 96
+// more; three stages the same as two.
 template <int RN, bool SWIGLU>
 __global__ void __launch_bounds__(kExpandThreads, expand_ctas<RN>())
 expand_tile_kernel(const Adapter p, int blocks) {
@@ -982,11 +985,15 @@ int padded_rank(int rank) {
 }
 
 // Which form.  Measured in graphs (us, few-rows form / tiles), 8 experts, rank 16, down
-// projection 14336 -> 4096: one adapter, 128 rows 13 / 25, 256 rows 22 / 28, 512 rows
-// 41 / 31, 1024 rows 77 / 35; 64 adapters, a row's own each, 512 rows 47 / 125, 1024 rows
-// 83 / 140, 2048 rows 156 / 160.  (Rank 8 to 128 and 4096 -> 28672 cross over near the
-// same places.)  Where the rows are no more than twice the pairs that they may fall
-// on, tiles would hold few rows each.
+// projection 14336 -> 4096: one adapter, 128 rows 13 / 25, 264 rows 23 / 27, 512 rows
+// 40 / 30, 1024 rows 77 / 32; 64 adapters, a row's own each, 264 rows 28 / 83, 512 rows
+// 47 / 111, 1024 rows 83 / 137, 2048 rows 156 / 160.  (Rank 8 to 128 and 4096 -> 28672
+// cross over near the same places.)  Where the rows are no more than twice the pairs that
+// they may fall on, tiles may hold few rows each.
+// The rule goes by what the host knows, the rows' capacity and the adapters loaded, not by
+// the rows and pairs in use, which only the device knows.  It costs most where many
+// adapters are loaded and all rows use one: 64 loaded, 512 rows 40 / 30, 1024 rows 77 / 33;
+// and a few tokens over very many experts, whose padded spans count as rows, take tiles.
 constexpr int64_t kFewRows = 256;
 constexpr int64_t kFewRowsScattered = 1024;
 bool few_rows_form(int64_t rows, int adapters, int experts) {

@@ -185,7 +185,9 @@ def route(x, router_weight, *, bias=None, topk=2):
     scores) and logits [T,E] fp32 (without the bias): the bits of
     ``MoEBlock.route`` and ``MoEBlock.logits``.  Gradients of the weights and of
     the logits (of ``balance_loss``, say) reach x as bf16 and router_weight as
-    fp32 through ``route_backward``.
+    fp32 through ``route_backward``.  The experts and the combine are forward-only:
+    the gradient of the routing weights comes from the caller's own combination of
+    expert outputs.
     """
     _check_router(x, router_weight)
     experts = router_weight.shape[0]
