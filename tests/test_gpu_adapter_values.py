@@ -158,3 +158,22 @@ def test_small_terms_of_a_long_inner_product_are_not_lost(rows):
     bound = 19 * 2.0**-23 + (k // 256 + 8) * 2.0**-24 + 2.0**-8 * exact
     error = float((out.double() - exact).abs().max())
     assert error <= bound, error / bound
+
+
+@pytest.mark.parametrize("rows", [5500, 6500, 7300, 8190, 8192, 8193])
+def test_every_size_of_the_sorting_cluster(rows):
+    """6 to 8 chunks of rows in one cluster, the most adapters, and the first size past it: x A^T B^T of
+    small whole numbers, so every sum is exact."""
+    from moe_dispatch import adapter_add
+
+    g = torch.Generator().manual_seed(rows)
+    adapters, k, n, rank = 512, 16, 8, 8
+    x = torch.randint(-2, 3, (rows, k), generator=g).float()
+    a = torch.randint(-1, 2, (adapters, 1, rank, k), generator=g).float()
+    b = torch.randint(-1, 2, (adapters, 1, n, rank), generator=g).float()
+    base = torch.randint(-4, 5, (rows, n), generator=g).float()
+    ids = torch.randint(-1, adapters, (rows,), generator=g)
+    s = torch.einsum("rk,rjk->rj", x, a[ids.clamp_min(0), 0])
+    want = base + (ids >= 0)[:, None] * torch.einsum("rj,rnj->rn", s, b[ids.clamp_min(0), 0])
+    out = adapter_add(*(t.to(BF16).cuda() for t in (base, x, a, b)), ids.cuda())
+    assert torch.equal(out.cpu(), want.to(BF16))  # integers below 2^24, rounded once

@@ -39,3 +39,16 @@ def test_one_gradient_alone(tokens, hidden, experts, topk, with_logits):
     ext.route_backward_out(*problem, None, out)
     assert torch.equal(out, dw) and bool((buffer[dw.numel():] == -77.0).all())
     assert ext.device_status() == 0
+
+
+@pytest.mark.parametrize("experts", [8, 40, 200])
+def test_route_of_no_tokens(experts):
+    from moe_dispatch import balance_loss, route
+
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    weight = torch.randn(experts, 64, device="cuda", requires_grad=True)
+    ids, weights, logits = route(x, weight, topk=2)
+    loss, counts = balance_loss(logits, ids)
+    grad_x, grad_weight = torch.autograd.grad(weights.sum() + loss, (x, weight))
+    assert ids.shape == (0, 2) and grad_x.shape == (0, 64) and loss.item() == 0.0
+    assert not counts.any() and grad_weight.shape == (experts, 64) and not grad_weight.any()
